@@ -18,10 +18,12 @@ AETHER_GEMM_WIDE_STORE = 1
 AETHER_ATTN_EXACT_MAX = 32    # attention: conservative path only (true-maximum shift from tile 0, a-posteriori check per tile)
 AETHER_VAE_TWO_LANES = 256    # VAE plan: tile batches of two on two streams (see include/aether_hip.h)
 AETHER_CONV_TAP_REUSE = 128   # conv: K order is (dt, dh, channel block, dw) -> the tap-reuse kernel may be used
+AETHER_STREAM_BF16 = 0         # type of a residual stream (rms_norm)
+AETHER_STREAM_FP32 = 1
 ATTN_Q_SCALE = 0.125 * 1.4426950408889634   # softmax scale x log2(e): the attention kernel works in the log2 domain
 PROF_CLASSES = ["other", "layernorm", "gemm_qkv", "qk_norm_rope", "attention", "gemm_out", "gemm_ff1", "gemm_ff2"]
 
-_vp, _i, _f, _fp, _sz = C.c_void_p, C.c_int, C.c_float, C.c_void_p, C.c_size_t
+_vp, _i, _f, _fp, _sz, _l = C.c_void_p, C.c_int, C.c_float, C.c_void_p, C.c_size_t, C.c_long
 
 
 class AetherDitConfig(C.Structure):
@@ -54,6 +56,10 @@ SIGNATURES = {
     "aether_unpatchify": (_i, [_vp, _i, _vp, _i, _i, _i, _i, _i, _i, _vp]),
     "aether_qk_norm_rope": (_i, [_vp, _i, _i, _i, _i, _fp, _fp, _fp, _fp, _f, _fp, _fp, _f, _vp, _vp, _vp, _i, _vp]),
     "aether_flash_attn_fwd": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
+    "aether_rms_norm": (_i, [_vp, _i, _l, _vp, _l, _vp, _l, _fp, _f, _vp, _l, _fp, _i, _i, _vp]),
+    "aether_rms_norm_bwd_workspace_bytes": (_sz, [_i, _i]),
+    "aether_rms_norm_bwd": (_i, [_vp, _l, _vp, _i, _l, _vp, _l, _fp, _f, _vp, _l, _vp, _l, _fp, _i, _i, _vp, _sz, _vp]),
+    "aether_quantize_rows_e4m3": (_i, [_vp, _l, _vp, _l, _fp, _i, _i, _vp]),
     "aether_dpm_step": (_i, [_vp, _i, _f, _vp, _fp, _vp, _f, _f, _f, _f, _f, _f, _f, _fp, _fp, _vp, C.c_long, _vp]),
     "aether_conv_gemm_bf16": (_i, [_vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _i, _vp, _i, _vp, _i, _fp, _vp, _i, _fp, _sz, _i, _vp]),
     "aether_im2col_first": (_i, [_vp, C.c_long, C.c_long, C.c_long, C.c_long, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _i, _vp]),
@@ -133,3 +139,10 @@ def current_stream():
     import torch
 
     return torch.cuda.current_stream().cuda_stream
+
+
+def stream_of(index: int):
+    """torch's current stream on device `index` as a hipStream_t (the raw query: no Stream object per call)."""
+    import torch
+
+    return torch._C._cuda_getCurrentRawStream(index)

@@ -123,3 +123,131 @@ def flash_attn_fwd(Qh, Kh, Vt, flags=0):
     rc = _lib.load().aether_flash_attn_fwd(_lib.ptr(Qh), _lib.ptr(Kh), _lib.ptr(Vt), _lib.ptr(O), B, H, S, Spad, flags, _lib.current_stream())
     _lib.check(rc, "aether_flash_attn_fwd")
     return O
+
+
+# ---- the text encoder's operators ------------------------------------------------------------------------------------
+# These take tensors of any leading shape, strides and device (another device than the current one included: the call runs on that
+# device's current stream), and refuse what they do not compute with ValueError before anything is enqueued.
+
+
+def _same_device(first, *others):
+    """The device of the call.  Every operand lives there."""
+    _need_cuda(first, *others)
+    dev = first.device
+    for t in others:
+        if t is not None and t.device != dev:
+            raise ValueError(f"operands are on different devices: {dev} and {t.device}")
+    return dev
+
+
+def _run(what, dev, fn, *args):
+    """fn(*args, stream) on `dev` and its current stream."""
+    if dev.index == torch.cuda.current_device():
+        rc = fn(*args, _lib.stream_of(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _lib.stream_of(dev.index))
+    if rc:
+        _lib.check(rc, what)
+
+
+def _rows(t, width, align=16):
+    """`t` as [rows, width] with unit stride, a row stride of whole 16-byte pieces (8 elements) and an aligned base; copied only where it is not so."""
+    if t.dim() != 2:
+        t = t.reshape(-1, width)
+    by, one = t.stride()
+    if one != 1 or by % 8 or (by < width and t.shape[0] > 1) or t.data_ptr() % align:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _vector(t):
+    """A 1-d operand with unit stride and a 16-byte aligned base; copied only where it is not so."""
+    return t if t.stride(0) == 1 and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+_STREAMS = {torch.bfloat16: _lib.AETHER_STREAM_BF16, torch.float32: _lib.AETHER_STREAM_FP32}
+
+
+def _norm_operands(x, w, delta, name):
+    if not (x.dtype in _STREAMS):
+        raise ValueError(f"{name}: the stream is bfloat16 or float32, got {x.dtype}")
+    if not (x.dim() >= 1 and x.shape[-1] > 0):
+        raise ValueError(f"{name}: the stream has no last dimension")
+    D = x.shape[-1]
+    if not (w.dtype == torch.float32 and tuple(w.shape) == (D,)):
+        raise ValueError(f"{name}: the weight is float32 [{D}], got {w.dtype} {list(w.shape)}")
+    if delta is not None:
+        if not (delta.dtype == torch.bfloat16 and delta.shape == x.shape):
+            raise ValueError(f"{name}: delta is bfloat16 {list(x.shape)}, got {delta.dtype} {list(delta.shape)}")
+    return D
+
+
+def _rms_norm(x, w, eps, delta, e4m3):
+    name = "rms_norm_e4m3" if e4m3 else "rms_norm"
+    dev = _same_device(x, w, delta)
+    D = _norm_operands(x, w, delta, name)
+    x2, w = _rows(x, D), _vector(w)
+    rows = x2.shape[0]
+    y = torch.empty(x.shape, dtype=torch.float8_e4m3fn if e4m3 else torch.bfloat16, device=dev)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev) if e4m3 else None
+    if delta is None:
+        d2, res = None, None
+    else:
+        d2, res = _rows(delta, D), torch.empty(x.shape, dtype=x.dtype, device=dev)
+    if rows:
+        _run(name, dev, _lib.load().aether_rms_norm, x2.data_ptr(), _STREAMS[x.dtype], x2.stride(0), _lib.ptr(d2), d2.stride(0) if d2 is not None else 0,
+             _lib.ptr(res), D, w.data_ptr(), float(eps), y.data_ptr(), D, _lib.ptr(scale), rows, D)
+    return y, scale, x if res is None else res
+
+
+def rms_norm(x, w, eps=1e-6, delta=None):
+    """h = x + delta;  y = h (mean(h²) + eps)^-1/2 w over the last dimension.  x: the residual stream [..., D], bfloat16 or float32; delta: a block's
+    output, bfloat16 [..., D], or None; w float32 [D]; D a multiple of 8 up to 16384.  -> (y bfloat16, h in the stream's type; x itself without
+    delta).  Statistics in fp32 of the unrounded sum."""
+    y, _, res = _rms_norm(x, w, eps, delta, False)
+    return y, res
+
+
+def rms_norm_e4m3(x, w, eps=1e-6, delta=None):
+    """`rms_norm` with its output in 8 bits -> (q float8_e4m3fn, scale float32 [...], h):  y ≈ q · scale with one power of two per row, the smallest
+    one that brings the row into ±448.  A row that holds an infinity or a NaN becomes NaN (scale and values)."""
+    return _rms_norm(x, w, eps, delta, True)
+
+
+def rms_norm_backward(dy, res, w, eps=1e-6, dres=None, need_ddelta=False):
+    """Gradients of `rms_norm` from its stored h (`res`): dy bfloat16 [..., D] for y, dres (the stream's type) for h or None.
+    -> (dx in the stream's type, ddelta bfloat16 or None, dw float32 [D]).  Summed in an order that depends on the sizes alone."""
+    dev = _same_device(res, dy, w, dres)
+    D = _norm_operands(res, w, dy, "rms_norm_backward")
+    if dres is not None:
+        if not (dres.dtype == res.dtype and dres.shape == res.shape):
+            raise ValueError(f"rms_norm_backward: dres is {res.dtype} {list(res.shape)}, got {dres.dtype} {list(dres.shape)}")
+    r2, g2, w = _rows(res, D), _rows(dy, D), _vector(w)
+    s2 = None if dres is None else _rows(dres, D)
+    rows = r2.shape[0]
+    dx = torch.empty(res.shape, dtype=res.dtype, device=dev)
+    # with a bf16 stream the rounded dx IS ddelta
+    ddelta = torch.empty(res.shape, dtype=torch.bfloat16, device=dev) if need_ddelta and res.dtype != torch.bfloat16 else None
+    dw = torch.empty(D, dtype=torch.float32, device=dev)
+    lib = _lib.load()
+    nbytes = lib.aether_rms_norm_bwd_workspace_bytes(rows, D)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _run("rms_norm_backward", dev, lib.aether_rms_norm_bwd, g2.data_ptr(), g2.stride(0), r2.data_ptr(), _STREAMS[res.dtype], r2.stride(0),
+         _lib.ptr(s2), s2.stride(0) if s2 is not None else 0, w.data_ptr(), float(eps), dx.data_ptr(), D, _lib.ptr(ddelta), D, dw.data_ptr(), rows, D,
+         ws.data_ptr(), nbytes)
+    return dx, (dx if res.dtype == torch.bfloat16 else ddelta) if need_ddelta else None, dw
+
+
+def quantize_rows_e4m3(x):
+    """x bfloat16 [rows, K] (K a multiple of 8) -> (q float8_e4m3fn [rows, K], scale float32 [rows]), x ≈ q · scale: a weight matrix in the form
+    `gated_ff_e4m3` takes (one power of two per row, as `rms_norm_e4m3`)."""
+    dev = _same_device(x)
+    if not (x.dtype == torch.bfloat16 and x.dim() == 2):
+        raise ValueError(f"quantize_rows_e4m3: bfloat16 [rows, K], got {x.dtype} {list(x.shape)}")
+    x2 = _rows(x, x.shape[1]) if x.numel() else x
+    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=dev)
+    scale = torch.empty(x.shape[0], dtype=torch.float32, device=dev)
+    if x.shape[0]:
+        _run("quantize_rows_e4m3", dev, _lib.load().aether_quantize_rows_e4m3, x2.data_ptr(), x2.stride(0), q.data_ptr(), x.shape[1], scale.data_ptr(), *x.shape)
+    return q, scale

@@ -121,6 +121,29 @@ int aether_qk_norm_rope(const void* qkv, int B, int S, int H, int n_text, const 
  * flags: AETHER_GEMM_WIDE_STORE (16-byte epilogue stores), AETHER_ATTN_EXACT_MAX. */
 int aether_flash_attn_fwd(const void* Qh, const void* Kh, const void* Vt, void* O, int B, int H, int S, int Spad, int flags, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * The text encoder's operators (the prompt embedding of P:290-297; the reference fills that slot with
+ * transformers' T5EncoderModel, scripts/demo.py:206-232)
+ * ------------------------------------------------------------------------------------------------ */
+
+#define AETHER_STREAM_BF16 0 /* type of a residual stream */
+#define AETHER_STREAM_FP32 1
+
+/* h = x + delta;  y = h · (mean(h²) + eps)^-1/2 · w.   x: the residual stream [rows, D], bf16 or fp32 (x_dtype); delta bf16 [rows, D] or NULL;
+ * h is written to res (the stream's type; needed with delta, may alias x or be NULL without); w fp32 [D].
+ * scale == NULL: y bf16.  scale != NULL: y is e4m3, scale fp32 [rows]: the smallest power of two s >= 2^-126 with max|y| / s <= 448, y = e4m3(y / s);
+ * a row with an infinity or a NaN in it gets the scale NaN and NaN throughout.
+ * D % 8 == 0, D <= 16384; leading dimensions in elements, multiples of 8.  Σ h² must stay in fp32's range. */
+int aether_rms_norm(const void* x, int x_dtype, long ldx, const void* delta, long ldd, void* res, long ldr, const float* w, float eps,
+                    void* y, long ldy, float* scale, int rows, int D, void* stream);
+/* Backward pass from the stored h (res): n = dy·w, ĥ = h·r:  dx = r·(n − ĥ·mean(n·ĥ)) + dres (the stream's type; dres may be NULL; may alias dres),
+ * ddelta = dx rounded to bf16 (may be NULL), dw = Σ_rows dy·ĥ (fp32 [D], summed in an order that depends on the sizes alone). */
+size_t aether_rms_norm_bwd_workspace_bytes(int rows, int D);
+int aether_rms_norm_bwd(const void* dy, long lddy, const void* res, int x_dtype, long ldr, const void* dres, long lddr, const float* w, float eps,
+                        void* dx, long lddx, void* ddelta, long ldds, float* dw, int rows, int D, void* workspace, size_t workspace_bytes, void* stream);
+/* q = e4m3(x / scale) with one power of two per row, chosen as above.  x bf16 [rows, K], K % 8 == 0. */
+int aether_quantize_rows_e4m3(const void* x, long ldx, void* q, long ldq, float* scale, int rows, int K, void* stream);
+
 /* Element-wise tail of one denoise step in ONE pass (aetherv1_pipeline_cogvideox.py:876-916): fp32 cast of the noise prediction (P:877),
  * classifier-free-guidance combine uncond + g·(cond − uncond) when nb = 2 (P:895-899), CogVideoXDPMScheduler.step for v-prediction
  * (P:907-915; x0 = sqrt(a_t)·sample − sqrt(1−a_t)·model_output, prev = m1·sample − m2·d + m_noise·noise with d = x0 on a first-order
