@@ -43,6 +43,14 @@ class AetherVaeConfig(C.Structure):
     ]
 
 
+class AetherRelbias(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("q_strides", C.c_long * 3), ("k_strides", C.c_long * 3),
+        ("v_strides", C.c_long * 3), ("table", C.c_void_p), ("mask", C.c_void_p), ("mask_sb", C.c_long), ("B", C.c_int),
+        ("S", C.c_int), ("H", C.c_int), ("scale", C.c_float), ("num_buckets", C.c_int), ("borders", C.POINTER(C.c_int)), ("n_borders", C.c_int),
+    ]
+
+
 # name -> (restype, argtypes); every symbol declared in include/aether_hip.h
 SIGNATURES = {
     "aether_last_error": (C.c_char_p, []),
@@ -60,6 +68,7 @@ SIGNATURES = {
     "aether_rms_norm_bwd_workspace_bytes": (_sz, [_i, _i]),
     "aether_rms_norm_bwd": (_i, [_vp, _l, _vp, _i, _l, _vp, _l, _fp, _f, _vp, _l, _vp, _l, _fp, _i, _i, _vp, _sz, _vp]),
     "aether_quantize_rows_e4m3": (_i, [_vp, _l, _vp, _l, _fp, _i, _i, _vp]),
+    "aether_relbias_attn": (_i, [C.POINTER(AetherRelbias), _vp, _fp, _vp]),
     "aether_dpm_step": (_i, [_vp, _i, _f, _vp, _fp, _vp, _f, _f, _f, _f, _f, _f, _f, _fp, _fp, _vp, C.c_long, _vp]),
     "aether_conv_gemm_bf16": (_i, [_vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _i, _vp, _i, _vp, _i, _fp, _vp, _i, _fp, _sz, _i, _vp]),
     "aether_im2col_first": (_i, [_vp, C.c_long, C.c_long, C.c_long, C.c_long, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _i, _vp]),

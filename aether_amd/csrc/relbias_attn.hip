@@ -1,0 +1,302 @@
+// Self-attention with a learned bias by bucket of the relative position, forward pass, head dimension 64:
+//
+//   S_ij = scale · q_i·k_j + T[bucket(j − i), h]  where key j counts,   P = softmax_j(S),   O = P V;   a row without keys gives 0.
+//
+// gfx950 design
+//   * A wave owns 32 queries, a workgroup NW waves of one (batch, head); tiles of 64 keys, K and V by 16-byte LDS-DMA into two buffers, one barrier
+//     per tile.  Sᵀ = K·Qᵀ on v_mfma_f32_32x32x16_bf16: a lane holds 32 scores of ONE query.  K rows enter in the order pi, so that the
+//     exponentiated scores are, in register order, the B operand of Oᵀ += Vᵀ·Pᵀ; Vᵀ comes out of the row-major tile by ds_read_b64_tr_b16.
+//   * The bias depends on key − query alone and is constant beyond `reach` (91 positions for 32 buckets up to 128): a tile that lies beyond it adds ONE
+//     number, folded into the fma that scales the scores.  Only the few tiles along the diagonal look their bias up, in a table of 2·reach + 1 floats
+//     in LDS, whose addresses are consecutive over the lanes (no bank conflicts).
+//   * Soft-max over one pass: the shift of a row is the true maximum of its first tile; later tiles are exponentiated against it and checked
+//     afterwards (a lane's partial sum above 2^100, or NaN, makes the wave take the classic online step on the scores it still holds).  Any shift
+//     gives the same soft-max; the check keeps exp2 inside fp32.  Sums are fp32; P is rounded to bf16 once, as the operand of P·V.
+//   * Keys that do not count: whole tiles are skipped; in a tile that holds some, their scores become −inf and their V elements 0 (a NaN or an infinity
+//     behind the mask reaches nothing).
+#include "relbias_attn.hpp"
+#include "../../include/aether_hip.h"
+
+namespace aether {
+
+constexpr int RB_BUF = 2 * RB_TILE;
+constexpr int RB_PAD = 96;                       // >= 31 + 63: a wave's 32 queries against 64 keys
+
+struct RbFwdArgs { RbArgs a; bf16_t* o; float* lse; };
+
+template <int NW>
+__global__ __launch_bounds__(NW * 64) void relbias_attn_fwd_kernel(RbFwdArgs args) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const RbArgs& p = args.a;
+    float* const tab = (float*)(smem + 2 * RB_BUF);
+    unsigned char* const words8 = (unsigned char*)(smem + 2 * RB_BUF + ((2 * (p.reach + RB_PAD) + 1) * 4 + 15) / 16 * 16);
+    const uint64_t* const words = (const uint64_t*)words8;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5, l32 = lane & 31;
+    const int wave_s = __builtin_amdgcn_readfirstlane(wave);
+    const int S = p.S;
+    const int wgid = xcd_remap((int)blockIdx.x, p.B * p.H * p.nqb);   // the query blocks of a head share an L2
+    const int bh = wgid / p.nqb, qb = wgid - bh * p.nqb;
+    const int b = bh / p.H, h = bh - b * p.H;
+    const int q0 = qb * (NW * 32) + wave_s * 32;                      // this wave's first query
+    const int qrow = q0 + l32;
+
+    rb_fill_table<RB_PAD>(p, h, tab, NW * 64);
+    if (p.mask) rb_fill_words(p.mask + (size_t)b * p.mask_sb, S, words8, NW * 64);
+
+    bf16x8 qf[4];
+    {
+        const bf16_t* qp = p.q.p + (size_t)b * p.q.sb + (size_t)h * p.q.sh + (size_t)min(qrow, S - 1) * p.q.ss;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) qf[ks] = *(const bf16x8*)(qp + 16 * ks + 8 * hi);
+    }
+    // ---- staging: a wave-instruction moves 8 rows x 128 bytes; rows at or beyond S are outside the descriptor and their keys do not count ----
+    const unsigned k_row = (unsigned)p.k.ss * 2, v_row = (unsigned)p.v.ss * 2;
+    const buf_rsrc_t k_rsrc = make_buf_rsrc(p.k.p + (size_t)b * p.k.sb + (size_t)h * p.k.sh, (unsigned)(S - 1) * k_row + 128);
+    const buf_rsrc_t v_rsrc = make_buf_rsrc(p.v.p + (size_t)b * p.v.sb + (size_t)h * p.v.sh, (unsigned)(S - 1) * v_row + 128);
+    unsigned k_off[8 / NW], v_off[8 / NW];
+#pragma unroll
+    for (int ps = 0; ps < 8 / NW; ++ps) {
+        const int r = (ps * NW + wave) * 8 + (lane >> 3), ch = lane & 7;
+        k_off[ps] = r * k_row + ((ch ^ ((r >> 1) & 7)) << 4);
+        v_off[ps] = r * v_row + ((ch ^ (2 * ((r >> 1) & 3))) << 4);
+    }
+    auto stage = [&](int j, int buf) {
+        char* const dst = smem + buf * RB_BUF + wave_s * 1024;
+#pragma unroll
+        for (int ps = 0; ps < 8 / NW; ++ps) {
+            bglds16(k_rsrc, k_off[ps], (unsigned)j * (RB_KV * k_row), dst + ps * (NW * 1024));
+            bglds16(v_rsrc, v_off[ps], (unsigned)j * (RB_KV * v_row), dst + RB_TILE + ps * (NW * 1024));
+        }
+    };
+    // ---- fragment addresses ----
+    const int a_ = l32 >> 3, h_ = (l32 >> 2) & 1, c_ = l32 & 3;
+    const int pi = 16 * (a_ >> 1) + 8 * h_ + 4 * (a_ & 1) + c_;       // the key that feeds MFMA row l32
+    int koff[4];
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) koff[ks] = pi * 128 + (((2 * ks + hi) ^ ((pi >> 1) & 7)) << 4);
+    // Vᵀ: this lane names key 8hi + (i >> 2) [+ 4, + 16 slab], elements 4(i & 3) .. of the 16-element group (lane >> 4) & 1 of a d half
+    const int ti = lane & 15, tkey = 8 * hi + (ti >> 2);
+    int voff[2][2];                                                   // [d half][keys + 0 / + 4]
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+        for (int f = 0; f < 2; ++f) {
+            const int key = tkey + 4 * f, chunk = dt * 4 + ((lane >> 4) & 1) * 2 + ((ti & 3) >> 1);
+            voff[dt][f] = RB_TILE + key * 128 + ((chunk ^ (2 * ((key >> 1) & 3))) << 4) + (ti & 1) * 8;   // + 16 keys: the same swizzle
+        }
+
+    f32x16 o[2];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) { o[0][i] = 0.f; o[1][i] = 0.f; }
+    float m_run = 0.f, l_run = 0.f;
+    bool started = false;
+
+    __syncthreads();                                                  // table and words are there
+    const float far_r = tab[2 * (p.reach + RB_PAD)], far_l = tab[0];
+    const int nkv = (S + RB_KV - 1) / RB_KV;
+    auto next_tile = [&](int j, uint64_t& w) {                        // the next tile from j on that holds a key, nkv if none does
+        for (; j < nkv; ++j)
+            if ((w = rb_word(p, words, j)) != 0) break;
+        return j;
+    };
+    uint64_t w = 0, w_next = 0;
+    int j = next_tile(0, w);
+    if (j < nkv) stage(j, 0);
+    drain_and_barrier();
+    int buf = 0;
+    while (j < nkv) {
+        const int j_next = next_tile(j + 1, w_next);
+        if (j_next < nkv) stage(j_next, buf ^ 1);
+        const char* base = smem + buf * RB_BUF;
+        f32x16 x[2];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) { x[0][i] = 0.f; x[1][i] = 0.f; }
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+                x[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(base + t * 4096 + koff[ks]), qf[ks], x[t], 0, 0, 0);
+        __builtin_amdgcn_s_setprio(0);
+        // x[t][r]: query l32, key 64j + 32t + 16(r >> 3) + 8hi + (r & 7)
+        const int d_lo = j * RB_KV - (q0 + 31), d_hi = j * RB_KV + 63 - q0;
+        if (d_lo >= p.reach || d_hi <= -p.reach) {
+            const float add = (d_lo >= p.reach ? far_r : far_l) - m_run;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) x[t][r] = fmaf(x[t][r], p.c, add);
+        } else {
+            // |d| <= reach + 94 here: inside the padded table.  A query row beyond the last one reads inside it too (its wave's own range).
+            const float* tb = tab + (j * RB_KV + 8 * hi - qrow + p.reach + RB_PAD);
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) x[t][r] = fmaf(x[t][r], p.c, tb[32 * t + 16 * (r >> 3) + (r & 7)] - m_run);
+        }
+        const bool part = w != ~0ull;
+        if (part) {
+            const uint64_t mine = w >> (8 * hi);
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (!((mine >> (32 * t + 16 * (r >> 3) + (r & 7))) & 1)) x[t][r] = -INFINITY;
+        }
+        unsigned pf[2][2][4];
+        float tsum = 0.f;
+        auto expo = [&]() {
+            float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float pa = __builtin_amdgcn_exp2f(x[t][8 * s + 2 * e]), pb = __builtin_amdgcn_exp2f(x[t][8 * s + 2 * e + 1]);
+                        pf[t][s][e] = pack_bf16x2(pa, pb);
+                        s0 += pa;
+                        s1 += pb;
+                    }
+            tsum = s0 + s1;
+        };
+        bool redo = !started;
+        if (!redo) {
+            expo();
+            redo = __any(!(tsum <= 1.2676506e30f)) != 0;               // 2^100
+        }
+        if (__builtin_expect(redo, 0)) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, fmaxf(x[0][r], x[1][r]));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const float up = started ? fmaxf(top, 0.f) : fmaxf(top, -1e30f);   // a first tile of −inf alone keeps a finite shift
+            if (started) {
+                const float alpha = __builtin_amdgcn_exp2f(-up);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) { o[0][i] *= alpha; o[1][i] *= alpha; }
+                l_run *= alpha;
+            }
+            m_run += up;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) { x[0][i] -= up; x[1][i] -= up; }
+            expo();
+            started = true;
+        }
+        l_run += tsum;
+        // ---- Oᵀ += Vᵀ · Pᵀ ----
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const bf16x8 pv = __builtin_bit_cast(bf16x8, make_uint4(pf[t][s][0], pf[t][s][1], pf[t][s][2], pf[t][s][3]));
+#pragma unroll
+                for (int dt = 0; dt < 2; ++dt) {
+                    const char* vb = base + (2 * t + s) * 2048;
+                    bf16x8 vf = rb_read_tr(vb + voff[dt][0], vb + voff[dt][1]);
+                    if (part) {
+                        const unsigned bits = (unsigned)(w >> (32 * t + 16 * s + 8 * hi)) & 0xffu;
+                        uint4 u = __builtin_bit_cast(uint4, vf);
+                        u.x &= (bits & 1 ? 0xffffu : 0u) | (bits & 2 ? 0xffff0000u : 0u);
+                        u.y &= (bits & 4 ? 0xffffu : 0u) | (bits & 8 ? 0xffff0000u : 0u);
+                        u.z &= (bits & 16 ? 0xffffu : 0u) | (bits & 32 ? 0xffff0000u : 0u);
+                        u.w &= (bits & 64 ? 0xffffu : 0u) | (bits & 128 ? 0xffff0000u : 0u);
+                        vf = __builtin_bit_cast(bf16x8, u);
+                    }
+                    o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pv, o[dt], 0, 0, 0);
+                }
+            }
+        __builtin_amdgcn_s_setprio(0);
+        drain_and_barrier();
+        j = j_next;
+        w = w_next;
+        buf ^= 1;
+    }
+    // ---- epilogue: O[b][q][h][d], d = 32dt + 8(r >> 2) + 4hi + (r & 3) ----
+    const float l_tot = l_run + __shfl_xor(l_run, 32, 64);
+    const float inv = started ? 1.0f / l_tot : 0.f;
+    if (args.lse && hi == 0 && qrow < S)      // +inf: the backward pass gets P = 0 everywhere in such a row
+        args.lse[(size_t)bh * S + qrow] = started ? m_run + __builtin_amdgcn_logf(l_tot) : INFINITY;
+    bf16_t* orow = args.o + (((size_t)b * S + min(qrow, S - 1)) * p.H + h) * RB_D;
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt) {
+        unsigned pk[4][2];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            pk[g][0] = pack_bf16x2(o[dt][4 * g + 0] * inv, o[dt][4 * g + 1] * inv);
+            pk[g][1] = pack_bf16x2(o[dt][4 * g + 2] * inv, o[dt][4 * g + 3] * inv);
+        }
+#pragma unroll
+        for (int g = 0; g < 4; g += 2) {
+            auto r0 = __builtin_amdgcn_permlane32_swap(pk[g][0], pk[g + 1][0], false, false);
+            auto r1 = __builtin_amdgcn_permlane32_swap(pk[g][1], pk[g + 1][1], false, false);
+            if (qrow < S) *(uint4*)(orow + 32 * dt + 8 * g + 8 * hi) = make_uint4(r0[0], r1[0], r0[1], r1[1]);
+        }
+    }
+}
+
+// Fills the arguments that both passes check alike.
+int rb_setup(RbArgs& p, const AetherRelbias* d) {
+    auto fail = [](int code, const char* msg) { return aether_set_error(code, msg); };
+    if (!d) return fail(AETHER_ERR_ARG, "relbias_attn: null descriptor");
+    if (d->B < 0 || d->S < 0 || d->H < 1) return fail(AETHER_ERR_SHAPE, "relbias_attn: B and S must not be negative, H must be positive");
+    if (d->S > RB_MAX_S) return fail(AETHER_ERR_SHAPE, "relbias_attn: S must be at most 65536");
+    if (d->num_buckets < 4 || d->num_buckets % 2 != 0 || d->num_buckets > 128) return fail(AETHER_ERR_SHAPE, "relbias_attn: num_buckets must be an even number in [4, 128]");
+    const int half = d->num_buckets / 2, near_n = half / 2;
+    if (!d->borders || d->n_borders != half - near_n - 1) return fail(AETHER_ERR_ARG, "relbias_attn: borders must name where each bucket behind the first logarithmic one begins");
+    int last = near_n;
+    for (int i = 0; i < d->n_borders; ++i) {
+        if (d->borders[i] < last) return fail(AETHER_ERR_ARG, "relbias_attn: borders must not fall, nor lie below num_buckets / 4");
+        last = d->borders[i];
+        p.border[i] = last;
+    }
+    if (last > RB_MAX_REACH) return fail(AETHER_ERR_SHAPE, "relbias_attn: the last bucket must begin at 1024 or before");
+    p.B = d->B; p.S = d->S; p.H = d->H;
+    p.half = half; p.near_n = near_n; p.n_border = d->n_borders; p.reach = last;
+    p.c = d->scale * RB_LOG2E;
+    p.table = (const bf16_t*)d->table;
+    p.mask = (const unsigned char*)d->mask; p.mask_sb = d->mask_sb;
+    if ((long)d->B * d->H * ((d->S + 31) / 32) > 0x7fffffffl) return fail(AETHER_ERR_SHAPE, "relbias_attn: too many query blocks");
+    if (d->B == 0 || d->S == 0) return AETHER_OK;
+    if (!d->table) return fail(AETHER_ERR_ARG, "relbias_attn: null table");
+    const struct { RbTensor* t; const void* ptr; const long* st; } in[3] = {{&p.q, d->q, d->q_strides}, {&p.k, d->k, d->k_strides}, {&p.v, d->v, d->v_strides}};
+    for (const auto& e : in) {
+        if (!e.ptr) return fail(AETHER_ERR_ARG, "relbias_attn: null operand");
+        if ((uintptr_t)e.ptr & 15 || e.st[0] % 8 || e.st[1] % 8 || e.st[2] % 8) return fail(AETHER_ERR_ALIGN, "relbias_attn: rows of q, k, v must be 16-byte aligned");
+        // one head's rows go through a 32-bit buffer descriptor, and the tile behind the last row is addressed (not fetched) too
+        if (e.st[1] < 0 || ((long)d->S + RB_KV) * e.st[1] * 2 + 128 >= (1l << 32)) return fail(AETHER_ERR_SHAPE, "relbias_attn: S times the row stride must stay below 4 GiB, and no stride may be negative");
+        if (e.st[0] < 0 || e.st[2] < 0) return fail(AETHER_ERR_SHAPE, "relbias_attn: S times the row stride must stay below 4 GiB, and no stride may be negative");
+        *e.t = RbTensor{(const bf16_t*)e.ptr, e.st[0], e.st[1], e.st[2]};
+    }
+    return AETHER_OK;
+}
+
+}  // namespace aether
+
+using namespace aether;
+
+extern "C" int aether_relbias_attn(const AetherRelbias* d, void* o, float* lse, void* stream) {
+    RbFwdArgs args = {};
+    int rc = rb_setup(args.a, d);
+    if (rc) return rc;
+    if (d->B == 0 || d->S == 0) return AETHER_OK;
+    if (!o) return aether_set_error(AETHER_ERR_ARG, "relbias_attn: null output");
+    if ((uintptr_t)o & 15) return aether_set_error(AETHER_ERR_ALIGN, "relbias_attn: the output must be 16-byte aligned");
+    args.o = (bf16_t*)o;
+    args.lse = lse;
+    RbArgs& p = args.a;
+    const size_t lds = 2 * RB_BUF + ((2 * (p.reach + RB_PAD) + 1) * 4 + 15) / 16 * 16 + (p.mask ? (size_t)(p.S + 63) / 64 * 8 : 0);
+    const long heads = (long)p.B * p.H;
+    hipStream_t s = (hipStream_t)stream;
+#define RB_LAUNCH(NW)                                                                                              \
+    do {                                                                                                           \
+        p.nqb = (p.S + NW * 32 - 1) / (NW * 32);                                                                   \
+        hipLaunchKernelGGL((relbias_attn_fwd_kernel<NW>), dim3((unsigned)(heads * p.nqb)), dim3(NW * 64), lds, s, args); \
+    } while (0)
+    if (p.S > 64 && heads * ((p.S + 127) / 128) >= 256) RB_LAUNCH(4);
+    else if (p.S > 32) RB_LAUNCH(2);
+    else RB_LAUNCH(1);
+#undef RB_LAUNCH
+    return aether_check_launch("relbias_attn");
+}

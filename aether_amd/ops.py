@@ -5,6 +5,9 @@ These are the calls the parity tests exercise one by one; the production transfo
 """
 from __future__ import annotations
 
+import ctypes as C
+import functools
+
 import torch
 
 from . import _lib
@@ -251,3 +254,69 @@ def quantize_rows_e4m3(x):
     if x.shape[0]:
         _run("quantize_rows_e4m3", dev, _lib.load().aether_quantize_rows_e4m3, x2.data_ptr(), x2.stride(0), q.data_ptr(), x.shape[1], scale.data_ptr(), *x.shape)
     return q, scale
+
+
+@functools.lru_cache(maxsize=None)
+def relbias_borders(num_buckets, max_distance):
+    """Where each bucket of one side behind the first logarithmic one begins.  One side has half = num_buckets / 2 buckets: the distances below
+    near = half // 2 have one each, the others are spaced over the logarithm up to max_distance: bucket near + b begins at the smallest n with
+    log(n / near) / log(max_distance / near) (half − near) >= b.  Compared as whole numbers, so that no rounding moves a border."""
+    if num_buckets < 4 or num_buckets % 2 or num_buckets > 128:
+        raise ValueError(f"num_buckets must be an even number in [4, 128], got {num_buckets}")
+    half = num_buckets // 2
+    near = half // 2
+    if max_distance != int(max_distance) or max_distance <= near:
+        raise ValueError(f"max_distance must be a whole number above num_buckets / 4 = {near}, got {max_distance}")
+    found, n = [], near
+    for b in range(1, half - near):
+        # (n / near)^(half - near) >= (max_distance / near)^b
+        while n ** (half - near) * near ** b < int(max_distance) ** b * near ** (half - near):
+            n += 1
+            if n > 1024:
+                raise ValueError(f"max_distance {max_distance} with {num_buckets} buckets: the last bucket must begin at 1024 or before")
+        found.append(n)
+    return (C.c_int * len(found))(*found)
+
+
+def _heads(t):
+    """[B, S, H, 64] with a dense last dimension, whole 16-byte pieces between rows and an aligned base; copied only where it is not so."""
+    sb, ss, sh, one = t.stride()
+    if one != 1 or sb % 8 or ss % 8 or sh % 8 or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _relbias(name, q, k, v, table, max_distance, scale, key_mask):
+    """(device, descriptor, what it points at) of a call."""
+    dev = _same_device(q, k, v, table, key_mask)
+    for n, t in (("q", q), ("k", k), ("v", v)):
+        if t.dtype != torch.bfloat16 or t.dim() != 4 or t.shape[3] != 64 or t.shape != q.shape:
+            raise ValueError(f"{name}: q, k, v are bfloat16 [B, S, H, 64] of one shape; {n} is {t.dtype} {list(t.shape)}")
+    B, S, H, _ = q.shape
+    if H < 1:
+        raise ValueError(f"{name}: no heads")
+    if table.dtype != torch.bfloat16 or table.dim() != 2 or table.shape[1] != H:
+        raise ValueError(f"{name}: the table is bfloat16 [num_buckets, {H}], got {table.dtype} {list(table.shape)}")
+    borders = relbias_borders(table.shape[0], max_distance)
+    q, k, v, table = _heads(q), _heads(k), _heads(v), table.contiguous()
+    if key_mask is not None:
+        if key_mask.dtype != torch.bool or key_mask.shape != (B, S):
+            raise ValueError(f"{name}: key_mask is bool [{B}, {S}], True where a key counts, got {key_mask.dtype} {list(key_mask.shape)}")
+        if key_mask.stride(1) != 1 or key_mask.stride(0) < 0:
+            key_mask = key_mask.contiguous()
+    d = _lib.AetherRelbias(q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride()[:3], k.stride()[:3], v.stride()[:3], table.data_ptr(),
+                           None if key_mask is None else key_mask.data_ptr(), 0 if key_mask is None else key_mask.stride(0), B, S, H, scale,
+                           table.shape[0], borders, len(borders))
+    return dev, d, (q, k, v, table, key_mask)
+
+
+def relbias_attn(q, k, v, table, max_distance=128, scale=1.0, key_mask=None, need_lse=False):
+    """Self-attention with a learned bias by relative position: S_ij = scale q_i·k_j + table[bucket(j − i), h], O = softmax(S) V over the keys that count.
+    q, k, v bfloat16 [B, S, H, 64] (views of a packed projection included), table bfloat16 [num_buckets, H] (buckets of both directions, exact up to
+    num_buckets / 4, logarithmic up to max_distance), key_mask bool [B, S], True where a key counts.  A row without keys gives 0; what stands at
+    keys that do not count reaches nothing.  -> o bfloat16 [B, S, H, 64], or (o, lse) for `relbias_attn_backward`."""
+    dev, d, keep = _relbias("relbias_attn", q, k, v, table, max_distance, scale, key_mask)
+    o = torch.empty(q.shape, dtype=torch.bfloat16, device=dev)
+    lse = torch.empty(q.shape[0], q.shape[2], q.shape[1], dtype=torch.float32, device=dev) if need_lse else None
+    _run("relbias_attn", dev, _lib.load().aether_relbias_attn, C.byref(d), o.data_ptr(), _lib.ptr(lse))
+    return (o, lse) if need_lse else o

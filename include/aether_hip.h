@@ -144,6 +144,28 @@ int aether_rms_norm_bwd(const void* dy, long lddy, const void* res, int x_dtype,
 /* q = e4m3(x / scale) with one power of two per row, chosen as above.  x bf16 [rows, K], K % 8 == 0. */
 int aether_quantize_rows_e4m3(const void* x, long ldx, void* q, long ldq, float* scale, int rows, int K, void* stream);
 
+/* Self-attention with a learned bias by bucket of the relative position, head_dim 64:
+ *   S_ij = scale · q_i·k_j + table[bucket(j − i)][h] where key j counts;  O = softmax_j(S) V;  a row without keys gives 0.
+ * bucket(d), n = |d|, half = num_buckets / 2, near = half / 2:  (d > 0 ? half : 0) + (n < near ? n : near + #{i : borders[i] <= n}); borders (HOST
+ * array of half − near − 1 distances, not falling) is where each bucket behind the first logarithmic one begins, at 1024 or before.
+ * q, k, v bf16 [B, S, H, 64] with strides (batch, position, head) in elements, multiples of 8, last dimension dense; S <= 65536.
+ * table bf16 [num_buckets, H]; mask: bytes [B, S] with batch stride mask_sb, 0 = the key does not count, or NULL.  What stands at a key that does not
+ * count (NaN, infinities) reaches no output. */
+typedef struct AetherRelbias {
+    const void* q; const void* k; const void* v;
+    long q_strides[3], k_strides[3], v_strides[3];
+    const void* table;
+    const void* mask;
+    long mask_sb;
+    int B, S, H;
+    float scale;
+    int num_buckets;
+    const int* borders; /* host */
+    int n_borders;
+} AetherRelbias;
+/* o bf16 [B, S, H, 64] dense; lse fp32 [B, H, S] (base-2 log of the row sums, +inf for a row without keys) for the backward pass, or NULL. */
+int aether_relbias_attn(const AetherRelbias* d, void* o, float* lse, void* stream);
+
 /* Element-wise tail of one denoise step in ONE pass (aetherv1_pipeline_cogvideox.py:876-916): fp32 cast of the noise prediction (P:877),
  * classifier-free-guidance combine uncond + g·(cond − uncond) when nb = 2 (P:895-899), CogVideoXDPMScheduler.step for v-prediction
  * (P:907-915; x0 = sqrt(a_t)·sample − sqrt(1−a_t)·model_output, prev = m1·sample − m2·d + m_noise·noise with d = x0 on a first-order

@@ -1,0 +1,243 @@
+"""relbias_attn against the definition in float64 on the same bf16 inputs.
+
+Tolerance of an output element o = Σ_j p_j v_j, with T = Σ_j p_j |v_j|: every p_j is rounded to bf16 (2^-8 p_j) before its product; a score is a sum
+of 64 exact products in fp32, scaled and exponentiated: its absolute error is at most 66 · 2^-24 · (Σ|q k| scale + |bias|) and moves p_j by as much,
+numerator and denominator each; the output is rounded once (2^-8 |o|).  Scores of the tests below have Σ|q k| · scale < 60 where nothing else is said:
+2 · 66 · 2^-24 · 66 < 2^-10.  Bound: (2^-8 + 2^-10) T + 2^-8 |o|."""
+import math
+
+import pytest
+import torch
+
+from relbias_reference import attention, bucket, inputs
+
+pytestmark = pytest.mark.gpu
+BF16 = 2.0 ** -8
+
+
+def _check_o(got, q, k, v, table, extra=2.0 ** -10, **kw):
+    d = [t.double() for t in (q, k, v, table)]
+    want, p = attention(*d, **kw)
+    mask = kw.get("key_mask")
+    va = d[2].abs() if mask is None else torch.where(mask[:, :, None, None], d[2].abs(), 0.0)
+    T = torch.matmul(p, va.permute(0, 2, 1, 3).contiguous()).permute(0, 2, 1, 3)
+    err = (got.double() - want).abs()
+    lim = (BF16 + extra) * T + BF16 * want.abs()
+    assert got.shape == want.shape and got.dtype == torch.bfloat16
+    assert bool(torch.isfinite(got.float()).all()) and bool((err <= lim).all()), f"worst {(err - lim).max().item():.3e}, rel {(err.norm() / want.norm()).item():.3e}"
+    return want, p
+
+
+LENGTHS = [1, 2, 31, 32, 33, 63, 64, 65, 96, 127, 128, 129, 191, 226, 300, 513, 1030]
+
+
+@pytest.mark.parametrize("S", LENGTHS)
+@pytest.mark.parametrize("B,H", [(1, 1), (2, 3)])
+def test_lengths(cuda, hip_lib, S, B, H):
+    from aether_amd import ops
+    qkv, table = inputs(B, S, H, device=cuda)
+    q, k, v = qkv.unbind(2)
+    o, lse = ops.relbias_attn(q, k, v, table, need_lse=True)
+    _check_o(o, q, k, v, table)
+    assert torch.equal(o, ops.relbias_attn(q, k, v, table)), "the statistics do not change the output"
+    # lse is the base-2 logarithm of the rows' sums of exp(score)
+    s = torch.matmul(q.double().permute(0, 2, 1, 3).contiguous(), k.double().permute(0, 2, 3, 1).contiguous())
+    bias = torch.tensor([[bucket(j - i, 32, 128) for j in range(S)] for i in range(S)], device=cuda)
+    s = s + table.double()[bias].permute(2, 0, 1)
+    assert bool(((torch.logsumexp(s, -1) / math.log(2) - lse.double()).abs() < 1e-4).all())
+
+
+@pytest.mark.parametrize("B,S,H", [(1, 226, 64), (16, 226, 64), (8, 64, 64), (1, 2050, 16), (40, 33, 8), (300, 5, 2)])
+def test_many_blocks(cuda, hip_lib, B, S, H):
+    """Grids beyond one workgroup per CU, every block size."""
+    from aether_amd import ops
+    qkv, table = inputs(B, S, H, device=cuda, seed=1)
+    q, k, v = qkv.unbind(2)
+    _check_o(ops.relbias_attn(q, k, v, table), q, k, v, table)
+
+
+@pytest.mark.parametrize("num_buckets,max_distance", [(4, 2), (4, 100), (6, 3), (8, 20), (10, 9), (32, 32), (32, 128), (64, 256), (128, 1000), (12, 1024)])
+@pytest.mark.parametrize("S", [65, 700])
+def test_buckets(cuda, hip_lib, num_buckets, max_distance, S):
+    """Every way the buckets are laid out: reach 1 ... 930, few and many borders.  A wrong bucket shows: the table's entries are far apart."""
+    from aether_amd import ops
+    qkv, table = inputs(1, S, 2, num_buckets, device=cuda, seed=2)
+    table = torch.randperm(num_buckets * 2, generator=torch.Generator().manual_seed(3)).view(num_buckets, 2).to(torch.bfloat16).to(cuda) / 4
+    q, k, v = qkv.unbind(2)
+    _check_o(ops.relbias_attn(q, k, v, table, max_distance), q, k, v, table, max_distance=max_distance)
+
+
+def _masks(B, S, cuda):
+    g = torch.Generator().manual_seed(S)
+    right = torch.arange(S)[None, :] < torch.tensor([S] + [max(1, (S * (b + 1)) // (B + 1)) for b in range(B - 1)])[:, None]
+    left = right.flip(1)
+    holes = torch.rand(B, S, generator=g) < 0.5
+    holes[:, S // 2] = True
+    one = torch.zeros(B, S, dtype=torch.bool)
+    one[torch.arange(B), torch.randint(0, S, (B,), generator=g)] = True
+    none = right.clone()
+    none[-1] = False
+    blocks = (torch.arange(S) // 64 % 2 == 1)[None, :].repeat(B, 1) | one
+    return {k: m.to(cuda) for k, m in dict(right=right, left=left, holes=holes, one=one, none=none, blocks=blocks).items()}
+
+
+@pytest.mark.parametrize("kind", ["right", "left", "holes", "one", "none", "blocks"])
+@pytest.mark.parametrize("S", [1, 33, 64, 226, 515])
+def test_masks(cuda, hip_lib, kind, S):
+    """Padding on either side, holes, one key alone, no key, whole tiles left out; NaN and infinities behind the mask reach nothing."""
+    from aether_amd import ops
+    B, H = 3, 2
+    qkv, table = inputs(B, S, H, device=cuda, seed=4)
+    mask = _masks(B, S, cuda)[kind]
+    q, k, v = qkv.unbind(2)
+    o, lse = ops.relbias_attn(q, k, v, table, key_mask=mask, need_lse=True)
+    _check_o(o, q, k, v, table, key_mask=mask)
+    empty = ~mask.any(1)
+    assert bool((o[empty] == 0).all()) and bool(torch.isposinf(lse[empty]).all()) and bool(torch.isfinite(lse[~empty]).all())
+    bad = qkv.clone()
+    for i, val in enumerate((math.nan, math.inf, -math.inf, 3e38)):
+        at = ~mask & ((torch.arange(S, device=cuda) % 4) == i)[None, :]
+        bad[:, :, 1:][at] = val
+    assert torch.equal(ops.relbias_attn(q, bad[:, :, 1], bad[:, :, 2], table, key_mask=mask), o)
+    if kind == "right":     # an unpadded call on the shorter prompt gives the same rows
+        n = int(mask[1].sum())
+        alone = ops.relbias_attn(q[1:2, :n], k[1:2, :n], v[1:2, :n], table)
+        assert bool(((alone.float() - o[1:2, :n].float()).abs() <= 2 * BF16 * o[1:2, :n].float().abs() + 1e-2).all())
+
+
+def test_mask_layouts(cuda, hip_lib):
+    from aether_amd import ops
+    qkv, table = inputs(3, 100, 2, device=cuda, seed=5)
+    q, k, v = qkv.unbind(2)
+    mask = _masks(3, 100, cuda)["holes"]
+    o = ops.relbias_attn(q, k, v, table, key_mask=mask)
+    assert torch.equal(ops.relbias_attn(q, k, v, table, key_mask=mask.t().contiguous().t()), o)
+    wide = torch.zeros(3, 137, dtype=torch.bool, device=cuda)
+    wide[:, 11:111] = mask
+    assert torch.equal(ops.relbias_attn(q, k, v, table, key_mask=wide[:, 11:111]), o)
+    one = mask[:1]
+    assert torch.equal(ops.relbias_attn(q, k, v, table, key_mask=one.expand(3, 100)), ops.relbias_attn(q, k, v, table, key_mask=one.repeat(3, 1)))
+    every = torch.ones(3, 100, dtype=torch.bool, device=cuda)
+    assert torch.equal(ops.relbias_attn(q, k, v, table, key_mask=every), ops.relbias_attn(q, k, v, table))
+
+
+def test_layouts(cuda, hip_lib):
+    """Packed, head-major, padded, broadcast, reversed-stride and misaligned operands; what lies around a view stays as it was."""
+    from aether_amd import ops
+    qkv, table = inputs(2, 70, 3, device=cuda, seed=6)
+    q, k, v = qkv.unbind(2)
+    o = ops.relbias_attn(q, k, v, table)
+    dense = [t.contiguous() for t in (q, k, v)]
+    assert torch.equal(ops.relbias_attn(*dense, table), o)
+    heads = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in (q, k, v)]
+    assert torch.equal(ops.relbias_attn(*heads, table), o)
+    wide = torch.full((2, 75, 3, 96), math.nan, dtype=torch.bfloat16, device=cuda)
+    wide[:, 2:72, :, 8:72] = k
+    assert torch.equal(ops.relbias_attn(q, wide[:, 2:72, :, 8:72], v, table), o)
+    off = torch.empty(q.numel() + 1, dtype=torch.bfloat16, device=cuda)[1:].view(q.shape).copy_(q)
+    assert torch.equal(ops.relbias_attn(off, k, v, table), o)
+    last = q.transpose(2, 3).contiguous().transpose(2, 3)
+    assert torch.equal(ops.relbias_attn(last, k, v, table), o)
+    assert torch.equal(ops.relbias_attn(q, k, v, table.t().contiguous().t()), o)
+    shared = ops.relbias_attn(q, k[:, :, :1].expand(-1, -1, 3, -1), v[:1].expand(2, -1, -1, -1), table)
+    assert torch.equal(shared, ops.relbias_attn(q, k[:, :, :1].repeat(1, 1, 3, 1), v[:1].repeat(2, 1, 1, 1), table))
+    assert ops.relbias_attn(q[:0], k[:0], v[:0], table).shape == (0, 70, 3, 64)
+    o0, lse0 = ops.relbias_attn(q[:, :0], k[:, :0], v[:, :0], table, need_lse=True)
+    assert o0.shape == (2, 0, 3, 64) and lse0.shape == (2, 3, 0)
+
+
+@pytest.mark.parametrize("order", ["early", "late", "rising", "falling", "far_below"])
+def test_score_ranges(cuda, hip_lib, order):
+    """Scores of several hundred, their peak in the first tile, the last one, rising or falling over the tiles, and all of them far below zero.
+    A score of 400 carries 66 · 2^-24 · 800 < 2^-8 of absolute error, numerator and denominator each."""
+    from aether_amd import ops
+    B, S, H = 1, 400, 2
+    qkv, table = inputs(B, S, H, device=cuda, seed=7)
+    at = torch.arange(S, device=cuda, dtype=torch.float32)
+    level = dict(early=400 * (at < 5), late=400 * (at > 390), rising=at, falling=400 - at, far_below=at * 0 - 400)[order]
+    q = qkv[:, :, 0].clone()
+    k = qkv[:, :, 1].clone()
+    q[..., 0], k[..., 0] = 4.0, (level / 4).to(torch.bfloat16)[None, :, None]
+    v = qkv[:, :, 2]
+    _check_o(ops.relbias_attn(q, k, v, table), q, k, v, table, extra=2.0 ** -6)
+
+
+def test_scale(cuda, hip_lib):
+    from aether_amd import ops
+    qkv, table = inputs(2, 150, 2, device=cuda, seed=8, qk=8.0)
+    q, k, v = qkv.unbind(2)
+    for scale in (0.125, 0.0, -0.1):
+        _check_o(ops.relbias_attn(q, k, v, table, scale=scale), q, k, v, table, scale=scale)
+
+
+def test_non_finite_inputs_stay_where_they_are(cuda, hip_lib):
+    """A NaN in one query makes that row NaN and no other."""
+    from aether_amd import ops
+    qkv, table = inputs(1, 200, 2, device=cuda, seed=9)
+    q, k, v = qkv.unbind(2)
+    o = ops.relbias_attn(q, k, v, table)
+    bad = q.clone()
+    bad[0, 77, 1, 5] = math.nan
+    got = ops.relbias_attn(bad, k, v, table)
+    assert bool(torch.isnan(got[0, 77, 1].float()).all())
+    keep = torch.ones(200, 2, dtype=torch.bool, device=cuda)
+    keep[77, 1] = False
+    assert bool(((got[0][keep].float() - o[0][keep].float()).abs() <= 2 * BF16 * o[0][keep].float().abs() + 1e-2).all())
+
+
+def test_long(cuda, hip_lib):
+    """A long sequence with a mask: only the last rows and the first are compared (the reference is quadratic)."""
+    from aether_amd import ops
+    S = 20000
+    qkv, table = inputs(1, S, 1, device=cuda, seed=10)
+    q, k, v = qkv.unbind(2)
+    mask = torch.arange(S, device=cuda)[None, :] < S - 1234
+    mask[0, 5000:9000] = False
+    o = ops.relbias_attn(q, k, v, table, key_mask=mask)
+    rows = torch.tensor([0, 1, 63, 64, 4999, 5000, 9000, 10007, S - 1235, S - 1234, S - 1], device=cuda)
+    s = torch.matmul(q[0, rows, 0].double(), k[0, :, 0].double().t().contiguous())
+    b = torch.tensor([[bucket(j - i, 32, 128) for j in range(S)] for i in rows.tolist()], device=cuda)
+    s = (s + table.double()[b][..., 0]).masked_fill(~mask, -math.inf)
+    p = torch.softmax(s, -1)
+    want, T = p @ v[0, :, 0].double(), p @ v[0, :, 0].double().abs()
+    err = (o[0, rows, 0].double() - want).abs()
+    assert bool((err <= (BF16 + 2.0 ** -10) * T + BF16 * want.abs()).all())
+
+
+def test_refusals(cuda, hip_lib):
+    from aether_amd import ops
+    qkv, table = inputs(2, 16, 2, device=cuda)
+    q, k, v = qkv.unbind(2)
+    mask = torch.ones(2, 16, dtype=torch.bool, device=cuda)
+    for bad in (lambda: ops.relbias_attn(q.half(), k, v, table), lambda: ops.relbias_attn(q, k[:, :8], v, table), lambda: ops.relbias_attn(q[..., :32], k[..., :32], v[..., :32], table),
+                lambda: ops.relbias_attn(q, k, v, table.float()), lambda: ops.relbias_attn(q, k, v, table[:, :1]), lambda: ops.relbias_attn(q, k, v, table[:31]),
+                lambda: ops.relbias_attn(q, k, v, table[:2]), lambda: ops.relbias_attn(q, k, v, table, max_distance=8), lambda: ops.relbias_attn(q, k, v, table, max_distance=5000),
+                lambda: ops.relbias_attn(q, k, v, table, key_mask=mask.float()), lambda: ops.relbias_attn(q, k, v, table, key_mask=mask[:, :8]),
+                lambda: ops.relbias_attn(q[0], k[0], v[0], table)):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(RuntimeError, match="device tensors"):
+        ops.relbias_attn(q, k, v, table, key_mask=mask.cpu())
+
+
+def test_graph(cuda, hip_lib):
+    """Captured and replayed on new values, eager work in between."""
+    from aether_amd import ops
+    qkv, table = inputs(2, 226, 4, device=cuda, seed=11)
+    mask = _masks(2, 226, cuda)["right"]
+    q, k, v = qkv.unbind(2)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.relbias_attn(q, k, v, table, key_mask=mask)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = ops.relbias_attn(q, k, v, table, key_mask=mask)
+    for n in (226, 100, 3):
+        qkv.mul_(-0.9)
+        mask[1] = torch.arange(226, device=cuda) < n
+        graph.replay()
+        want = ops.relbias_attn(q, k, v, table, key_mask=mask)
+        torch.cuda.synchronize()
+        assert torch.equal(o, want)

@@ -70,3 +70,57 @@ def test_wrappers_refuse_host_tensors(hip_lib):
                  lambda: ops.quantize_rows_e4m3(x.bfloat16())):
         with pytest.raises(RuntimeError, match="device tensors"):
             call()
+
+
+# ---- attention with a relative position bias --------------------------------------------------------------------------------------------
+def _relbias(lib, o=4096, **kw):
+    import ctypes as C
+    from aether_amd import _lib
+    a = dict(q=4096, k=4096, v=4096, st=(64 * 64, 64, 64 * 32), table=4096, mask=None, B=1, S=32, H=2, num_buckets=32, borders=(12, 16, 23, 32, 46, 64, 91))
+    a.update(kw)
+    b = a["borders"]
+    arr = (C.c_int * len(b))(*b) if b is not None else None
+    d = _lib.AetherRelbias(a["q"], a["k"], a["v"], a["st"], a["st"], a["st"], a["table"], a["mask"], 0, a["B"], a["S"], a["H"], 1.0, a["num_buckets"], arr, len(b or ()))
+    return lib.aether_relbias_attn(C.byref(d), o, None, None)
+
+
+@pytest.mark.parametrize("kw,code,text", [
+    (dict(B=-1), -2, b"negative"), (dict(S=-1), -2, b"negative"), (dict(H=0), -2, b"negative"), (dict(S=65537), -2, b"65536"),
+    (dict(num_buckets=3, borders=()), -2, b"num_buckets"), (dict(num_buckets=2, borders=()), -2, b"num_buckets"), (dict(num_buckets=130), -2, b"num_buckets"),
+    (dict(borders=(12, 16)), -1, b"borders"), (dict(borders=None), -1, b"borders"), (dict(borders=(7, 16, 23, 32, 46, 64, 91)), -1, b"borders"),
+    (dict(borders=(12, 11, 23, 32, 46, 64, 91)), -1, b"borders"), (dict(borders=(12, 16, 23, 32, 46, 64, 1025)), -2, b"1024"),
+    (dict(table=None), -1, b"table"), (dict(q=None), -1, b"operand"), (dict(v=None), -1, b"operand"), (dict(k=4104), -3, b"aligned"),
+    (dict(st=(4096, 60, 64)), -3, b"aligned"), (dict(st=(4096, -64, 64)), -2, b"stride"), (dict(st=(-4096, 64, 64)), -2, b"stride"),
+    (dict(st=(0, 1 << 15, 64), S=65536), -2, b"4 GiB"), (dict(o=None), -1, b"output"), (dict(o=4104), -3, b"aligned"),
+    (dict(B=1 << 20, H=1 << 10, S=65536), -2, b"blocks"),
+])
+def test_relbias_entry_refuses(hip_lib, kw, code, text):
+    assert _relbias(hip_lib, **kw) == code and text in hip_lib.aether_last_error()
+
+
+def test_relbias_entry_without_rows(hip_lib):
+    assert _relbias(hip_lib, S=0, q=None, table=None, o=None) == 0 and _relbias(hip_lib, B=0, q=None, table=None, o=None) == 0
+    assert hip_lib.aether_relbias_attn(None, 4096, None, None) == -1
+
+
+def test_bucket_borders():
+    """The borders against the published definition evaluated in float64 (away from its own roundings) and by counting."""
+    import math
+    from aether_amd.ops import relbias_borders
+    from relbias_reference import bucket
+    assert list(relbias_borders(32, 128)) == [12, 16, 23, 32, 46, 64, 91]
+    for nb, md in ((4, 2), (6, 3), (8, 20), (10, 9), (32, 128), (64, 256), (128, 1000), (32, 32), (12, 1024), (32, 1024)):
+        half = nb // 2
+        near = half // 2
+        borders = list(relbias_borders(nb, md))
+        assert len(borders) == half - near - 1 and borders == sorted(borders)
+        for n in range(1, 1400):
+            ours = n if n < near else near + sum(b <= n for b in borders)
+            assert ours == bucket(-n, nb, md) == bucket(n, nb, md) - half
+            if n >= near:
+                x = math.log(n / near) / math.log(md / near) * (half - near)
+                if abs(x - round(x)) > 1e-9:
+                    assert ours == min(half - 1, near + math.floor(x))
+    for nb, md in ((2, 10), (5, 10), (130, 1000), (32, 8), (32, 7), (32, 128.5), (32, 100000)):
+        with pytest.raises(ValueError):
+            relbias_borders(nb, md)
