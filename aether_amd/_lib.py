@@ -23,7 +23,7 @@ AETHER_STREAM_FP32 = 1
 ATTN_Q_SCALE = 0.125 * 1.4426950408889634   # softmax scale x log2(e): the attention kernel works in the log2 domain
 PROF_CLASSES = ["other", "layernorm", "gemm_qkv", "qk_norm_rope", "attention", "gemm_out", "gemm_ff1", "gemm_ff2"]
 
-_vp, _i, _f, _fp, _sz, _l = C.c_void_p, C.c_int, C.c_float, C.c_void_p, C.c_size_t, C.c_long
+_vp, _i, _f, _fp, _sz, _l, _lp = C.c_void_p, C.c_int, C.c_float, C.c_void_p, C.c_size_t, C.c_long, C.POINTER(C.c_long)
 
 
 class AetherDitConfig(C.Structure):
@@ -68,7 +68,9 @@ SIGNATURES = {
     "aether_rms_norm_bwd_workspace_bytes": (_sz, [_i, _i]),
     "aether_rms_norm_bwd": (_i, [_vp, _l, _vp, _i, _l, _vp, _l, _fp, _f, _vp, _l, _vp, _l, _fp, _i, _i, _vp, _sz, _vp]),
     "aether_quantize_rows_e4m3": (_i, [_vp, _l, _vp, _l, _fp, _i, _i, _vp]),
-    "aether_relbias_attn": (_i, [C.POINTER(AetherRelbias), _vp, _fp, _vp]),
+    "aether_relbias_attn": (_i, [C.POINTER(AetherRelbias), _vp, _vp, _fp, _vp]),
+    "aether_relbias_attn_bwd_workspace_bytes": (_sz, [C.POINTER(AetherRelbias), _i]),
+    "aether_relbias_attn_bwd": (_i, [C.POINTER(AetherRelbias), _vp, _lp, _vp, _lp, _vp, _fp, _vp, _lp, _vp, _lp, _vp, _lp, _vp, _vp, _sz, _vp]),
     "aether_dpm_step": (_i, [_vp, _i, _f, _vp, _fp, _vp, _f, _f, _f, _f, _f, _f, _f, _fp, _fp, _vp, C.c_long, _vp]),
     "aether_conv_gemm_bf16": (_i, [_vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _i, _vp, _i, _vp, _i, _fp, _vp, _i, _fp, _sz, _i, _vp]),
     "aether_im2col_first": (_i, [_vp, C.c_long, C.c_long, C.c_long, C.c_long, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _i, _vp]),

@@ -12,6 +12,8 @@
 //   * Soft-max over one pass: the shift of a row is the true maximum of its first tile; later tiles are exponentiated against it and checked
 //     afterwards (a lane's partial sum above 2^100, or NaN, makes the wave take the classic online step on the scores it still holds).  Any shift
 //     gives the same soft-max; the check keeps exp2 inside fp32.  Sums are fp32; P is rounded to bf16 once, as the operand of P·V.
+//   * For a backward pass the output is needed beyond bf16: δ = dO·O is subtracted from numbers that may be nearly equal to it.  TRAIN multiplies V with P in
+//     two bf16 parts (P = hi + lo to 2^-17) and also stores what the rounding of O left (o_low), so that O + o_low is good to 2^-16.
 //   * Keys that do not count: whole tiles are skipped; in a tile that holds some, their scores become −inf and their V elements 0 (a NaN or an infinity
 //     behind the mask reaches nothing).
 #include "relbias_attn.hpp"
@@ -19,12 +21,9 @@
 
 namespace aether {
 
-constexpr int RB_BUF = 2 * RB_TILE;
-constexpr int RB_PAD = 96;                       // >= 31 + 63: a wave's 32 queries against 64 keys
+struct RbFwdArgs { RbArgs a; bf16_t* o; bf16_t* o_low; float* lse; };   // o_low, lse: for a backward pass
 
-struct RbFwdArgs { RbArgs a; bf16_t* o; float* lse; };
-
-template <int NW>
+template <int NW, bool TRAIN>
 __global__ __launch_bounds__(NW * 64) void relbias_attn_fwd_kernel(RbFwdArgs args) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const RbArgs& p = args.a;
@@ -40,7 +39,7 @@ __global__ __launch_bounds__(NW * 64) void relbias_attn_fwd_kernel(RbFwdArgs arg
     const int q0 = qb * (NW * 32) + wave_s * 32;                      // this wave's first query
     const int qrow = q0 + l32;
 
-    rb_fill_table<RB_PAD>(p, h, tab, NW * 64);
+    rb_fill_table(p, h, tab, NW * 64);
     if (p.mask) rb_fill_words(p.mask + (size_t)b * p.mask_sb, S, words8, NW * 64);
 
     bf16x8 qf[4];
@@ -57,8 +56,8 @@ __global__ __launch_bounds__(NW * 64) void relbias_attn_fwd_kernel(RbFwdArgs arg
 #pragma unroll
     for (int ps = 0; ps < 8 / NW; ++ps) {
         const int r = (ps * NW + wave) * 8 + (lane >> 3), ch = lane & 7;
-        k_off[ps] = r * k_row + ((ch ^ ((r >> 1) & 7)) << 4);
-        v_off[ps] = r * v_row + ((ch ^ (2 * ((r >> 1) & 3))) << 4);
+        k_off[ps] = r * k_row + ((ch ^ rb_swz(r)) << 4);
+        v_off[ps] = r * v_row + ((ch ^ rb_swz(r)) << 4);
     }
     auto stage = [&](int j, int buf) {
         char* const dst = smem + buf * RB_BUF + wave_s * 1024;
@@ -68,22 +67,9 @@ __global__ __launch_bounds__(NW * 64) void relbias_attn_fwd_kernel(RbFwdArgs arg
             bglds16(v_rsrc, v_off[ps], (unsigned)j * (RB_KV * v_row), dst + RB_TILE + ps * (NW * 1024));
         }
     };
-    // ---- fragment addresses ----
-    const int a_ = l32 >> 3, h_ = (l32 >> 2) & 1, c_ = l32 & 3;
-    const int pi = 16 * (a_ >> 1) + 8 * h_ + 4 * (a_ & 1) + c_;       // the key that feeds MFMA row l32
-    int koff[4];
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) koff[ks] = pi * 128 + (((2 * ks + hi) ^ ((pi >> 1) & 7)) << 4);
-    // Vᵀ: this lane names key 8hi + (i >> 2) [+ 4, + 16 slab], elements 4(i & 3) .. of the 16-element group (lane >> 4) & 1 of a d half
-    const int ti = lane & 15, tkey = 8 * hi + (ti >> 2);
-    int voff[2][2];                                                   // [d half][keys + 0 / + 4]
-#pragma unroll
-    for (int dt = 0; dt < 2; ++dt)
-#pragma unroll
-        for (int f = 0; f < 2; ++f) {
-            const int key = tkey + 4 * f, chunk = dt * 4 + ((lane >> 4) & 1) * 2 + ((ti & 3) >> 1);
-            voff[dt][f] = RB_TILE + key * 128 + ((chunk ^ (2 * ((key >> 1) & 3))) << 4) + (ti & 1) * 8;   // + 16 keys: the same swizzle
-        }
+    int koff[4], voff[2][2];
+    rb_row_offsets(lane, koff);
+    rb_tr_offsets(lane, voff);
 
     f32x16 o[2];
 #pragma unroll
@@ -143,7 +129,7 @@ __global__ __launch_bounds__(NW * 64) void relbias_attn_fwd_kernel(RbFwdArgs arg
                 for (int r = 0; r < 16; ++r)
                     if (!((mine >> (32 * t + 16 * (r >> 3) + (r & 7))) & 1)) x[t][r] = -INFINITY;
         }
-        unsigned pf[2][2][4];
+        unsigned pf[2][2][4], pl[TRAIN ? 2 : 1][2][4];
         float tsum = 0.f;
         auto expo = [&]() {
             float s0 = 0.f, s1 = 0.f;
@@ -155,6 +141,8 @@ __global__ __launch_bounds__(NW * 64) void relbias_attn_fwd_kernel(RbFwdArgs arg
                     for (int e = 0; e < 4; ++e) {
                         const float pa = __builtin_amdgcn_exp2f(x[t][8 * s + 2 * e]), pb = __builtin_amdgcn_exp2f(x[t][8 * s + 2 * e + 1]);
                         pf[t][s][e] = pack_bf16x2(pa, pb);
+                        if constexpr (TRAIN)
+                            pl[t][s][e] = pack_bf16x2(pa - __uint_as_float(pf[t][s][e] << 16), pb - __uint_as_float(pf[t][s][e] & 0xffff0000u));
                         s0 += pa;
                         s1 += pb;
                     }
@@ -193,18 +181,12 @@ __global__ __launch_bounds__(NW * 64) void relbias_attn_fwd_kernel(RbFwdArgs arg
                 const bf16x8 pv = __builtin_bit_cast(bf16x8, make_uint4(pf[t][s][0], pf[t][s][1], pf[t][s][2], pf[t][s][3]));
 #pragma unroll
                 for (int dt = 0; dt < 2; ++dt) {
-                    const char* vb = base + (2 * t + s) * 2048;
+                    const char* vb = base + RB_TILE + (2 * t + s) * 2048;
                     bf16x8 vf = rb_read_tr(vb + voff[dt][0], vb + voff[dt][1]);
-                    if (part) {
-                        const unsigned bits = (unsigned)(w >> (32 * t + 16 * s + 8 * hi)) & 0xffu;
-                        uint4 u = __builtin_bit_cast(uint4, vf);
-                        u.x &= (bits & 1 ? 0xffffu : 0u) | (bits & 2 ? 0xffff0000u : 0u);
-                        u.y &= (bits & 4 ? 0xffffu : 0u) | (bits & 8 ? 0xffff0000u : 0u);
-                        u.z &= (bits & 16 ? 0xffffu : 0u) | (bits & 32 ? 0xffff0000u : 0u);
-                        u.w &= (bits & 64 ? 0xffffu : 0u) | (bits & 128 ? 0xffff0000u : 0u);
-                        vf = __builtin_bit_cast(bf16x8, u);
-                    }
+                    if (part) vf = rb_keep(vf, (unsigned)(w >> (32 * t + 16 * s + 8 * hi)) & 0xffu);
                     o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pv, o[dt], 0, 0, 0);
+                    if constexpr (TRAIN)
+                        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, __builtin_bit_cast(bf16x8, make_uint4(pl[t][s][0], pl[t][s][1], pl[t][s][2], pl[t][s][3])), o[dt], 0, 0, 0);
                 }
             }
         __builtin_amdgcn_s_setprio(0);
@@ -216,27 +198,30 @@ __global__ __launch_bounds__(NW * 64) void relbias_attn_fwd_kernel(RbFwdArgs arg
     // ---- epilogue: O[b][q][h][d], d = 32dt + 8(r >> 2) + 4hi + (r & 3) ----
     const float l_tot = l_run + __shfl_xor(l_run, 32, 64);
     const float inv = started ? 1.0f / l_tot : 0.f;
-    if (args.lse && hi == 0 && qrow < S)      // +inf: the backward pass gets P = 0 everywhere in such a row
-        args.lse[(size_t)bh * S + qrow] = started ? m_run + __builtin_amdgcn_logf(l_tot) : INFINITY;
-    bf16_t* orow = args.o + (((size_t)b * S + min(qrow, S - 1)) * p.H + h) * RB_D;
+    const size_t at = (((size_t)b * S + min(qrow, S - 1)) * p.H + h) * RB_D;
+    if constexpr (TRAIN) {
+        if (hi == 0 && qrow < S)              // +inf: the backward pass gets P = 0 everywhere in such a row
+            args.lse[(size_t)bh * S + qrow] = started ? m_run + __builtin_amdgcn_logf(l_tot) : INFINITY;
+        f32x16 low[2];
 #pragma unroll
-    for (int dt = 0; dt < 2; ++dt) {
-        unsigned pk[4][2];
+        for (int dt = 0; dt < 2; ++dt)
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            pk[g][0] = pack_bf16x2(o[dt][4 * g + 0] * inv, o[dt][4 * g + 1] * inv);
-            pk[g][1] = pack_bf16x2(o[dt][4 * g + 2] * inv, o[dt][4 * g + 3] * inv);
-        }
-#pragma unroll
-        for (int g = 0; g < 4; g += 2) {
-            auto r0 = __builtin_amdgcn_permlane32_swap(pk[g][0], pk[g + 1][0], false, false);
-            auto r1 = __builtin_amdgcn_permlane32_swap(pk[g][1], pk[g + 1][1], false, false);
-            if (qrow < S) *(uint4*)(orow + 32 * dt + 8 * g + 8 * hi) = make_uint4(r0[0], r1[0], r0[1], r1[1]);
-        }
+            for (int i = 0; i < 16; ++i) low[dt][i] = o[dt][i] * inv - (float)(bf16_t)(o[dt][i] * inv);
+        rb_store(low, 1.f, args.o_low + at, hi, qrow < S);
     }
+    rb_store(o, inv, args.o + at, hi, qrow < S);
 }
 
-// Fills the arguments that both passes check alike.
+// One head's rows go through a 32-bit buffer descriptor, and the tile behind the last row is addressed (not fetched) too.
+int rb_tensor(RbTensor& t, const void* ptr, const long* st, int S) {
+    if (!ptr) return aether_set_error(AETHER_ERR_ARG, "relbias_attn: null operand");
+    if ((uintptr_t)ptr & 15 || st[0] % 8 || st[1] % 8 || st[2] % 8) return aether_set_error(AETHER_ERR_ALIGN, "relbias_attn: rows of [B, S, H, 64] operands must be 16-byte aligned");
+    if (st[0] < 0 || st[1] < 0 || st[2] < 0 || ((long)S + RB_KV) * st[1] * 2 + 128 >= (1l << 32))
+        return aether_set_error(AETHER_ERR_SHAPE, "relbias_attn: S times the row stride must stay below 4 GiB, and no stride may be negative");
+    t = RbTensor{(const bf16_t*)ptr, st[0], st[1], st[2]};
+    return AETHER_OK;
+}
+
 int rb_setup(RbArgs& p, const AetherRelbias* d) {
     auto fail = [](int code, const char* msg) { return aether_set_error(code, msg); };
     if (!d) return fail(AETHER_ERR_ARG, "relbias_attn: null descriptor");
@@ -260,15 +245,10 @@ int rb_setup(RbArgs& p, const AetherRelbias* d) {
     if ((long)d->B * d->H * ((d->S + 31) / 32) > 0x7fffffffl) return fail(AETHER_ERR_SHAPE, "relbias_attn: too many query blocks");
     if (d->B == 0 || d->S == 0) return AETHER_OK;
     if (!d->table) return fail(AETHER_ERR_ARG, "relbias_attn: null table");
-    const struct { RbTensor* t; const void* ptr; const long* st; } in[3] = {{&p.q, d->q, d->q_strides}, {&p.k, d->k, d->k_strides}, {&p.v, d->v, d->v_strides}};
-    for (const auto& e : in) {
-        if (!e.ptr) return fail(AETHER_ERR_ARG, "relbias_attn: null operand");
-        if ((uintptr_t)e.ptr & 15 || e.st[0] % 8 || e.st[1] % 8 || e.st[2] % 8) return fail(AETHER_ERR_ALIGN, "relbias_attn: rows of q, k, v must be 16-byte aligned");
-        // one head's rows go through a 32-bit buffer descriptor, and the tile behind the last row is addressed (not fetched) too
-        if (e.st[1] < 0 || ((long)d->S + RB_KV) * e.st[1] * 2 + 128 >= (1l << 32)) return fail(AETHER_ERR_SHAPE, "relbias_attn: S times the row stride must stay below 4 GiB, and no stride may be negative");
-        if (e.st[0] < 0 || e.st[2] < 0) return fail(AETHER_ERR_SHAPE, "relbias_attn: S times the row stride must stay below 4 GiB, and no stride may be negative");
-        *e.t = RbTensor{(const bf16_t*)e.ptr, e.st[0], e.st[1], e.st[2]};
-    }
+    int rc = rb_tensor(p.q, d->q, d->q_strides, d->S);
+    if (!rc) rc = rb_tensor(p.k, d->k, d->k_strides, d->S);
+    if (!rc) rc = rb_tensor(p.v, d->v, d->v_strides, d->S);
+    if (rc) return rc;
     return AETHER_OK;
 }
 
@@ -276,27 +256,33 @@ int rb_setup(RbArgs& p, const AetherRelbias* d) {
 
 using namespace aether;
 
-extern "C" int aether_relbias_attn(const AetherRelbias* d, void* o, float* lse, void* stream) {
+extern "C" int aether_relbias_attn(const AetherRelbias* d, void* o, void* o_low, float* lse, void* stream) {
     RbFwdArgs args = {};
     int rc = rb_setup(args.a, d);
     if (rc) return rc;
     if (d->B == 0 || d->S == 0) return AETHER_OK;
     if (!o) return aether_set_error(AETHER_ERR_ARG, "relbias_attn: null output");
-    if ((uintptr_t)o & 15) return aether_set_error(AETHER_ERR_ALIGN, "relbias_attn: the output must be 16-byte aligned");
+    if ((o_low != nullptr) != (lse != nullptr)) return aether_set_error(AETHER_ERR_ARG, "relbias_attn: o_low and lse are given together");
+    if (((uintptr_t)o | (uintptr_t)o_low) & 15) return aether_set_error(AETHER_ERR_ALIGN, "relbias_attn: the output must be 16-byte aligned");
     args.o = (bf16_t*)o;
+    args.o_low = (bf16_t*)o_low;
     args.lse = lse;
     RbArgs& p = args.a;
-    const size_t lds = 2 * RB_BUF + ((2 * (p.reach + RB_PAD) + 1) * 4 + 15) / 16 * 16 + (p.mask ? (size_t)(p.S + 63) / 64 * 8 : 0);
-    const long heads = (long)p.B * p.H;
+    const size_t lds = 2 * RB_BUF + rb_table_bytes(p.reach) + rb_words_bytes(p);
+    const int nw = rb_waves(p);
+    p.nqb = (p.S + nw * 32 - 1) / (nw * 32);
+    const dim3 grid((unsigned)((long)p.B * p.H * p.nqb));
     hipStream_t s = (hipStream_t)stream;
-#define RB_LAUNCH(NW)                                                                                              \
-    do {                                                                                                           \
-        p.nqb = (p.S + NW * 32 - 1) / (NW * 32);                                                                   \
-        hipLaunchKernelGGL((relbias_attn_fwd_kernel<NW>), dim3((unsigned)(heads * p.nqb)), dim3(NW * 64), lds, s, args); \
+#define RB_LAUNCH(NW)                                                                                                \
+    do {                                                                                                             \
+        if (lse) hipLaunchKernelGGL((relbias_attn_fwd_kernel<NW, true>), grid, dim3(NW * 64), lds, s, args);         \
+        else hipLaunchKernelGGL((relbias_attn_fwd_kernel<NW, false>), grid, dim3(NW * 64), lds, s, args);            \
     } while (0)
-    if (p.S > 64 && heads * ((p.S + 127) / 128) >= 256) RB_LAUNCH(4);
-    else if (p.S > 32) RB_LAUNCH(2);
-    else RB_LAUNCH(1);
+    switch (nw) {
+        case 4: RB_LAUNCH(4); break;
+        case 2: RB_LAUNCH(2); break;
+        default: RB_LAUNCH(1); break;
+    }
 #undef RB_LAUNCH
     return aether_check_launch("relbias_attn");
 }

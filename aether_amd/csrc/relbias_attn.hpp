@@ -1,4 +1,5 @@
-// What the forward and the backward pass of attention with a relative position bias share: arguments, the bias table in LDS, the key mask.
+// What the forward and the backward pass of attention with a relative position bias share: arguments, the bias table in LDS, the key mask, the layout
+// of a tile.
 #pragma once
 #include "common.hpp"
 
@@ -10,6 +11,8 @@ constexpr int RB_TILE = RB_KV * RB_D * 2;
 constexpr int RB_MAX_BORDERS = 64;
 constexpr int RB_MAX_REACH = 1024;    // largest distance whose bucket may differ from the farthest one's
 constexpr int RB_MAX_S = 65536;
+constexpr int RB_BUF = 2 * RB_TILE;   // two tiles that are staged together
+constexpr int RB_PAD = 96;            // >= 31 + 63: a wave's 32 rows against the 64 of a tile
 constexpr float RB_LOG2E = 1.4426950408889634f;
 
 // [B, S, H, 64] with any strides (elements); the last one is 1
@@ -27,13 +30,12 @@ struct RbArgs {
     int nqb;                          // query blocks per (batch, head)
 };
 
-// The bias of one head over d, in LDS in log2 units: tab[d + reach + pad], d in [-reach - pad, reach + pad]; the pad lets a tile that straddles the
+// The bias of one head over d, in LDS in log2 units: tab[d + reach + pad], d in [-reach - pad, reach + pad] (pad = RB_PAD); the pad lets a tile that straddles the
 // reach read past it without a clamp.
-template <int PAD>
 AE_DEV void rb_fill_table(const RbArgs& p, int h, float* tab, int nthreads) {
-    const int n_tab = 2 * (p.reach + PAD) + 1;
+    const int n_tab = 2 * (p.reach + RB_PAD) + 1;
     for (int i = threadIdx.x; i < n_tab; i += nthreads) {
-        const int d = i - p.reach - PAD, n = d < 0 ? -d : d;
+        const int d = i - p.reach - RB_PAD, n = d < 0 ? -d : d;
         int b = n;
         if (n >= p.near_n) {
             b = p.near_n;
@@ -68,7 +70,61 @@ AE_DEV uint64_t rb_word(const RbArgs& p, const uint64_t* words, int j) {
     return left >= 64 ? ~0ull : (1ull << left) - 1;
 }
 
-// (d, e) of the transposing LDS read: within 16 lanes, lane 4r + c names row r, elements 4c .. 4c + 3 of a 4 x 16 piece, and lane i receives column i
+// A 64 x 64 tile in LDS: 128-byte rows, the 16-byte chunk c of row r stands at c ^ swz(r).  swz takes all eight values over r's bits 1 ... 3, so that 32 rows
+// read at one chunk spread over the banks; and rows r, r + 2 differ in its bit 1, so that the 4 x 32-byte pieces of a transposing read do too.
+AE_DEV int rb_swz(int r) { return (((r >> 1) & 3) << 1) | ((r >> 3) & 1); }
+
+// the row of a 32-row half that feeds MFMA row i: the 16 results of a lane are then rows 16(r >> 3) + 8hi + (r & 7), in register order the B operand
+// of a product over these rows
+AE_DEV int rb_pi(int i) { return 16 * (i >> 4) + 8 * ((i >> 2) & 1) + 4 * ((i >> 3) & 1) + (i & 3); }
+
+// offsets of a lane's A fragments from a tile: rows in the order pi, 16 ks + 8 hi ... + 7
+AE_DEV void rb_row_offsets(int lane, int (&off)[4]) {
+    const int r = rb_pi(lane & 31), hi = lane >> 5;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) off[ks] = r * 128 + (((2 * ks + hi) ^ rb_swz(r)) << 4);
+}
+// offsets of a lane's transposed fragments: column 32 dt + (lane & 31), rows 8hi + 4f ... + 3 of 16; 16 rows further the swizzle is the same
+AE_DEV void rb_tr_offsets(int lane, int (&off)[2][2]) {
+    const int i = lane & 15, hi = lane >> 5;
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+        for (int f = 0; f < 2; ++f) {
+            const int r = 8 * hi + 4 * f + (i >> 2), chunk = dt * 4 + ((lane >> 4) & 1) * 2 + ((i & 3) >> 1);
+            off[dt][f] = r * 128 + ((chunk ^ rb_swz(r)) << 4) + (i & 1) * 8;
+        }
+}
+// zeroes the elements of a fragment of eight rows whose bit is not set
+AE_DEV bf16x8 rb_keep(bf16x8 f, unsigned bits) {
+    uint4 u = __builtin_bit_cast(uint4, f);
+    u.x &= (bits & 1 ? 0xffffu : 0u) | (bits & 2 ? 0xffff0000u : 0u);
+    u.y &= (bits & 4 ? 0xffffu : 0u) | (bits & 8 ? 0xffff0000u : 0u);
+    u.z &= (bits & 16 ? 0xffffu : 0u) | (bits & 32 ? 0xffff0000u : 0u);
+    u.w &= (bits & 64 ? 0xffffu : 0u) | (bits & 128 ? 0xffff0000u : 0u);
+    return __builtin_bit_cast(bf16x8, u);
+}
+
+// a lane's column of a 64 x 32 result (rows d = 32dt + 8(r >> 2) + 4hi + (r & 3)) times `f` -> 64 bf16 at `row`, in 16-byte pieces
+AE_DEV void rb_store(const f32x16 (&o)[2], float f, bf16_t* row, int hi, bool ok) {
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt) {
+        unsigned pk[4][2];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            pk[g][0] = pack_bf16x2(o[dt][4 * g + 0] * f, o[dt][4 * g + 1] * f);
+            pk[g][1] = pack_bf16x2(o[dt][4 * g + 2] * f, o[dt][4 * g + 3] * f);
+        }
+#pragma unroll
+        for (int g = 0; g < 4; g += 2) {
+            auto r0 = __builtin_amdgcn_permlane32_swap(pk[g][0], pk[g + 1][0], false, false);
+            auto r1 = __builtin_amdgcn_permlane32_swap(pk[g][1], pk[g + 1][1], false, false);
+            if (ok) *(uint4*)(row + 32 * dt + 8 * g + 8 * hi) = make_uint4(r0[0], r1[0], r0[1], r1[1]);
+        }
+    }
+}
+
+// The transposing LDS read: within 16 lanes, lane 4r + c names row r, elements 4c .. 4c + 3 of a 4 x 16 piece, and lane i receives column i
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 AE_DEV bf16x8 rb_read_tr(const char* a, const char* b) {
     const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)a);
@@ -78,4 +134,14 @@ AE_DEV bf16x8 rb_read_tr(const char* a, const char* b) {
     return __builtin_bit_cast(bf16x8, v);
 }
 
+}  // namespace aether
+
+struct AetherRelbias;
+namespace aether {
+inline size_t rb_table_bytes(int reach) { return (size_t)((2 * (reach + RB_PAD) + 1) * 4 + 15) / 16 * 16; }
+inline size_t rb_words_bytes(const RbArgs& p) { return p.mask ? (size_t)(p.S + 63) / 64 * 8 : 0; }
+int rb_setup(RbArgs& p, const AetherRelbias* d);   // fills the arguments; an error code and its message where the call is refused
+int rb_tensor(RbTensor& t, const void* ptr, const long* strides, int S);
+// waves of a workgroup (32 rows each): four where that still gives every CU a workgroup, else fewer
+inline int rb_waves(const RbArgs& p) { return p.S <= 32 ? 1 : p.S > 64 && (long)p.B * p.H * ((p.S + 127) / 128) >= 256 ? 4 : 2; }
 }  // namespace aether

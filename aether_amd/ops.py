@@ -314,9 +314,47 @@ def relbias_attn(q, k, v, table, max_distance=128, scale=1.0, key_mask=None, nee
     """Self-attention with a learned bias by relative position: S_ij = scale q_i·k_j + table[bucket(j − i), h], O = softmax(S) V over the keys that count.
     q, k, v bfloat16 [B, S, H, 64] (views of a packed projection included), table bfloat16 [num_buckets, H] (buckets of both directions, exact up to
     num_buckets / 4, logarithmic up to max_distance), key_mask bool [B, S], True where a key counts.  A row without keys gives 0; what stands at
-    keys that do not count reaches nothing.  -> o bfloat16 [B, S, H, 64], or (o, lse) for `relbias_attn_backward`."""
+    keys that do not count reaches nothing.  -> o bfloat16 [B, S, H, 64]; with need_lse (o, lse), where lse (float32, flat) is what
+    `relbias_attn_backward` needs besides o: the rows' log-sums to base 2 [B, H, S], then, from the next 16 bytes on, o's rounding remainders
+    (bfloat16 [B, S, H, 64]).  P then multiplies v in two parts, and o is a little more exact than without."""
     dev, d, keep = _relbias("relbias_attn", q, k, v, table, max_distance, scale, key_mask)
     o = torch.empty(q.shape, dtype=torch.bfloat16, device=dev)
-    lse = torch.empty(q.shape[0], q.shape[2], q.shape[1], dtype=torch.float32, device=dev) if need_lse else None
-    _run("relbias_attn", dev, _lib.load().aether_relbias_attn, C.byref(d), o.data_ptr(), _lib.ptr(lse))
+    n = o.numel() // 64
+    lse = torch.empty(_lse_pad(n) + 32 * n, dtype=torch.float32, device=dev) if need_lse else None
+    at = lse.data_ptr() if need_lse else None
+    _run("relbias_attn", dev, _lib.load().aether_relbias_attn, C.byref(d), o.data_ptr(), at + 4 * _lse_pad(n) if need_lse else None, at)
     return (o, lse) if need_lse else o
+
+
+def _lse_pad(n):
+    return (n + 3) // 4 * 4         # the remainders behind the log-sums begin at whole 16 bytes
+
+
+_Strides = C.c_long * 3
+
+
+def relbias_attn_backward(do, q, k, v, o, lse, table, max_distance=128, scale=1.0, key_mask=None, need_dtable=True):
+    """Gradients of `relbias_attn` from its inputs, its output o and its lse: -> (dq, dk, dv bfloat16 [B, S, H, 64], thirds of one packed
+    [B, S, 3, H, 64] buffer; dtable bfloat16 [num_buckets, H] or None).  dk and dv are 0 at keys that do not count.  Summed in an order that
+    depends on the sizes alone."""
+    name = "relbias_attn_backward"
+    dev, d, keep = _relbias(name, q, k, v, table, max_distance, scale, key_mask)
+    _same_device(q, do, o, lse)
+    B, S, H, _ = q.shape
+    for n, t in (("do", do), ("o", o)):
+        if t.dtype != torch.bfloat16 or t.shape != q.shape:
+            raise ValueError(f"{name}: {n} is bfloat16 {list(q.shape)}, got {t.dtype} {list(t.shape)}")
+    n = B * H * S
+    if lse.dtype != torch.float32 or tuple(lse.shape) != (_lse_pad(n) + 32 * n,):
+        raise ValueError(f"{name}: lse is what relbias_attn gave with need_lse, float32 [{_lse_pad(n) + 32 * n}], got {lse.dtype} {list(lse.shape)}")
+    do, o, lse = _heads(do), _heads(o), _vector(lse)
+    dqkv = torch.empty(B, S, 3, H, 64, dtype=torch.bfloat16, device=dev)
+    dq, dk, dv = dqkv.unbind(2)
+    dtable = torch.empty(table.shape, dtype=torch.bfloat16, device=dev) if need_dtable else None
+    lib = _lib.load()
+    nbytes = lib.aether_relbias_attn_bwd_workspace_bytes(C.byref(d), need_dtable)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    st = _Strides(S * 3 * H * 64, 3 * H * 64, 64)
+    _run(name, dev, lib.aether_relbias_attn_bwd, C.byref(d), do.data_ptr(), _Strides(*do.stride()[:3]), o.data_ptr(), _Strides(*o.stride()[:3]), lse.data_ptr() + 4 * _lse_pad(n), lse.data_ptr(),
+         dq.data_ptr(), st, dk.data_ptr(), st, dv.data_ptr(), st, _lib.ptr(dtable), ws.data_ptr(), nbytes)
+    return dq, dk, dv, dtable

@@ -163,8 +163,16 @@ typedef struct AetherRelbias {
     const int* borders; /* host */
     int n_borders;
 } AetherRelbias;
-/* o bf16 [B, S, H, 64] dense; lse fp32 [B, H, S] (base-2 log of the row sums, +inf for a row without keys) for the backward pass, or NULL. */
-int aether_relbias_attn(const AetherRelbias* d, void* o, float* lse, void* stream);
+/* o bf16 [B, S, H, 64] dense.  For a backward pass also o_low bf16 [B, S, H, 64] (what the rounding of o left: o + o_low is good to 2^-16) and
+ * lse fp32 [B, H, S] (base-2 log of the row sums, +inf for a row without keys); both or neither. */
+int aether_relbias_attn(const AetherRelbias* d, void* o, void* o_low, float* lse, void* stream);
+/* Backward pass: go = dO and o as above with strides of their own (batch, position, head); dq, dk, dv bf16 [B, S, H, 64] with strides of their own (they
+ * may be thirds of one packed buffer); dtable bf16 [num_buckets, H] or NULL.  dk and dv are 0 at keys that do not count.  Sums in an order that depends on
+ * the sizes alone. */
+size_t aether_relbias_attn_bwd_workspace_bytes(const AetherRelbias* d, int need_dtable);
+int aether_relbias_attn_bwd(const AetherRelbias* d, const void* go, const long* go_strides, const void* o, const long* o_strides, const void* o_low,
+                            const float* lse, void* dq, const long* dq_strides, void* dk, const long* dk_strides, void* dv, const long* dv_strides, void* dtable,
+                            void* workspace, size_t workspace_bytes, void* stream);
 
 /* Element-wise tail of one denoise step in ONE pass (aetherv1_pipeline_cogvideox.py:876-916): fp32 cast of the noise prediction (P:877),
  * classifier-free-guidance combine uncond + g·(cond − uncond) when nb = 2 (P:895-899), CogVideoXDPMScheduler.step for v-prediction

@@ -76,12 +76,12 @@ def test_wrappers_refuse_host_tensors(hip_lib):
 def _relbias(lib, o=4096, **kw):
     import ctypes as C
     from aether_amd import _lib
-    a = dict(q=4096, k=4096, v=4096, st=(64 * 64, 64, 64 * 32), table=4096, mask=None, B=1, S=32, H=2, num_buckets=32, borders=(12, 16, 23, 32, 46, 64, 91))
+    a = dict(low=None, lse=None, q=4096, k=4096, v=4096, st=(64 * 64, 64, 64 * 32), table=4096, mask=None, B=1, S=32, H=2, num_buckets=32, borders=(12, 16, 23, 32, 46, 64, 91))
     a.update(kw)
     b = a["borders"]
     arr = (C.c_int * len(b))(*b) if b is not None else None
     d = _lib.AetherRelbias(a["q"], a["k"], a["v"], a["st"], a["st"], a["st"], a["table"], a["mask"], 0, a["B"], a["S"], a["H"], 1.0, a["num_buckets"], arr, len(b or ()))
-    return lib.aether_relbias_attn(C.byref(d), o, None, None)
+    return lib.aether_relbias_attn(C.byref(d), o, a["low"], a["lse"], None)
 
 
 @pytest.mark.parametrize("kw,code,text", [
@@ -91,7 +91,7 @@ def _relbias(lib, o=4096, **kw):
     (dict(borders=(12, 11, 23, 32, 46, 64, 91)), -1, b"borders"), (dict(borders=(12, 16, 23, 32, 46, 64, 1025)), -2, b"1024"),
     (dict(table=None), -1, b"table"), (dict(q=None), -1, b"operand"), (dict(v=None), -1, b"operand"), (dict(k=4104), -3, b"aligned"),
     (dict(st=(4096, 60, 64)), -3, b"aligned"), (dict(st=(4096, -64, 64)), -2, b"stride"), (dict(st=(-4096, 64, 64)), -2, b"stride"),
-    (dict(st=(0, 1 << 15, 64), S=65536), -2, b"4 GiB"), (dict(o=None), -1, b"output"), (dict(o=4104), -3, b"aligned"),
+    (dict(st=(0, 1 << 15, 64), S=65536), -2, b"4 GiB"), (dict(o=None), -1, b"output"), (dict(low=4096), -1, b"together"), (dict(lse=4096), -1, b"together"), (dict(low=4104, lse=4096), -3, b"aligned"), (dict(o=4104), -3, b"aligned"),
     (dict(B=1 << 20, H=1 << 10, S=65536), -2, b"blocks"),
 ])
 def test_relbias_entry_refuses(hip_lib, kw, code, text):
@@ -100,7 +100,7 @@ def test_relbias_entry_refuses(hip_lib, kw, code, text):
 
 def test_relbias_entry_without_rows(hip_lib):
     assert _relbias(hip_lib, S=0, q=None, table=None, o=None) == 0 and _relbias(hip_lib, B=0, q=None, table=None, o=None) == 0
-    assert hip_lib.aether_relbias_attn(None, 4096, None, None) == -1
+    assert hip_lib.aether_relbias_attn(None, 4096, None, None, None) == -1
 
 
 def test_bucket_borders():
@@ -124,3 +124,22 @@ def test_bucket_borders():
     for nb, md in ((2, 10), (5, 10), (130, 1000), (32, 8), (32, 7), (32, 128.5), (32, 100000)):
         with pytest.raises(ValueError):
             relbias_borders(nb, md)
+
+
+@pytest.mark.parametrize("kw,code,text", [
+    (dict(lse=None), -1, b"lse"), (dict(low=None), -1, b"o_low"), (dict(low=4104), -3, b"aligned"), (dict(go=None), -1, b"operand"), (dict(o=4100), -3, b"aligned"), (dict(dq=None), -1, b"operand"),
+    (dict(st=(4096, 4, 64)), -3, b"aligned"), (dict(ws=None), -1, b"workspace"), (dict(ws=4104), -1, b"workspace"), (dict(n=32 * 2 * 4 + 255), -1, b"workspace"),
+])
+def test_relbias_backward_entry_refuses(hip_lib, kw, code, text):
+    import ctypes as C
+    from aether_amd import _lib
+    a = dict(go=4096, o=4096, low=4096, lse=4096, dq=4096, dk=4096, dv=4096, dt=4096, ws=4096, n=1 << 20, st=(64 * 64, 64, 64 * 32))
+    a.update(kw)
+    b = (C.c_int * 7)(12, 16, 23, 32, 46, 64, 91)
+    ok = (64 * 64, 64, 64 * 32)
+    d = _lib.AetherRelbias(4096, 4096, 4096, ok, ok, ok, 4096, None, 0, 1, 32, 2, 1.0, 32, b, 7)
+    assert hip_lib.aether_relbias_attn_bwd_workspace_bytes(C.byref(d), 1) == 32 * 2 * 4 + 2 * 32 * 4
+    assert hip_lib.aether_relbias_attn_bwd_workspace_bytes(C.byref(d), 0) == 32 * 2 * 4
+    st = (C.c_long * 3)(*a["st"])
+    rc = hip_lib.aether_relbias_attn_bwd(C.byref(d), a["go"], st, a["o"], st, a["low"], a["lse"], a["dq"], st, a["dk"], st, a["dv"], st, a["dt"], a["ws"], a["n"], None)
+    assert rc == code and text in hip_lib.aether_last_error()
