@@ -20,6 +20,8 @@ AETHER_VAE_TWO_LANES = 256    # VAE plan: tile batches of two on two streams (se
 AETHER_CONV_TAP_REUSE = 128   # conv: K order is (dt, dh, channel block, dw) -> the tap-reuse kernel may be used
 AETHER_STREAM_BF16 = 0         # type of a residual stream (rms_norm)
 AETHER_STREAM_FP32 = 1
+AETHER_ACT_GELU_TANH = 0       # activation of gated_ff
+AETHER_ACT_SILU = 1
 ATTN_Q_SCALE = 0.125 * 1.4426950408889634   # softmax scale x log2(e): the attention kernel works in the log2 domain
 PROF_CLASSES = ["other", "layernorm", "gemm_qkv", "qk_norm_rope", "attention", "gemm_out", "gemm_ff1", "gemm_ff2"]
 
@@ -71,6 +73,10 @@ SIGNATURES = {
     "aether_relbias_attn": (_i, [C.POINTER(AetherRelbias), _vp, _vp, _fp, _vp]),
     "aether_relbias_attn_bwd_workspace_bytes": (_sz, [C.POINTER(AetherRelbias), _i]),
     "aether_relbias_attn_bwd": (_i, [C.POINTER(AetherRelbias), _vp, _lp, _vp, _lp, _vp, _fp, _vp, _lp, _vp, _lp, _vp, _lp, _vp, _vp, _sz, _vp]),
+    "aether_gated_ff": (_i, [_vp, _l, _vp, _vp, _l, _vp, _l, _fp, _i, _i, _i, _i, _vp]),
+    "aether_gated_ff_e4m3": (_i, [_vp, _l, _fp, _vp, _fp, _vp, _fp, _l, _vp, _l, _i, _i, _i, _i, _vp]),
+    "aether_gated_ff_bwd_workspace_bytes": (_sz, [_i, _i, _i]),
+    "aether_gated_ff_bwd": (_i, [_vp, _l, _vp, _l, _vp, _vp, _l, _fp, _vp, _l, _vp, _i, _i, _i, _i, _vp, _sz, _vp]),
     "aether_dpm_step": (_i, [_vp, _i, _f, _vp, _fp, _vp, _f, _f, _f, _f, _f, _f, _f, _fp, _fp, _vp, C.c_long, _vp]),
     "aether_conv_gemm_bf16": (_i, [_vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _i, _vp, _i, _vp, _i, _fp, _vp, _i, _fp, _sz, _i, _vp]),
     "aether_im2col_first": (_i, [_vp, C.c_long, C.c_long, C.c_long, C.c_long, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _i, _vp]),

@@ -1,0 +1,385 @@
+// Gated feed-forward product:  h = act(x Wgᵀ) ⊙ (x Wuᵀ),  x [M, K], Wg and Wu [F, K] (rows are output features), h bf16 [M, F]; act = tanh-GELU or
+// SiLU; operands in bf16, or in e4m3 with one scale per row of x, Wg and Wu.  And its backward pass.
+//
+// One kernel: the W tile of a workgroup holds, for each group of 32 output columns, 32 rows of Wg and the same 32 rows of Wu, so that both products of an
+// element end up in the same lane's accumulators; activation, product and rounding happen in registers and neither projection goes to memory
+// (for a backward pass both are also written, in fp32: rounding them to bf16 there would cost the gradients as much again as rounding the
+// gradients does).
+//
+// Main loop: 8 waves as WM x WN; a wave owns MT·32 rows and 32 pairs of columns on v_mfma_f32_32x32x16_bf16, or v_mfma_..._32x32x64_f8f6f4 for e4m3.  A K tile is
+// 128 bytes of every row either way.  Tiles come by 16-byte LDS-DMA into two buffers; 128-byte LDS rows are XOR-swizzled in 16-byte chunks.  The two
+// waves that share a SIMD alternate: one reads its next fragments and issues the next tile's DMA while the other feeds the matrix pipe.
+#include <type_traits>
+#include "common.hpp"
+#include "../../include/aether_hip.h"
+
+namespace aether {
+
+typedef unsigned char u8_t;
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+struct FfArgs {
+    const void* x; long ldx;             // elements
+    const void* wg; const void* wu; long ldw;
+    const float* sx; const float* sg; const float* su;   // e4m3: scale of each row
+    bf16_t* h; long ldh;
+    float* gu;                           // fp32 [M][2F]: both projections, or null
+    int M, F, K;
+    unsigned x_bytes, w_bytes;
+    int tiles_m, tiles_n;
+};
+
+enum { ACT_GELU_TANH = AETHER_ACT_GELU_TANH, ACT_SILU = AETHER_ACT_SILU };
+
+// sigma(t) = 1 / (1 + e^-t)
+AE_DEV float ff_sigmoid(float t) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * t)); }
+// tanh-GELU(g) = g · sigma(2u), u = sqrt(2/pi) (g + 0.044715 g³): the argument of sigma, and its slope in g
+AE_DEV float ff_gelu_arg(float g) { return 1.5957691216057308f * (g + 0.044715f * g * g * g); }
+template <int ACT>
+AE_DEV float ff_act(float g) {
+    return g * ff_sigmoid(ACT == ACT_SILU ? g : ff_gelu_arg(g));
+}
+// act(g) and act'(g) = s + g s (1 − s) t'(g) with s = sigma(t(g)); where s is 0 or 1 the second term is 0 whatever t' is
+template <int ACT>
+AE_DEV void ff_act_slope(float g, float& a, float& slope) {
+    const float s = ff_sigmoid(ACT == ACT_SILU ? g : ff_gelu_arg(g));
+    const float dt = ACT == ACT_SILU ? 1.0f : 1.5957691216057308f * (1.0f + 0.134145f * g * g);
+    const float c = s * (1.0f - s);
+    a = g * s;
+    slope = s + (c == 0.f ? 0.f : g * c * dt);
+}
+
+template <class ET> struct FfType;
+template <> struct FfType<bf16_t> { static constexpr int SIZE = 2, SLOTS = 4, CHUNKS = 1; };   // per K tile: MFMA steps, 16-byte chunks a lane reads per step
+template <> struct FfType<u8_t> { static constexpr int SIZE = 1, SLOTS = 2, CHUNKS = 2; };
+
+AE_DEV f32x16 ff_mfma(const i32x4 (&a)[1], const i32x4 (&b)[1], f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a[0]), __builtin_bit_cast(bf16x8, b[0]), c, 0, 0, 0);
+}
+AE_DEV f32x16 ff_mfma(const i32x4 (&a)[2], const i32x4 (&b)[2], f32x16 c) {
+    const i32x8 x = {a[0][0], a[0][1], a[0][2], a[0][3], a[1][0], a[1][1], a[1][2], a[1][3]};
+    const i32x8 y = {b[0][0], b[0][1], b[0][2], b[0][3], b[1][0], b[1][1], b[1][2], b[1][3]};
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x, y, c, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);   // block scales 2^0
+}
+
+// (g, u) of one lane: 16 rows' worth of a 32 x 32 result, column (= row of x) l32, n = 8(r >> 2) + 4hi + (r & 3)
+template <class ET, int ACT>
+AE_DEV void ff_finish(const FfArgs& p, f32x16 g, f32x16 u, int m, int n0, int hi) {
+    const bool ok = m < p.M;
+    const size_t row = (size_t)min(m, p.M - 1);
+    if constexpr (std::is_same<ET, u8_t>::value) {
+        const float sx = p.sx[row];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const f32x4 a = *(const f32x4*)(p.sg + n0 + 8 * q + 4 * hi), b = *(const f32x4*)(p.su + n0 + 8 * q + 4 * hi);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { g[4 * q + e] *= sx * a[e]; u[4 * q + e] *= sx * b[e]; }
+        }
+    }
+    if (p.gu && ok) {
+        float* const gp = p.gu + row * (2 * (size_t)p.F) + n0 + 4 * hi;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            *(f32x4*)(gp + 8 * q) = f32x4{g[4 * q], g[4 * q + 1], g[4 * q + 2], g[4 * q + 3]};
+            *(f32x4*)(gp + p.F + 8 * q) = f32x4{u[4 * q], u[4 * q + 1], u[4 * q + 2], u[4 * q + 3]};
+        }
+    }
+    unsigned pk[4][2];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        pk[q][0] = pack_bf16x2(ff_act<ACT>(g[4 * q]) * u[4 * q], ff_act<ACT>(g[4 * q + 1]) * u[4 * q + 1]);
+        pk[q][1] = pack_bf16x2(ff_act<ACT>(g[4 * q + 2]) * u[4 * q + 2], ff_act<ACT>(g[4 * q + 3]) * u[4 * q + 3]);
+    }
+#pragma unroll
+    for (int q = 0; q < 4; q += 2) {
+        auto r0 = __builtin_amdgcn_permlane32_swap(pk[q][0], pk[q + 1][0], false, false);
+        auto r1 = __builtin_amdgcn_permlane32_swap(pk[q][1], pk[q + 1][1], false, false);
+        if (ok) *(uint4*)(p.h + row * p.ldh + n0 + 8 * q + 8 * hi) = make_uint4(r0[0], r1[0], r0[1], r1[1]);
+    }
+}
+
+template <class ET, int WM, int WN, int MT, int ACT>
+__global__ __launch_bounds__(512) void gated_ff_kernel(FfArgs p) {
+    static_assert(WM * WN == 8, "8 wavefronts per workgroup");
+    constexpr int BM = WM * MT * 32, BN = WN * 32;                    // rows, pairs of columns
+    constexpr int X_TILE = BM * 128, W_TILE = WN * 64 * 128, BUF = X_TILE + W_TILE;
+    constexpr int X_ROUNDS = BM / 64, W_ROUNDS = WN;
+    constexpr int SLOTS = FfType<ET>::SLOTS, CH = FfType<ET>::CHUNKS, ES = FfType<ET>::SIZE;
+    __shared__ __attribute__((aligned(16))) char smem[2 * BUF];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / WN, wn = wave % WN, hi = lane >> 5, l32 = lane & 31;
+    const int wave_s = __builtin_amdgcn_readfirstlane(wave);
+    // XCD-aware remap, then groups of four row tiles x all column tiles, row tile fastest: neighbours share W tiles in their L2
+    int tile_m, tile_n;
+    {
+        const int id = xcd_remap((int)blockIdx.x, p.tiles_m * p.tiles_n);
+        const int group = id / (4 * p.tiles_n), gsz = min(4, p.tiles_m - group * 4), in = id - group * 4 * p.tiles_n;
+        tile_m = group * 4 + in % gsz;
+        tile_n = in / gsz;
+    }
+    const int m0 = tile_m * BM, n0 = tile_n * BN;
+
+    // ---- staging: a wave-instruction moves 8 rows x 128 bytes; waves 0-3 carry rows of Wg, waves 4-7 the same rows of Wu ----
+    const int srow = wave * 8 + (lane >> 3);
+    const unsigned schunk = ((lane & 7) ^ ((srow >> 1) & 7)) * 16;
+    unsigned x_off[X_ROUNDS], w_off[W_ROUNDS];
+#pragma unroll
+    for (int r = 0; r < X_ROUNDS; ++r) x_off[r] = (unsigned)min(m0 + r * 64 + srow, p.M - 1) * (unsigned)(p.ldx * ES) + schunk;
+#pragma unroll
+    for (int r = 0; r < W_ROUNDS; ++r) w_off[r] = (unsigned)min(n0 + r * 32 + (srow & 31), p.F - 1) * (unsigned)(p.ldw * ES) + schunk;
+    const buf_rsrc_t x_rsrc = make_buf_rsrc(p.x, p.x_bytes), w_rsrc = make_buf_rsrc(wave_s < 4 ? p.wg : p.wu, p.w_bytes);
+    char* const lds_stage = smem + wave_s * 1024;
+    const int nk = p.K * ES / 128;
+    constexpr int NP = X_ROUNDS + W_ROUNDS, NPART = SLOTS > 2 ? 3 : 1;
+    // past the last K tile the staging fetches that tile again, into the buffer that nobody reads any more: no branch, the same counts of loads
+    auto stage_part = [&](int kt, int buf, int part, int nparts) {
+        const unsigned soff = 128u * (unsigned)min(kt, nk - 1);
+        char* const dst = lds_stage + buf * BUF;
+#pragma unroll
+        for (int r = 0; r < X_ROUNDS; ++r)
+            if (r * nparts / NP == part) bglds16(x_rsrc, x_off[r], soff, dst + r * 8192);
+#pragma unroll
+        for (int r = 0; r < W_ROUNDS; ++r)
+            if ((X_ROUNDS + r) * nparts / NP == part) bglds16(w_rsrc, w_off[r], soff, dst + X_TILE + r * 8192);
+    };
+    // ---- fragments ----
+    const int swz = (lane >> 1) & 7;
+    const int x_row = (wm * MT * 32 + l32) * 128, w_row = X_TILE + (wn * 64 + l32) * 128;
+    i32x4 wf[2][CH], xf[MT][CH];
+    auto load_frags = [&](const char* base, int slot) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int off = ((2 * (slot * CH + c) + hi) ^ swz) << 4;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) wf[t][c] = *(const i32x4*)(base + w_row + t * 4096 + off);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) xf[mt][c] = *(const i32x4*)(base + x_row + mt * 4096 + off);
+        }
+    };
+    f32x16 acc[MT][2];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) { acc[mt][0][i] = 0.f; acc[mt][1][i] = 0.f; }
+    auto mma = [&]() {
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) acc[mt][t] = ff_mfma(wf[t], xf[mt], acc[mt][t]);
+        __builtin_amdgcn_s_setprio(0);
+    };
+    auto slot_end = [&]() {
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    stage_part(0, 0, 0, 1);
+    drain_and_barrier();
+    // Waves 0-3 load in slots 0, 2, 4 ... and compute in 1, 3, 5 ...; waves 4-7 one slot later.  With 2·SLOTS slots a tile, the last read of tile kt − 1 lies in
+    // slot 2·SLOTS·kt − 1: its buffer is free for all of tile kt.  The DMA of tile kt + 1 is waited for before the barrier that ends tile kt.
+    if (wave_s < 4) {
+        for (int kt = 0; kt < nk; ++kt) {
+            const char* base = smem + (kt & 1) * BUF;
+#pragma unroll
+            for (int sl = 0; sl < SLOTS; ++sl) {
+                load_frags(base, sl);
+                if (sl < NPART) stage_part(kt + 1, (kt + 1) & 1, sl, NPART);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                slot_end();
+                mma();
+                if (sl == SLOTS - 1) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                slot_end();
+            }
+        }
+    } else {
+        for (int kt = 0; kt < nk; ++kt) {
+            const char* base = smem + (kt & 1) * BUF;
+            if (kt > 0) mma();
+            slot_end();
+#pragma unroll
+            for (int sl = 0; sl < SLOTS; ++sl) {
+                load_frags(base, sl);
+                if (sl < NPART) stage_part(kt + 1, (kt + 1) & 1, sl, NPART);
+                if (sl == SLOTS - 1) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                slot_end();
+                if (sl < SLOTS - 1) {
+                    mma();
+                    slot_end();
+                }
+            }
+        }
+        mma();
+    }
+    const int n = n0 + wn * 32;
+    if (n >= p.F) return;                                             // F % 32 == 0: a wave's columns are all in or all out
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) ff_finish<ET, ACT>(p, acc[mt][0], acc[mt][1], m0 + (wm * MT + mt) * 32 + l32, n, hi);
+}
+
+// ---- backward ------------------------------------------------------------------------------------------------------------------------------
+// dg = dh u act'(g), du = dh act(g), as [M][2F] for the product with the weights and transposed, [2F][Mp], for the one with x.  A workgroup turns a
+// 64 x 64 piece through LDS.  Columns M ... Mp − 1 of the transposed form are zeros.
+template <int ACT>
+__global__ __launch_bounds__(256) void gated_ff_dgu_kernel(const float* __restrict__ gu, const bf16_t* __restrict__ dh, long lddh, int M, int F, int Mp,
+                                                           bf16_t* __restrict__ dgu, bf16_t* __restrict__ dgut) {
+    __shared__ unsigned short t[2][64][66];
+    const int m0 = blockIdx.y * 64, f0 = blockIdx.x * 64;
+    for (int i = threadIdx.x; i < 64 * 16; i += 256) {                // four columns at a time
+        const int r = i >> 4, c = (i & 15) * 4, m = m0 + r, f = f0 + c;
+        unsigned short g4[4] = {0, 0, 0, 0}, u4[4] = {0, 0, 0, 0};
+        if (m < M && f < F) {
+            const f32x4 g = *(const f32x4*)(gu + (size_t)m * 2 * F + f), u = *(const f32x4*)(gu + (size_t)m * 2 * F + F + f);
+            const u16x4 d = *(const u16x4*)((const unsigned short*)dh + (size_t)m * lddh + f);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float a, slope;
+                ff_act_slope<ACT>(g[e], a, slope);
+                const float dd = bf16_bits_to_f32(d[e]);
+                g4[e] = f32_to_bf16_bits(dd * u[e] * slope);
+                u4[e] = f32_to_bf16_bits(dd * a);
+            }
+            *(u16x4*)((unsigned short*)dgu + (size_t)m * 2 * F + f) = u16x4{g4[0], g4[1], g4[2], g4[3]};
+            *(u16x4*)((unsigned short*)dgu + (size_t)m * 2 * F + F + f) = u16x4{u4[0], u4[1], u4[2], u4[3]};
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { t[0][r][c + e] = g4[e]; t[1][r][c + e] = u4[e]; }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * 64 * 16; i += 256) {
+        const int which = i >> 10, c = (i >> 4) & 63, r = (i & 15) * 4;
+        if (f0 + c >= F) continue;
+        u16x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = t[which][r + e][c];
+        *(u16x4*)((unsigned short*)dgut + ((size_t)which * F + f0 + c) * Mp + m0 + r) = v;
+    }
+}
+
+// out[c][r] = in[r][c] for r < rows, 0 for rows <= r < fill
+__global__ __launch_bounds__(256) void transpose_bf16_kernel(const bf16_t* __restrict__ in, long ldi, int rows, int cols, bf16_t* __restrict__ out, long ldo, int fill) {
+    __shared__ unsigned short t[64][66];
+    const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
+    for (int i = threadIdx.x; i < 64 * 16; i += 256) {
+        const int r = i >> 4, c = (i & 15) * 4;
+        u16x4 v = {0, 0, 0, 0};
+        if (r0 + r < rows && c0 + c < cols) v = *(const u16x4*)((const unsigned short*)in + (size_t)(r0 + r) * ldi + c0 + c);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[r][c + e] = v[e];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 64 * 16; i += 256) {
+        const int c = i >> 4, r = (i & 15) * 4;
+        if (c0 + c >= cols || r0 + r >= fill) continue;        // (fill is a multiple of 4)
+        u16x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = t[r + e][c];
+        *(u16x4*)((unsigned short*)out + (size_t)(c0 + c) * ldo + r0 + r) = v;
+    }
+}
+
+static int ff_check(const void* x, long ldx, const void* wg, const void* wu, long ldw, int M, int F, int K, int act, int size) {
+    if (act != ACT_GELU_TANH && act != ACT_SILU) return aether_set_error(AETHER_ERR_ARG, "gated_ff: unknown activation");
+    if (M < 0 || F <= 0 || K <= 0) return aether_set_error(AETHER_ERR_SHAPE, "gated_ff: M must not be negative, F and K must be positive");
+    if (F % 32 || (long)K * size % 128) return aether_set_error(AETHER_ERR_SHAPE, "gated_ff: F must be a multiple of 32, K of 64 (bf16) or 128 (e4m3)");
+    if (M > (1 << 30) || (size_t)M * F >= (1ull << 46)) return aether_set_error(AETHER_ERR_SHAPE, "gated_ff: too many rows");
+    if (M == 0) return AETHER_OK;
+    if (!x || !wg || !wu) return aether_set_error(AETHER_ERR_ARG, "gated_ff: null operand");
+    if (ldx < K || ldw < K) return aether_set_error(AETHER_ERR_SHAPE, "gated_ff: a leading dimension is shorter than a row");
+    if (ldx * size % 16 || ldw * size % 16 || (((uintptr_t)x | (uintptr_t)wg | (uintptr_t)wu) & 15)) return aether_set_error(AETHER_ERR_ALIGN, "gated_ff: rows must be 16-byte aligned");
+    if ((size_t)F * ldw * size >= (1ull << 32)) return aether_set_error(AETHER_ERR_SHAPE, "gated_ff: a weight must be below 4 GiB (the reach of a buffer descriptor)");
+    if ((size_t)ldx * size * 256 >= (1ull << 32)) return aether_set_error(AETHER_ERR_SHAPE, "gated_ff: a row of x is too far from the next");
+    return AETHER_OK;
+}
+
+template <class ET>
+static int ff_forward(FfArgs p, int act, hipStream_t s) {
+    constexpr int ES = FfType<ET>::SIZE;
+    p.w_bytes = (unsigned)(((size_t)(p.F - 1) * p.ldw + p.K) * ES);
+    // rows in launches whose part of x a buffer descriptor reaches
+    const int M = p.M, most = (int)((((1ull << 32) - 1) / ((size_t)p.ldx * ES)) / 256 * 256);
+    const FfArgs whole = p;
+    for (int m = 0; m < M; m += most) {
+        p.M = M - m < most ? M - m : most;
+        p.x = (const char*)whole.x + (size_t)m * p.ldx * ES;
+        p.sx = whole.sx ? whole.sx + m : nullptr;
+        p.h = whole.h + (size_t)m * p.ldh;
+        p.gu = whole.gu ? whole.gu + (size_t)m * 2 * p.F : nullptr;
+        p.x_bytes = (unsigned)(((size_t)(p.M - 1) * p.ldx + p.K) * ES);
+#define FF_LAUNCH(WM, WN, MT)                                                                                                          \
+    do {                                                                                                                               \
+        p.tiles_m = (p.M + WM * MT * 32 - 1) / (WM * MT * 32);                                                                         \
+        p.tiles_n = (p.F + WN * 32 - 1) / (WN * 32);                                                                                   \
+        const dim3 grid(p.tiles_m * p.tiles_n);                                                                                        \
+        if (act == ACT_SILU) hipLaunchKernelGGL((gated_ff_kernel<ET, WM, WN, MT, ACT_SILU>), grid, dim3(512), 0, s, p);                \
+        else hipLaunchKernelGGL((gated_ff_kernel<ET, WM, WN, MT, ACT_GELU_TANH>), grid, dim3(512), 0, s, p);                           \
+    } while (0)
+        FF_LAUNCH(2, 4, 4);
+#undef FF_LAUNCH
+        int rc = aether_check_launch("gated_ff");
+        if (rc) return rc;
+    }
+    return AETHER_OK;
+}
+
+}  // namespace aether
+
+using namespace aether;
+
+extern "C" int aether_gated_ff(const void* x, long ldx, const void* wg, const void* wu, long ldw, void* h, long ldh, float* gu, int M, int F, int K, int act, void* stream) {
+    int rc = ff_check(x, ldx, wg, wu, ldw, M, F, K, act, 2);
+    if (rc || M == 0) return rc;
+    if (!h) return aether_set_error(AETHER_ERR_ARG, "gated_ff: null output");
+    if (ldh < F || ldh % 8 || (((uintptr_t)h | (uintptr_t)gu) & 15)) return aether_set_error(AETHER_ERR_ALIGN, "gated_ff: rows of the output must be 16-byte aligned");
+    FfArgs p = {x, ldx, wg, wu, ldw, nullptr, nullptr, nullptr, (bf16_t*)h, ldh, gu, M, F, K};
+    return ff_forward<bf16_t>(p, act, (hipStream_t)stream);
+}
+
+extern "C" int aether_gated_ff_e4m3(const void* x, long ldx, const float* x_scale, const void* wg, const float* wg_scale, const void* wu, const float* wu_scale, long ldw,
+                                    void* h, long ldh, int M, int F, int K, int act, void* stream) {
+    int rc = ff_check(x, ldx, wg, wu, ldw, M, F, K, act, 1);
+    if (rc || M == 0) return rc;
+    if (!h || !x_scale || !wg_scale || !wu_scale) return aether_set_error(AETHER_ERR_ARG, "gated_ff_e4m3: null output or scale");
+    if (ldh < F || ldh % 8 || (((uintptr_t)h | (uintptr_t)wg_scale | (uintptr_t)wu_scale) & 15) || ((uintptr_t)x_scale & 3))
+        return aether_set_error(AETHER_ERR_ALIGN, "gated_ff_e4m3: rows of the output and the weights' scales must be 16-byte aligned");
+    FfArgs p = {x, ldx, wg, wu, ldw, x_scale, wg_scale, wu_scale, (bf16_t*)h, ldh, nullptr, M, F, K};
+    return ff_forward<u8_t>(p, act, (hipStream_t)stream);
+}
+
+extern "C" size_t aether_gated_ff_bwd_workspace_bytes(int M, int F, int K) {
+    if (M <= 0 || F <= 0 || K <= 0) return 0;
+    const size_t Mp = ((size_t)M + 63) / 64 * 64;
+    return 2 * ((size_t)M * 2 * F + 2 * (size_t)F * Mp + (size_t)K * Mp + (size_t)K * 2 * F) + 4 * 256;
+}
+
+extern "C" int aether_gated_ff_bwd(const void* dh, long lddh, const void* x, long ldx, const void* wg, const void* wu, long ldw, const float* gu, void* dx, long lddx,
+                                   void* dw, int M, int F, int K, int act, void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = ff_check(x, ldx, wg, wu, ldw, M, F, K, act, 2);
+    if (rc) return rc;
+    if (!dw || (M > 0 && (!dh || !gu || !dx))) return aether_set_error(AETHER_ERR_ARG, "gated_ff_bwd: null operand");
+    if (M == 0) return aether_set_error(AETHER_ERR_SHAPE, "gated_ff_bwd: no rows");
+    if (lddh < F || lddh % 8 || lddx < K || lddx % 8 || (((uintptr_t)dh | (uintptr_t)gu | (uintptr_t)dx | (uintptr_t)dw | (uintptr_t)workspace) & 15))
+        return aether_set_error(AETHER_ERR_ALIGN, "gated_ff_bwd: rows must be 16-byte aligned");
+    const size_t Mp = ((size_t)M + 63) / 64 * 64;
+    if (Mp * 2 * F * 2 >= (1ull << 32) || (size_t)2 * F * K * 2 >= (1ull << 32)) return aether_set_error(AETHER_ERR_SHAPE, "gated_ff_bwd: M·2F and 2F·K elements must stay below 4 GiB");
+    if (!workspace || workspace_bytes < aether_gated_ff_bwd_workspace_bytes(M, F, K)) return aether_set_error(AETHER_ERR_ARG, "gated_ff_bwd: workspace too small (aether_gated_ff_bwd_workspace_bytes)");
+    hipStream_t s = (hipStream_t)stream;
+    auto up = [](char* p) { return (char*)(((uintptr_t)p + 255) & ~(uintptr_t)255); };
+    char* w = up((char*)workspace);
+    bf16_t* dgu = (bf16_t*)w; w = up(w + (size_t)M * 2 * F * 2);
+    bf16_t* dgut = (bf16_t*)w; w = up(w + 2 * (size_t)F * Mp * 2);
+    bf16_t* xt = (bf16_t*)w; w = up(w + (size_t)K * Mp * 2);
+    bf16_t* wt = (bf16_t*)w;
+    const dim3 eg((F + 63) / 64, (unsigned)(Mp / 64));
+    if (act == ACT_SILU) hipLaunchKernelGGL((gated_ff_dgu_kernel<ACT_SILU>), eg, dim3(256), 0, s, gu, (const bf16_t*)dh, lddh, M, F, (int)Mp, dgu, dgut);
+    else hipLaunchKernelGGL((gated_ff_dgu_kernel<ACT_GELU_TANH>), eg, dim3(256), 0, s, gu, (const bf16_t*)dh, lddh, M, F, (int)Mp, dgu, dgut);
+    hipLaunchKernelGGL(transpose_bf16_kernel, dim3((K + 63) / 64, (unsigned)(Mp / 64)), dim3(256), 0, s, (const bf16_t*)x, ldx, M, K, xt, (long)Mp, (int)Mp);
+    hipLaunchKernelGGL(transpose_bf16_kernel, dim3((K + 63) / 64, (F + 63) / 64), dim3(256), 0, s, (const bf16_t*)wg, ldw, F, K, wt, 2 * (long)F, F);
+    hipLaunchKernelGGL(transpose_bf16_kernel, dim3((K + 63) / 64, (F + 63) / 64), dim3(256), 0, s, (const bf16_t*)wu, ldw, F, K, wt + F, 2 * (long)F, F);
+    rc = aether_check_launch("gated_ff_bwd");
+    if (rc) return rc;
+    rc = aether_gemm_bf16(dgu, 2 * F, wt, 2 * F, dx, (int)lddx, M, K, 2 * F, nullptr, AETHER_EPI_BIAS, nullptr, 0, nullptr, nullptr, 0, 0, 0, nullptr, 0, 0, stream);
+    if (rc) return rc;
+    return aether_gemm_bf16(dgut, (int)Mp, xt, (int)Mp, dw, K, 2 * F, K, (int)Mp, nullptr, AETHER_EPI_BIAS, nullptr, 0, nullptr, nullptr, 0, 0, 0, nullptr, 0, 0, stream);
+}

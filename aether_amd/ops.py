@@ -154,12 +154,12 @@ def _run(what, dev, fn, *args):
         _lib.check(rc, what)
 
 
-def _rows(t, width, align=16):
-    """`t` as [rows, width] with unit stride, a row stride of whole 16-byte pieces (8 elements) and an aligned base; copied only where it is not so."""
+def _rows(t, width):
+    """`t` as [rows, width] with unit stride, an aligned base and rows a multiple of 8 elements and of 16 bytes apart; copied only where it is not so."""
     if t.dim() != 2:
         t = t.reshape(-1, width)
     by, one = t.stride()
-    if one != 1 or by % 8 or (by < width and t.shape[0] > 1) or t.data_ptr() % align:
+    if one != 1 or by % 8 or by * t.element_size() % 16 or by < width or t.data_ptr() % 16:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -358,3 +358,83 @@ def relbias_attn_backward(do, q, k, v, o, lse, table, max_distance=128, scale=1.
     _run(name, dev, lib.aether_relbias_attn_bwd, C.byref(d), do.data_ptr(), _Strides(*do.stride()[:3]), o.data_ptr(), _Strides(*o.stride()[:3]), lse.data_ptr() + 4 * _lse_pad(n), lse.data_ptr(),
          dq.data_ptr(), st, dk.data_ptr(), st, dv.data_ptr(), st, _lib.ptr(dtable), ws.data_ptr(), nbytes)
     return dq, dk, dv, dtable
+
+
+_ACTS = {"gelu_tanh": _lib.AETHER_ACT_GELU_TANH, "silu": _lib.AETHER_ACT_SILU}
+
+
+def _ff_operands(name, x, wg, wu, act, dtype):
+    if act not in _ACTS:
+        raise ValueError(f"{name}: act is one of {list(_ACTS)}, got {act!r}")
+    if x.dtype != dtype or wg.dtype != dtype or wu.dtype != dtype:
+        raise ValueError(f"{name}: x, wg and wu are {dtype}, got {x.dtype}, {wg.dtype}, {wu.dtype}")
+    if x.dim() < 1 or wg.dim() != 2 or wg.shape != wu.shape or wg.shape[1] != x.shape[-1]:
+        raise ValueError(f"{name}: x [..., K], wg and wu [F, K], got {list(x.shape)}, {list(wg.shape)}, {list(wu.shape)}")
+    F, K = wg.shape
+    if F == 0 or F % 32 or K == 0 or K * x.element_size() % 128:
+        raise ValueError(f"{name}: F must be a multiple of 32 and K of {128 // x.element_size()}, got F = {F}, K = {K}")
+    wg, wu = _rows(wg, K), _rows(wu, K)
+    if wg.stride(0) != wu.stride(0):
+        wg, wu = wg.contiguous(), wu.contiguous()
+    return _rows(x, K), wg, wu, F, K
+
+
+def gated_ff(x, wg, wu, act="gelu_tanh", need_gu=False):
+    """h = act(x wgᵀ) ⊙ (x wuᵀ): both projections, the activation and the product in one kernel.  x bfloat16 [..., K], wg and wu bfloat16 [F, K], K a multiple
+    of 64, F of 32; act "gelu_tanh" or "silu".  -> h bfloat16 [..., F]; with need_gu (h, gu), where gu float32 [rows, 2F] holds both projections for
+    `gated_ff_backward`."""
+    dev = _same_device(x, wg, wu)
+    x2, wg, wu, F, K = _ff_operands("gated_ff", x, wg, wu, act, torch.bfloat16)
+    M = x2.shape[0]
+    h = torch.empty(*x.shape[:-1], F, dtype=torch.bfloat16, device=dev)
+    gu = torch.empty(M, 2 * F, dtype=torch.float32, device=dev) if need_gu else None
+    if M:
+        _run("gated_ff", dev, _lib.load().aether_gated_ff, x2.data_ptr(), x2.stride(0), wg.data_ptr(), wu.data_ptr(), wg.stride(0), h.data_ptr(), F, _lib.ptr(gu),
+             M, F, K, _ACTS[act])
+    return (h, gu) if need_gu else h
+
+
+def gated_ff_e4m3(x, x_scale, wg, wg_scale, wu, wu_scale, act="gelu_tanh"):
+    """`gated_ff` on 8-bit operands: x float8_e4m3fn [..., K] with x_scale float32 [...] (`rms_norm_e4m3`), wg and wu float8_e4m3fn [F, K] with a scale float32 [F]
+    each (`quantize_rows_e4m3`); K a multiple of 128, F of 32.  -> h bfloat16 [..., F]."""
+    name = "gated_ff_e4m3"
+    dev = _same_device(x, wg, wu, x_scale, wg_scale, wu_scale)
+    x2, wg, wu, F, K = _ff_operands(name, x, wg, wu, act, torch.float8_e4m3fn)
+    for n, t, shape in (("x_scale", x_scale, x.shape[:-1]), ("wg_scale", wg_scale, (F,)), ("wu_scale", wu_scale, (F,))):
+        if t.dtype != torch.float32 or tuple(t.shape) != tuple(shape):
+            raise ValueError(f"{name}: {n} is float32 {list(shape)}, got {t.dtype} {list(t.shape)}")
+    M = x2.shape[0]
+    h = torch.empty(*x.shape[:-1], F, dtype=torch.bfloat16, device=dev)
+    if M:
+        x_scale, wg_scale, wu_scale = x_scale.contiguous(), _vector(wg_scale), _vector(wu_scale)
+        _run(name, dev, _lib.load().aether_gated_ff_e4m3, x2.data_ptr(), x2.stride(0), x_scale.data_ptr(), wg.data_ptr(), wg_scale.data_ptr(), wu.data_ptr(),
+             wu_scale.data_ptr(), wg.stride(0), h.data_ptr(), F, M, F, K, _ACTS[act])
+    return h
+
+
+def gated_ff_backward(dh, x, wg, wu, gu, act="gelu_tanh"):
+    """Gradients of `gated_ff` (bfloat16 operands) from its inputs and gu: dh bfloat16 [..., F] -> (dx bfloat16 like x, dwg, dwu bfloat16 [F, K], the halves of one
+    [2F, K] buffer).  dh act'(g) u and dh act(g) are rounded to bf16 once, as operands of the products; sums are fp32, in an order that depends on the
+    sizes alone."""
+    name = "gated_ff_backward"
+    dev = _same_device(x, dh, wg, wu, gu)
+    x2, wg, wu, F, K = _ff_operands(name, x, wg, wu, act, torch.bfloat16)
+    M = x2.shape[0]
+    if dh.dtype != torch.bfloat16 or tuple(dh.shape) != (*x.shape[:-1], F):
+        raise ValueError(f"{name}: dh is bfloat16 {[*x.shape[:-1], F]}, got {dh.dtype} {list(dh.shape)}")
+    if gu.dtype != torch.float32 or tuple(gu.shape) != (M, 2 * F):
+        raise ValueError(f"{name}: gu is float32 [{M}, {2 * F}], as gated_ff gave it, got {gu.dtype} {list(gu.shape)}")
+    dx = torch.empty(x.shape, dtype=torch.bfloat16, device=dev)
+    if M == 0:
+        dw = torch.zeros(2 * F, K, dtype=torch.bfloat16, device=dev)
+        return dx, dw[:F], dw[F:]
+    d2, gu = _rows(dh, F), _rows(gu, 2 * F)
+    if gu.stride(0) != 2 * F:
+        gu = gu.contiguous()
+    dw = torch.empty(2 * F, K, dtype=torch.bfloat16, device=dev)
+    lib = _lib.load()
+    nbytes = lib.aether_gated_ff_bwd_workspace_bytes(M, F, K)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _run(name, dev, lib.aether_gated_ff_bwd, d2.data_ptr(), d2.stride(0), x2.data_ptr(), x2.stride(0), wg.data_ptr(), wu.data_ptr(), wg.stride(0), gu.data_ptr(),
+         dx.data_ptr(), K, dw.data_ptr(), M, F, K, _ACTS[act], ws.data_ptr(), nbytes)
+    return dx, dw[:F], dw[F:]

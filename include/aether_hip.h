@@ -174,6 +174,20 @@ int aether_relbias_attn_bwd(const AetherRelbias* d, const void* go, const long* 
                             const float* lse, void* dq, const long* dq_strides, void* dk, const long* dk_strides, void* dv, const long* dv_strides, void* dtable,
                             void* workspace, size_t workspace_bytes, void* stream);
 
+/* Gated feed-forward product: h = act(x·Wgᵀ) ⊙ (x·Wuᵀ).  x [M, K], wg and wu [F, K] (one leading dimension, elements), h bf16 [M, F] (ldh % 8 == 0).
+ * F % 32 == 0; K % 64 == 0 (bf16) or K % 128 == 0 (e4m3); rows 16-byte aligned; a weight below 4 GiB.  gu: fp32 [M][2F], x·Wgᵀ then x·Wuᵀ, for the backward
+ * pass, or NULL. */
+#define AETHER_ACT_GELU_TANH 0
+#define AETHER_ACT_SILU 1
+int aether_gated_ff(const void* x, long ldx, const void* wg, const void* wu, long ldw, void* h, long ldh, float* gu, int M, int F, int K, int act, void* stream);
+/* Operands in e4m3 with one fp32 scale per row of x [M], wg [F], wu [F] (aether_rms_norm, aether_quantize_rows_e4m3). */
+int aether_gated_ff_e4m3(const void* x, long ldx, const float* x_scale, const void* wg, const float* wg_scale, const void* wu, const float* wu_scale, long ldw,
+                         void* h, long ldh, int M, int F, int K, int act, void* stream);
+/* Backward pass, M > 0: dx bf16 [M, K]; dw bf16 [2F, K] dense, the gradient of wg and then that of wu.  dh bf16 [M, F]; gu as the forward pass wrote it. */
+size_t aether_gated_ff_bwd_workspace_bytes(int M, int F, int K);
+int aether_gated_ff_bwd(const void* dh, long lddh, const void* x, long ldx, const void* wg, const void* wu, long ldw, const float* gu, void* dx, long lddx,
+                        void* dw, int M, int F, int K, int act, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Element-wise tail of one denoise step in ONE pass (aetherv1_pipeline_cogvideox.py:876-916): fp32 cast of the noise prediction (P:877),
  * classifier-free-guidance combine uncond + g·(cond − uncond) when nb = 2 (P:895-899), CogVideoXDPMScheduler.step for v-prediction
  * (P:907-915; x0 = sqrt(a_t)·sample − sqrt(1−a_t)·model_output, prev = m1·sample − m2·d + m_noise·noise with d = x0 on a first-order

@@ -143,3 +143,42 @@ def test_relbias_backward_entry_refuses(hip_lib, kw, code, text):
     st = (C.c_long * 3)(*a["st"])
     rc = hip_lib.aether_relbias_attn_bwd(C.byref(d), a["go"], st, a["o"], st, a["low"], a["lse"], a["dq"], st, a["dk"], st, a["dv"], st, a["dt"], a["ws"], a["n"], None)
     assert rc == code and text in hip_lib.aether_last_error()
+
+
+# ---- gated feed-forward -----------------------------------------------------------------------------------------------------------------
+_FF = dict(x=4096, ldx=128, wg=4096, wu=4096, ldw=128, h=4096, ldh=64, M=4, F=64, K=128, act=0)
+
+
+@pytest.mark.parametrize("kw,code,text", [
+    (dict(act=2), -1, b"activation"), (dict(M=-1), -2, b"negative"), (dict(F=0), -2, b"positive"), (dict(K=0), -2, b"positive"), (dict(F=48), -2, b"multiple of 32"),
+    (dict(K=96), -2, b"64"), (dict(x=None), -1, b"null"), (dict(wu=None), -1, b"null"), (dict(ldx=64), -2, b"shorter"), (dict(ldw=64), -2, b"shorter"),
+    (dict(ldx=132), -3, b"aligned"), (dict(x=4104), -3, b"aligned"), (dict(F=1 << 20, K=4096, ldw=4096, ldx=4096, ldh=1 << 20), -2, b"4 GiB"),
+    (dict(ldx=1 << 23), -2, b"too far"), (dict(h=None), -1, b"output"), (dict(ldh=32), -3, b"aligned"), (dict(h=4104), -3, b"aligned"), (dict(M=(1 << 30) + 1), -2, b"rows"),
+])
+def test_gated_ff_entry_refuses(hip_lib, kw, code, text):
+    a = {**_FF, **kw}
+    rc = hip_lib.aether_gated_ff(a["x"], a["ldx"], a["wg"], a["wu"], a["ldw"], a["h"], a["ldh"], None, a["M"], a["F"], a["K"], a["act"], None)
+    assert rc == code and text in hip_lib.aether_last_error()
+
+
+@pytest.mark.parametrize("kw,code", [(dict(K=64), -2), (dict(sx=None), -1), (dict(sg=None), -1), (dict(su=4100), -3), (dict(h=None), -1), (dict(ldh=60), -3), (dict(ldw=136), -3)])
+def test_gated_ff_e4m3_entry_refuses(hip_lib, kw, code):
+    a = {**_FF, **dict(sx=4096, sg=4096, su=4096), **kw}
+    assert hip_lib.aether_gated_ff_e4m3(a["x"], a["ldx"], a["sx"], a["wg"], a["sg"], a["wu"], a["su"], a["ldw"], a["h"], a["ldh"], a["M"], a["F"], a["K"], a["act"], None) == code
+
+
+@pytest.mark.parametrize("kw,code,text", [
+    (dict(dw=None), -1, b"null"), (dict(dh=None), -1, b"null"), (dict(gu=None), -1, b"null"), (dict(dx=None), -1, b"null"), (dict(M=0), -2, b"rows"), (dict(lddh=32), -3, b"aligned"),
+    (dict(lddx=64), -3, b"aligned"), (dict(dw=4104), -3, b"aligned"), (dict(ws=None), -1, b"workspace"), (dict(n=1000), -1, b"workspace"), (dict(act=5), -1, b"activation"),
+    (dict(M=1 << 26), -2, b"4 GiB"),
+])
+def test_gated_ff_backward_entry_refuses(hip_lib, kw, code, text):
+    a = {**_FF, **dict(dh=4096, lddh=64, gu=4096, dx=4096, lddx=128, dw=4096, ws=4096, n=1 << 30), **kw}
+    rc = hip_lib.aether_gated_ff_bwd(a["dh"], a["lddh"], a["x"], a["ldx"], a["wg"], a["wu"], a["ldw"], a["gu"], a["dx"], a["lddx"], a["dw"], a["M"], a["F"], a["K"], a["act"],
+                                     a["ws"], a["n"], None)
+    assert rc == code and text in hip_lib.aether_last_error()
+
+
+def test_gated_ff_entries_without_rows(hip_lib):
+    assert hip_lib.aether_gated_ff(None, 128, None, None, 128, None, 64, None, 0, 64, 128, 0, None) == 0
+    assert hip_lib.aether_gated_ff_e4m3(None, 128, None, None, None, None, None, 128, None, 64, 0, 64, 128, 0, None) == 0
