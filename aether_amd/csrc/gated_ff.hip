@@ -357,9 +357,9 @@ extern "C" int aether_gated_ff_bwd(const void* dh, long lddh, const void* x, lon
                                    void* dw, int M, int F, int K, int act, void* workspace, size_t workspace_bytes, void* stream) {
     int rc = ff_check(x, ldx, wg, wu, ldw, M, F, K, act, 2);
     if (rc) return rc;
-    if (!dw || (M > 0 && (!dh || !gu || !dx))) return aether_set_error(AETHER_ERR_ARG, "gated_ff_bwd: null operand");
+    if ((!dx && !dw) || (M > 0 && (!dh || !gu))) return aether_set_error(AETHER_ERR_ARG, "gated_ff_bwd: null operand");
     if (M == 0) return aether_set_error(AETHER_ERR_SHAPE, "gated_ff_bwd: no rows");
-    if (lddh < F || lddh % 8 || lddx < K || lddx % 8 || (((uintptr_t)dh | (uintptr_t)gu | (uintptr_t)dx | (uintptr_t)dw | (uintptr_t)workspace) & 15))
+    if (lddh < F || lddh % 8 || (dx && (lddx < K || lddx % 8)) || (((uintptr_t)dh | (uintptr_t)gu | (uintptr_t)dx | (uintptr_t)dw | (uintptr_t)workspace) & 15))
         return aether_set_error(AETHER_ERR_ALIGN, "gated_ff_bwd: rows must be 16-byte aligned");
     const size_t Mp = ((size_t)M + 63) / 64 * 64;
     if (Mp * 2 * F * 2 >= (1ull << 32) || (size_t)2 * F * K * 2 >= (1ull << 32)) return aether_set_error(AETHER_ERR_SHAPE, "gated_ff_bwd: M·2F and 2F·K elements must stay below 4 GiB");
@@ -374,12 +374,17 @@ extern "C" int aether_gated_ff_bwd(const void* dh, long lddh, const void* x, lon
     const dim3 eg((F + 63) / 64, (unsigned)(Mp / 64));
     if (act == ACT_SILU) hipLaunchKernelGGL((gated_ff_dgu_kernel<ACT_SILU>), eg, dim3(256), 0, s, gu, (const bf16_t*)dh, lddh, M, F, (int)Mp, dgu, dgut);
     else hipLaunchKernelGGL((gated_ff_dgu_kernel<ACT_GELU_TANH>), eg, dim3(256), 0, s, gu, (const bf16_t*)dh, lddh, M, F, (int)Mp, dgu, dgut);
-    hipLaunchKernelGGL(transpose_bf16_kernel, dim3((K + 63) / 64, (unsigned)(Mp / 64)), dim3(256), 0, s, (const bf16_t*)x, ldx, M, K, xt, (long)Mp, (int)Mp);
-    hipLaunchKernelGGL(transpose_bf16_kernel, dim3((K + 63) / 64, (F + 63) / 64), dim3(256), 0, s, (const bf16_t*)wg, ldw, F, K, wt, 2 * (long)F, F);
-    hipLaunchKernelGGL(transpose_bf16_kernel, dim3((K + 63) / 64, (F + 63) / 64), dim3(256), 0, s, (const bf16_t*)wu, ldw, F, K, wt + F, 2 * (long)F, F);
     rc = aether_check_launch("gated_ff_bwd");
-    if (rc) return rc;
-    rc = aether_gemm_bf16(dgu, 2 * F, wt, 2 * F, dx, (int)lddx, M, K, 2 * F, nullptr, AETHER_EPI_BIAS, nullptr, 0, nullptr, nullptr, 0, 0, 0, nullptr, 0, 0, stream);
-    if (rc) return rc;
-    return aether_gemm_bf16(dgut, (int)Mp, xt, (int)Mp, dw, K, 2 * F, K, (int)Mp, nullptr, AETHER_EPI_BIAS, nullptr, 0, nullptr, nullptr, 0, 0, 0, nullptr, 0, 0, stream);
+    if (!rc && dx) {
+        hipLaunchKernelGGL(transpose_bf16_kernel, dim3((K + 63) / 64, (F + 63) / 64), dim3(256), 0, s, (const bf16_t*)wg, ldw, F, K, wt, 2 * (long)F, F);
+        hipLaunchKernelGGL(transpose_bf16_kernel, dim3((K + 63) / 64, (F + 63) / 64), dim3(256), 0, s, (const bf16_t*)wu, ldw, F, K, wt + F, 2 * (long)F, F);
+        rc = aether_check_launch("gated_ff_bwd (weights turned)");
+        if (!rc) rc = aether_gemm_bf16(dgu, 2 * F, wt, 2 * F, dx, (int)lddx, M, K, 2 * F, nullptr, AETHER_EPI_BIAS, nullptr, 0, nullptr, nullptr, 0, 0, 0, nullptr, 0, 0, stream);
+    }
+    if (!rc && dw) {
+        hipLaunchKernelGGL(transpose_bf16_kernel, dim3((K + 63) / 64, (unsigned)(Mp / 64)), dim3(256), 0, s, (const bf16_t*)x, ldx, M, K, xt, (long)Mp, (int)Mp);
+        rc = aether_check_launch("gated_ff_bwd (input turned)");
+        if (!rc) rc = aether_gemm_bf16(dgut, (int)Mp, xt, (int)Mp, dw, K, 2 * F, K, (int)Mp, nullptr, AETHER_EPI_BIAS, nullptr, 0, nullptr, nullptr, 0, 0, 0, nullptr, 0, 0, stream);
+    }
+    return rc;
 }

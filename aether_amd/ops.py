@@ -412,9 +412,9 @@ def gated_ff_e4m3(x, x_scale, wg, wg_scale, wu, wu_scale, act="gelu_tanh"):
     return h
 
 
-def gated_ff_backward(dh, x, wg, wu, gu, act="gelu_tanh"):
+def gated_ff_backward(dh, x, wg, wu, gu, act="gelu_tanh", need_dx=True, need_dw=True):
     """Gradients of `gated_ff` (bfloat16 operands) from its inputs and gu: dh bfloat16 [..., F] -> (dx bfloat16 like x, dwg, dwu bfloat16 [F, K], the halves of one
-    [2F, K] buffer).  dh act'(g) u and dh act(g) are rounded to bf16 once, as operands of the products; sums are fp32, in an order that depends on the
+    [2F, K] buffer; None for what is not needed).  dh act'(g) u and dh act(g) are rounded to bf16 once, as operands of the products; sums are fp32, in an order that depends on the
     sizes alone."""
     name = "gated_ff_backward"
     dev = _same_device(x, dh, wg, wu, gu)
@@ -424,17 +424,17 @@ def gated_ff_backward(dh, x, wg, wu, gu, act="gelu_tanh"):
         raise ValueError(f"{name}: dh is bfloat16 {[*x.shape[:-1], F]}, got {dh.dtype} {list(dh.shape)}")
     if gu.dtype != torch.float32 or tuple(gu.shape) != (M, 2 * F):
         raise ValueError(f"{name}: gu is float32 [{M}, {2 * F}], as gated_ff gave it, got {gu.dtype} {list(gu.shape)}")
-    dx = torch.empty(x.shape, dtype=torch.bfloat16, device=dev)
-    if M == 0:
-        dw = torch.zeros(2 * F, K, dtype=torch.bfloat16, device=dev)
-        return dx, dw[:F], dw[F:]
+    dx = torch.empty(x.shape, dtype=torch.bfloat16, device=dev) if need_dx else None
+    dw = (torch.empty if M else torch.zeros)(2 * F, K, dtype=torch.bfloat16, device=dev) if need_dw else None
+    out = dx, dw[:F] if need_dw else None, dw[F:] if need_dw else None
+    if M == 0 or not (need_dx or need_dw):
+        return out
     d2, gu = _rows(dh, F), _rows(gu, 2 * F)
     if gu.stride(0) != 2 * F:
         gu = gu.contiguous()
-    dw = torch.empty(2 * F, K, dtype=torch.bfloat16, device=dev)
     lib = _lib.load()
     nbytes = lib.aether_gated_ff_bwd_workspace_bytes(M, F, K)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _run(name, dev, lib.aether_gated_ff_bwd, d2.data_ptr(), d2.stride(0), x2.data_ptr(), x2.stride(0), wg.data_ptr(), wu.data_ptr(), wg.stride(0), gu.data_ptr(),
-         dx.data_ptr(), K, dw.data_ptr(), M, F, K, _ACTS[act], ws.data_ptr(), nbytes)
-    return dx, dw[:F], dw[F:]
+         _lib.ptr(dx), K, _lib.ptr(dw), M, F, K, _ACTS[act], ws.data_ptr(), nbytes)
+    return out

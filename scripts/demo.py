@@ -10,7 +10,8 @@ and window w runs on rank w mod N (aether_amd/windows.py); rank 0 blends and sav
 
 Extra, optional flags (the reference's flags are unchanged): --empty_prompt_embeds (a .pt with the cached T5 embedding
 of "" — the only thing the text encoder is ever used for, P:290-297), --synthetic_weights (seeded random weights, for
-smoke runs without checkpoints).  The window merge (disparity scale fitting, camera alignment, pose smoothing, point maps:
+smoke runs without checkpoints), --native_text_encoder (this repository's text encoder instead of transformers' when the empty prompt is
+encoded).  The window merge (disparity scale fitting, camera alignment, pose smoothing, point maps:
 D:254-422) runs on the host like the reference's (aether_amd/windows.py + aether_amd/geometry.py, pinned against the
 reference's own functions by tests/golden/blend.npz); merged rgb / disparity / poses / point maps are written as .npz + a
 preview frame — mp4 / GLB export (D:425-521: imageio, trimesh) is outside this repo's scope.
@@ -81,6 +82,8 @@ def parse_args(argv=None) -> argparse.Namespace:
     p.add_argument("--empty_prompt_embeds", type=str, default=None, help="[aether_amd] .pt file with the T5 embedding of the empty prompt [1,226,4096].")
     p.add_argument("--synthetic_weights", action="store_true", default=False, help="[aether_amd] seeded random weights instead of checkpoints (smoke runs).")
     p.add_argument("--synthetic_layers", type=int, default=42, help="[aether_amd] depth of the synthetic transformer.")
+    p.add_argument("--native_text_encoder", action="store_true", default=False,
+                   help="[aether_amd] encode the prompt with aether_amd.text_encoder (bf16, HIP kernels) instead of transformers' T5EncoderModel.")
     p.add_argument("--float64_outputs", action="store_true", default=False,
                    help="[aether_amd] merged arrays of a long clip as float64 like the reference's numpy merge (default float32: half the D2H bytes).")
     return p.parse_args(argv)
@@ -114,9 +117,14 @@ def build_pipeline(args: argparse.Namespace, device: torch.device) -> AetherV1Pi
         if args.empty_prompt_embeds is not None:
             prompt_embeds = torch.load(args.empty_prompt_embeds, map_location="cpu")
         else:
-            from transformers import AutoTokenizer, T5EncoderModel
+            from transformers import AutoTokenizer
             tokenizer = AutoTokenizer.from_pretrained(cog, subfolder="tokenizer")
-            text_encoder = T5EncoderModel.from_pretrained(cog, subfolder="text_encoder")
+            if args.native_text_encoder:
+                from aether_amd.text_encoder import AetherTextEncoder
+                text_encoder = AetherTextEncoder.from_pretrained(cog, subfolder="text_encoder", device=device)
+            else:
+                from transformers import T5EncoderModel
+                text_encoder = T5EncoderModel.from_pretrained(cog, subfolder="text_encoder")
     pipeline = AetherV1PipelineCogVideoX(tokenizer=tokenizer, text_encoder=text_encoder, vae=vae, scheduler=scheduler,
                                          transformer=transformer, empty_prompt_embeds=prompt_embeds)
     pipeline.vae.enable_slicing()

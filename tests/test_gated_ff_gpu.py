@@ -152,6 +152,8 @@ def _check_backward(x, wg, wu, dh, act):
         _within(x_, y, l + BF16 * y.abs() + 1e-30, name)
     again = ops.gated_ff_backward(dh, x, wg, wu, gu, act)
     assert all(torch.equal(p, q) for p, q in zip(got, again)), "the same order of sums every time"
+    only_x, only_w = (ops.gated_ff_backward(dh, x, wg, wu, gu, act, need_dx=not w, need_dw=w) for w in (False, True))
+    assert torch.equal(only_x[0], got[0]) and only_x[1:] == (None, None) and only_w[0] is None and torch.equal(only_w[1], got[1]) and torch.equal(only_w[2], got[2])
     return got
 
 

@@ -168,7 +168,7 @@ def test_gated_ff_e4m3_entry_refuses(hip_lib, kw, code):
 
 
 @pytest.mark.parametrize("kw,code,text", [
-    (dict(dw=None), -1, b"null"), (dict(dh=None), -1, b"null"), (dict(gu=None), -1, b"null"), (dict(dx=None), -1, b"null"), (dict(M=0), -2, b"rows"), (dict(lddh=32), -3, b"aligned"),
+    (dict(dw=None, dx=None), -1, b"null"), (dict(dh=None), -1, b"null"), (dict(gu=None), -1, b"null"), (dict(M=0), -2, b"rows"), (dict(lddh=32), -3, b"aligned"),
     (dict(lddx=64), -3, b"aligned"), (dict(dw=4104), -3, b"aligned"), (dict(ws=None), -1, b"workspace"), (dict(n=1000), -1, b"workspace"), (dict(act=5), -1, b"activation"),
     (dict(M=1 << 26), -2, b"4 GiB"),
 ])
