@@ -16,6 +16,7 @@
 //     two bf16 parts (P = hi + lo to 2^-17) and also stores what the rounding of O left (o_low), so that O + o_low is good to 2^-16.
 //   * Keys that do not count: whole tiles are skipped; in a tile that holds some, their scores become −inf and their V elements 0 (a NaN or an infinity
 //     behind the mask reaches nothing).
+#include <type_traits>
 #include "relbias_attn.hpp"
 #include "../../include/aether_hip.h"
 
@@ -24,11 +25,11 @@ namespace aether {
 struct RbFwdArgs { RbArgs a; bf16_t* o; bf16_t* o_low; float* lse; };   // o_low, lse: for a backward pass
 
 template <int NW, bool TRAIN>
-__global__ __launch_bounds__(NW * 64) void relbias_attn_fwd_kernel(RbFwdArgs args) {
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(3, 3))) void relbias_attn_fwd_kernel(RbFwdArgs args) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const RbArgs& p = args.a;
-    float* const tab = (float*)(smem + 2 * RB_BUF);
-    unsigned char* const words8 = (unsigned char*)(smem + 2 * RB_BUF + ((2 * (p.reach + RB_PAD) + 1) * 4 + 15) / 16 * 16);
+    float* const tab = (float*)(smem + RB_RING);
+    unsigned char* const words8 = (unsigned char*)(smem + RB_RING + ((2 * (p.reach + RB_PAD) + 1) * 4 + 15) / 16 * 16);
     const uint64_t* const words = (const uint64_t*)words8;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5, l32 = lane & 31;
     const int wave_s = __builtin_amdgcn_readfirstlane(wave);
@@ -60,7 +61,7 @@ __global__ __launch_bounds__(NW * 64) void relbias_attn_fwd_kernel(RbFwdArgs arg
         v_off[ps] = r * v_row + ((ch ^ rb_swz(r)) << 4);
     }
     auto stage = [&](int j, int buf) {
-        char* const dst = smem + buf * RB_BUF + wave_s * 1024;
+        char* const dst = smem + buf + wave_s * 1024;
 #pragma unroll
         for (int ps = 0; ps < 8 / NW; ++ps) {
             bglds16(k_rsrc, k_off[ps], (unsigned)j * (RB_KV * k_row), dst + ps * (NW * 1024));
@@ -77,6 +78,7 @@ __global__ __launch_bounds__(NW * 64) void relbias_attn_fwd_kernel(RbFwdArgs arg
     float m_run = 0.f, l_run = 0.f;
     bool started = false;
 
+    rb_arrived(qf);
     __syncthreads();                                                  // table and words are there
     const float far_r = tab[2 * (p.reach + RB_PAD)], far_l = tab[0];
     const int nkv = (S + RB_KV - 1) / RB_KV;
@@ -85,115 +87,125 @@ __global__ __launch_bounds__(NW * 64) void relbias_attn_fwd_kernel(RbFwdArgs arg
             if ((w = rb_word(p, words, j)) != 0) break;
         return j;
     };
-    uint64_t w = 0, w_next = 0;
-    int j = next_tile(0, w);
-    if (j < nkv) stage(j, 0);
-    drain_and_barrier();
+    uint64_t w = 0, w1 = 0, w2 = 0;
+    int j = next_tile(0, w), j1 = next_tile(j + 1, w1);
     int buf = 0;
+    if (j < nkv) stage(j, 0);
+    if (j1 < nkv) stage(j1, RB_BUF);
+    drain_and_barrier();
     while (j < nkv) {
-        const int j_next = next_tile(j + 1, w_next);
-        if (j_next < nkv) stage(j_next, buf ^ 1);
-        const char* base = smem + buf * RB_BUF;
+        const char* base = smem + buf;
+        const int j2 = next_tile(j1 + 1, w2);
         f32x16 x[2];
 #pragma unroll
         for (int i = 0; i < 16; ++i) { x[0][i] = 0.f; x[1][i] = 0.f; }
         __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks)
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int ks = 0; ks < 4; ++ks)
                 x[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(base + t * 4096 + koff[ks]), qf[ks], x[t], 0, 0, 0);
         __builtin_amdgcn_s_setprio(0);
         // x[t][r]: query l32, key 64j + 32t + 16(r >> 3) + 8hi + (r & 7)
         const int d_lo = j * RB_KV - (q0 + 31), d_hi = j * RB_KV + 63 - q0;
-        if (d_lo >= p.reach || d_hi <= -p.reach) {
-            const float add = (d_lo >= p.reach ? far_r : far_l) - m_run;
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
+        const bool right = d_lo >= p.reach, left = d_hi <= -p.reach;
+        const bool part = w != ~0ull;
+        // One half of the tile: soft-max, then its share of Oᵀ += Vᵀ·Pᵀ.  The first half's soft-max runs behind the second half's scores on the matrix pipe,
+        // the second half's behind the first half's products.
+        auto half = [&](auto t_tag) {
+            constexpr int t = decltype(t_tag)::value;
+            const unsigned wt = (unsigned)(w >> (32 * t));
+            if (part && wt == 0) return;                              // (wave-uniform) no key in this half
+            if (right || left) {
+                const float add = (right ? far_r : far_l) - m_run;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) x[t][r] = fmaf(x[t][r], p.c, add);
-        } else {
-            // |d| <= reach + 94 here: inside the padded table.  A query row beyond the last one reads inside it too (its wave's own range).
-            const float* tb = tab + (j * RB_KV + 8 * hi - qrow + p.reach + RB_PAD);
+            } else {
+                // |d| <= reach + 94 here: inside the padded table.  A query row beyond the last one reads inside it too (its wave's own range).
+                const float* tb = tab + (j * RB_KV + 32 * t + 8 * hi - qrow + p.reach + RB_PAD);
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) x[t][r] = fmaf(x[t][r], p.c, tb[32 * t + 16 * (r >> 3) + (r & 7)] - m_run);
-        }
-        const bool part = w != ~0ull;
-        if (part) {
-            const uint64_t mine = w >> (8 * hi);
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
+                for (int r = 0; r < 16; ++r) x[t][r] = fmaf(x[t][r], p.c, tb[16 * (r >> 3) + (r & 7)] - m_run);
+            }
+            if (__builtin_expect(part, 0)) {
+                const unsigned mine = wt >> (8 * hi);
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    if (!((mine >> (32 * t + 16 * (r >> 3) + (r & 7))) & 1)) x[t][r] = -INFINITY;
-        }
-        unsigned pf[2][2][4], pl[TRAIN ? 2 : 1][2][4];
-        float tsum = 0.f;
-        auto expo = [&]() {
-            float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
+                    if (!((mine >> (16 * (r >> 3) + (r & 7))) & 1)) x[t][r] = -INFINITY;
+            }
+            unsigned pf[2][4], pl[2][4];
+            float tsum = 0.f;
+            auto expo = [&]() {
+                float s0 = 0.f, s1 = 0.f;
 #pragma unroll
                 for (int s = 0; s < 2; ++s)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const float pa = __builtin_amdgcn_exp2f(x[t][8 * s + 2 * e]), pb = __builtin_amdgcn_exp2f(x[t][8 * s + 2 * e + 1]);
-                        pf[t][s][e] = pack_bf16x2(pa, pb);
-                        if constexpr (TRAIN)
-                            pl[t][s][e] = pack_bf16x2(pa - __uint_as_float(pf[t][s][e] << 16), pb - __uint_as_float(pf[t][s][e] & 0xffff0000u));
-                        s0 += pa;
-                        s1 += pb;
+                        pf[s][e] = pack_bf16x2(pa, pb);
+                        if constexpr (TRAIN) {
+                            pl[s][e] = pack_bf16x2(pa - __uint_as_float(pf[s][e] << 16), pb - __uint_as_float(pf[s][e] & 0xffff0000u));
+                            s0 += pa;
+                            s1 += pb;
+                        } else {                                      // the sum of the rounded values: numerator and denominator round alike, one instruction a pair
+                            bf16x2 ones;
+                            ones[0] = (__bf16)1.0f; ones[1] = (__bf16)1.0f;
+                            if (e & 1) s1 = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pf[s][e]), ones, s1, false);
+                            else s0 = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pf[s][e]), ones, s0, false);
+                        }
                     }
-            tsum = s0 + s1;
-        };
-        bool redo = !started;
-        if (!redo) {
-            expo();
-            redo = __any(!(tsum <= 1.2676506e30f)) != 0;               // 2^100
-        }
-        if (__builtin_expect(redo, 0)) {
-            float top = -INFINITY;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) top = fmaxf(top, fmaxf(x[0][r], x[1][r]));
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const float up = started ? fmaxf(top, 0.f) : fmaxf(top, -1e30f);   // a first tile of −inf alone keeps a finite shift
-            if (started) {
-                const float alpha = __builtin_amdgcn_exp2f(-up);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) { o[0][i] *= alpha; o[1][i] *= alpha; }
-                l_run *= alpha;
+                tsum = s0 + s1;
+            };
+            bool redo = !started;
+            if (!redo) {
+                expo();
+                redo = __any(!(tsum <= 1.2676506e30f)) != 0;          // 2^100
             }
-            m_run += up;
+            if (__builtin_expect(redo, 0)) {
+                float top = x[t][0];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) { x[0][i] -= up; x[1][i] -= up; }
-            expo();
-            started = true;
-        }
-        l_run += tsum;
-        // ---- Oᵀ += Vᵀ · Pᵀ ----
-        __builtin_amdgcn_s_setprio(1);
+                for (int r = 1; r < 16; ++r) top = fmaxf(top, x[t][r]);
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                const float up = started ? fmaxf(top, 0.f) : top == -INFINITY ? 0.f : top;
+                if (started) {
+                    const float alpha = __builtin_amdgcn_exp2f(-up);
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+                    for (int i = 0; i < 16; ++i) { o[0][i] *= alpha; o[1][i] *= alpha; }
+                    l_run *= alpha;
+                }
+                m_run += up;
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const bf16x8 pv = __builtin_bit_cast(bf16x8, make_uint4(pf[t][s][0], pf[t][s][1], pf[t][s][2], pf[t][s][3]));
+                for (int i = 0; i < 16; ++i) x[t][i] -= up;
+                expo();
+                started = true;
+            }
+            l_run += tsum;
+            bf16x8 vf[2][2];
+            rb_read_tr(vf, base + RB_TILE + t * 4096, voff);
+            if (__builtin_expect(part, 0)) {
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int dt = 0; dt < 2; ++dt) vf[s][dt] = rb_keep(vf[s][dt], (wt >> (16 * s + 8 * hi)) & 0xffu);
+            }
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
 #pragma unroll
                 for (int dt = 0; dt < 2; ++dt) {
-                    const char* vb = base + RB_TILE + (2 * t + s) * 2048;
-                    bf16x8 vf = rb_read_tr(vb + voff[dt][0], vb + voff[dt][1]);
-                    if (part) vf = rb_keep(vf, (unsigned)(w >> (32 * t + 16 * s + 8 * hi)) & 0xffu);
-                    o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pv, o[dt], 0, 0, 0);
+                    o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[s][dt], __builtin_bit_cast(bf16x8, make_uint4(pf[s][0], pf[s][1], pf[s][2], pf[s][3])), o[dt], 0, 0, 0);
                     if constexpr (TRAIN)
-                        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, __builtin_bit_cast(bf16x8, make_uint4(pl[t][s][0], pl[t][s][1], pl[t][s][2], pl[t][s][3])), o[dt], 0, 0, 0);
+                        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[s][dt], __builtin_bit_cast(bf16x8, make_uint4(pl[s][0], pl[s][1], pl[s][2], pl[s][3])), o[dt], 0, 0, 0);
                 }
-            }
-        __builtin_amdgcn_s_setprio(0);
-        drain_and_barrier();
-        j = j_next;
-        w = w_next;
-        buf ^= 1;
+            __builtin_amdgcn_s_setprio(0);
+        };
+        half(std::integral_constant<int, 0>{});
+        half(std::integral_constant<int, 1>{});
+        rb_tiles_landed();                                            // tile j1, issued one tile ago
+        if (j2 < nkv) stage(j2, rb_next(rb_next(buf)));               // its buffer was last read before the previous barrier
+        rb_reads_done_barrier();
+        j = j1; w = w1;
+        j1 = j2; w1 = w2;
+        buf = rb_next(buf);
     }
     // ---- epilogue: O[b][q][h][d], d = 32dt + 8(r >> 2) + 4hi + (r & 3) ----
     const float l_tot = l_run + __shfl_xor(l_run, 32, 64);
@@ -268,7 +280,7 @@ extern "C" int aether_relbias_attn(const AetherRelbias* d, void* o, void* o_low,
     args.o_low = (bf16_t*)o_low;
     args.lse = lse;
     RbArgs& p = args.a;
-    const size_t lds = 2 * RB_BUF + rb_table_bytes(p.reach) + rb_words_bytes(p);
+    const size_t lds = RB_RING + rb_table_bytes(p.reach) + rb_words_bytes(p);
     const int nw = rb_waves(p);
     p.nqb = (p.S + nw * 32 - 1) / (nw * 32);
     const dim3 grid((unsigned)((long)p.B * p.H * p.nqb));

@@ -95,6 +95,13 @@ AE_DEV void rb_tr_offsets(int lane, int (&off)[2][2]) {
             off[dt][f] = r * 128 + ((chunk ^ rb_swz(r)) << 4) + (i & 1) * 8;
         }
 }
+// Makes the wait for a fragment's loads happen here.  Left to its first use inside a loop, the compiler counts it together with the loop's own tile loads
+// and waits for those too.
+AE_DEV void rb_arrived(bf16x8 (&f)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(f[i]));
+}
+
 // zeroes the elements of a fragment of eight rows whose bit is not set
 AE_DEV bf16x8 rb_keep(bf16x8 f, unsigned bits) {
     uint4 u = __builtin_bit_cast(uint4, f);
@@ -124,14 +131,30 @@ AE_DEV void rb_store(const f32x16 (&o)[2], float f, bf16_t* row, int hi, bool ok
     }
 }
 
-// The transposing LDS read: within 16 lanes, lane 4r + c names row r, elements 4c .. 4c + 3 of a 4 x 16 piece, and lane i receives column i
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-AE_DEV bf16x8 rb_read_tr(const char* a, const char* b) {
-    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)a);
-    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)b);
+// The transposed fragments of 32 rows of a tile: f[s][dt] holds column 32 dt + (lane & 31), rows 16 s + 8hi ... + 7.  The transposing LDS read moves a 4 x 16 piece
+// per 16 lanes: lane 4r + c names row r, elements 4c ... 4c + 3, and lane i receives column i.  Before these reads the compiler waits for every LDS-DMA in
+// flight; the loops therefore issue the tile after the next behind them.
+AE_DEV void rb_read_tr(bf16x8 (&f)[2][2], const char* at, const int (&off)[2][2]) {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
     typedef short s16x8 __attribute__((ext_vector_type(8)));
-    const s16x8 v = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-    return __builtin_bit_cast(bf16x8, v);
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int dt = 0; dt < 2; ++dt) {
+            const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + 2048 * s + off[dt][0]));
+            const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + 2048 * s + off[dt][1]));
+            f[s][dt] = __builtin_bit_cast(bf16x8, s16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]});
+        }
+}
+
+// Three buffers of two tiles: while one is worked on, the next one is complete or arriving, and the one after it is issued.
+constexpr int RB_RING = 3 * RB_BUF;
+AE_DEV int rb_next(int buf) { return buf == 2 * RB_BUF ? 0 : buf + RB_BUF; }   // buffers by their offsets
+AE_DEV void rb_tiles_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+AE_DEV void rb_reads_done_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
 }
 
 }  // namespace aether

@@ -10,9 +10,13 @@
 // row-major tiles by ds_read_b64_tr_b16.
 // δ is a product with O on the matrix pipe like dP is one with v, in the same order of sums: a row that has one key has O = v, so that its dP − δ is 0, not the
 // difference of two roundings.
-// dT: beyond `reach` a tile's dS go into one number per lane.  Near the diagonal an element adds to its distance's entry in LDS; a wave has its own table for
-// each half of its lanes, in which the 32 lanes of an instruction name 32 different entries, so that no two adds ever race.  Keys that do not count: their
+// dT: beyond `reach` a tile's dS go into one number per lane.  Near the diagonal dS is summed along its diagonals in registers: the 16 values of a lane are
+// rotated over the 32 queries by their key's place (ds_swizzle, a constant each), which brings a diagonal into one lane; what wraps around joins the next
+// 32 keys' diagonals, so that every entry of a wave's table of distances is stored once, by plain stores.  (LDS float atomics in their place: 200 cycles an
+// instruction, three quarters of this kernel's time at 16 x 226 x 64 heads.)  Keys that do not count: their
 // P and dS are 0 whatever k and v hold there, and so are dk and dv.
+#include <type_traits>
+#include <utility>
 #include "relbias_attn.hpp"
 #include "../../include/aether_hip.h"
 
@@ -28,15 +32,18 @@ struct RbBwdArgs {
     float scale;
 };
 
+template <int... Is, class F> AE_DEV void rb_static_for_impl(F&& f, std::integer_sequence<int, Is...>) { (f(std::integral_constant<int, Is>{}), ...); }
+template <int N, class F> AE_DEV void rb_static_for(F&& f) { rb_static_for_impl(f, std::make_integer_sequence<int, N>{}); }
+
 template <int NW>
-__global__ __launch_bounds__(NW * 64) void relbias_attn_dq_kernel(RbBwdArgs args) {
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void relbias_attn_dq_kernel(RbBwdArgs args) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const RbArgs& p = args.a;
     const int n_tab = 2 * (p.reach + RB_PAD) + 1;
     const int tab_bytes = (n_tab * 4 + 15) / 16 * 16;
-    float* const tab = (float*)(smem + 2 * RB_BUF);
-    float* const hist = (float*)(smem + 2 * RB_BUF + tab_bytes);              // [wave][hi][n_tab]
-    unsigned char* const words8 = (unsigned char*)(smem + 2 * RB_BUF + tab_bytes * (args.part ? 1 + 2 * NW : 1));
+    float* const tab = (float*)(smem + RB_RING);
+    float* const hist = (float*)(smem + RB_RING + tab_bytes);              // [wave][hi][n_tab]
+    unsigned char* const words8 = (unsigned char*)(smem + RB_RING + tab_bytes * (args.part ? 1 + 2 * NW : 1));
     const uint64_t* const words = (const uint64_t*)words8;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5, l32 = lane & 31;
     const int wave_s = __builtin_amdgcn_readfirstlane(wave);
@@ -90,7 +97,7 @@ __global__ __launch_bounds__(NW * 64) void relbias_attn_dq_kernel(RbBwdArgs args
         v_off[ps] = r * v_row + ((ch ^ rb_swz(r)) << 4);
     }
     auto stage = [&](int j, int buf) {
-        char* const dst = smem + buf * RB_BUF + wave_s * 1024;
+        char* const dst = smem + buf + wave_s * 1024;
 #pragma unroll
         for (int ps = 0; ps < 8 / NW; ++ps) {
             bglds16(k_rsrc, k_off[ps], (unsigned)j * (RB_KV * k_row), dst + ps * (NW * 1024));
@@ -101,10 +108,17 @@ __global__ __launch_bounds__(NW * 64) void relbias_attn_dq_kernel(RbBwdArgs args
     rb_row_offsets(lane, roff);
     rb_tr_offsets(lane, toff);
 
+    rb_arrived(qf);
+    rb_arrived(gf);
     f32x16 dq[2];
 #pragma unroll
     for (int i = 0; i < 16; ++i) { dq[0][i] = 0.f; dq[1][i] = 0.f; }
     float sum_r = 0.f, sum_l = 0.f;                                   // dS beyond the reach, on either side
+    float carry = 0.f;                                                // diagonals that go on into the keys from carry_at on (wave-uniform; < 0: none)
+    int carry_at = -1;
+    auto put = [&](int at, float v) {
+        if (at < n_tab) my_hist[at] = v;                              // (beyond it there are only zeros: no pair of the wave is that far apart)
+    };
 
     __syncthreads();
     const float far_r = tab[2 * (p.reach + RB_PAD)], far_l = tab[0];
@@ -114,85 +128,113 @@ __global__ __launch_bounds__(NW * 64) void relbias_attn_dq_kernel(RbBwdArgs args
             if ((w = rb_word(p, words, j)) != 0) break;
         return j;
     };
-    uint64_t w = 0, w_next = 0;
-    int j = next_tile(0, w);
-    if (j < nkv) stage(j, 0);
-    drain_and_barrier();
+    uint64_t w = 0, w1 = 0, w2 = 0;
+    int j = next_tile(0, w), j1 = next_tile(j + 1, w1);
     int buf = 0;
+    if (j < nkv) stage(j, 0);
+    if (j1 < nkv) stage(j1, RB_BUF);
+    drain_and_barrier();
     while (j < nkv) {
-        const int j_next = next_tile(j + 1, w_next);
-        if (j_next < nkv) stage(j_next, buf ^ 1);
-        const char* base = smem + buf * RB_BUF;
+        const int j2 = next_tile(j1 + 1, w2);
+        const char* base = smem + buf;
         const bool part = w != ~0ull;
         const int d_lo = j * RB_KV - (q0 + 31), d_hi = j * RB_KV + 63 - q0;
         const bool right = d_lo >= p.reach, left = d_hi <= -p.reach;
+        f32x16 x[2], dp[2];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            f32x16 x, dp;
+        for (int i = 0; i < 16; ++i) { x[0][i] = 0.f; x[1][i] = 0.f; dp[0][i] = 0.f; dp[1][i] = 0.f; }
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) { x[i] = 0.f; dp[i] = 0.f; }
-            __builtin_amdgcn_s_setprio(1);
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) {
-                x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(base + t * 4096 + roff[ks]), qf[ks], x, 0, 0, 0);
-                dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(base + RB_TILE + t * 4096 + roff[ks]), gf[ks], dp, 0, 0, 0);
+                x[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(base + t * 4096 + roff[ks]), qf[ks], x[t], 0, 0, 0);
+                dp[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(base + RB_TILE + t * 4096 + roff[ks]), gf[ks], dp[t], 0, 0, 0);
             }
-            __builtin_amdgcn_s_setprio(0);
-            // x[r], dp[r]: query l32, key 64j + 32t + 16(r >> 3) + 8hi + (r & 7)
-            const int d0 = j * RB_KV + 32 * t + 8 * hi - qrow + p.reach + RB_PAD;   // the distance of r = 0, as an index of tab
+        __builtin_amdgcn_s_setprio(0);
+        // x[t][r], dp[t][r]: query l32, key 64j + 32t + 16(r >> 3) + 8hi + (r & 7)
+        auto half = [&](auto t_tag) {
+            constexpr int t = decltype(t_tag)::value;
+            const unsigned wt = (unsigned)(w >> (32 * t));
+            if (part && wt == 0) return;                              // (wave-uniform) no key in this half
+            const int k_at = j * RB_KV + 32 * t;
+            const int d0 = k_at + 8 * hi - qrow + p.reach + RB_PAD;   // the distance of r = 0, as an index of tab
+            f32x16& ds = x[t];
             if (right || left) {
                 const float add = (right ? far_r : far_l) - lse;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) x[r] = fmaf(x[r], p.c, add);
+                for (int r = 0; r < 16; ++r) ds[r] = fmaf(ds[r], p.c, add);
             } else {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) x[r] = fmaf(x[r], p.c, tab[d0 + 16 * (r >> 3) + (r & 7)] - lse);
+                for (int r = 0; r < 16; ++r) ds[r] = fmaf(ds[r], p.c, tab[d0 + 16 * (r >> 3) + (r & 7)] - lse);
             }
 #pragma unroll
-            for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(x[r]) * (dp[r] - delta);
-            if (part) {
-                const uint64_t mine = w >> (32 * t + 8 * hi);
+            for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(ds[r]) * (dp[t][r] - delta);
+            if (__builtin_expect(part, 0)) {
+                const unsigned mine = wt >> (8 * hi);
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    if (!((mine >> (16 * (r >> 3) + (r & 7))) & 1)) x[r] = 0.f;
+                    if (!((mine >> (16 * (r >> 3) + (r & 7))) & 1)) ds[r] = 0.f;
             }
             if (args.part) {
                 if (right || left) {
                     float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-                    for (int r = 0; r < 16; r += 2) { s0 += x[r]; s1 += x[r + 1]; }
+                    for (int r = 0; r < 16; r += 2) { s0 += ds[r]; s1 += ds[r + 1]; }
                     if (right) sum_r += s0 + s1;
                     else sum_l += s0 + s1;
                 } else {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        __hip_atomic_fetch_add(my_hist + d0 + 16 * (r >> 3) + (r & 7), x[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                    // element (query l32, key k_at + kr + 8hi), kr = 16(r >> 3) + (r & 7): rotated by kr it is in lane i = l32 - kr of its half (of 32
+                    // lanes), distance k_at + 8hi - q0 - i; or, wrapped, in lane i = l32 - kr + 32, distance 32 more
+                    float whole = 0.f, wrap = 0.f;
+                    rb_static_for<16>([&](auto r_tag) {
+                        constexpr int r = decltype(r_tag)::value, kr = 16 * (r >> 3) + (r & 7);
+                        const float y = kr ? __int_as_float(__builtin_amdgcn_ds_swizzle(__float_as_int(ds[r]), 0xc000 | (kr << 5))) : ds[r];
+                        const float z = l32 > 31 - kr ? y : 0.f;
+                        wrap += z;
+                        whole += y - z;
+                    });
+                    if (k_at != carry_at) {                           // the diagonals carried here do not continue where this begins
+                        if (carry_at >= 0) put(carry_at + 8 * hi - q0 - l32 + p.reach + RB_PAD, carry);
+                        carry = 0.f;
+                    }
+                    put(d0 + qrow - q0 - l32, whole + carry);
+                    carry = wrap;
+                    carry_at = k_at + 32;
                 }
+            }
+            bf16x8 kf[2][2];
+            rb_read_tr(kf, base + t * 4096, toff);
+            if (__builtin_expect(part, 0)) {
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int dt = 0; dt < 2; ++dt) kf[s][dt] = rb_keep(kf[s][dt], (wt >> (16 * s + 8 * hi)) & 0xffu);
             }
             __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-                const bf16x8 ds = __builtin_bit_cast(bf16x8, make_uint4(pack_bf16x2(x[8 * s], x[8 * s + 1]), pack_bf16x2(x[8 * s + 2], x[8 * s + 3]),
-                                                                        pack_bf16x2(x[8 * s + 4], x[8 * s + 5]), pack_bf16x2(x[8 * s + 6], x[8 * s + 7])));
+                const bf16x8 df = __builtin_bit_cast(bf16x8, make_uint4(pack_bf16x2(ds[8 * s], ds[8 * s + 1]), pack_bf16x2(ds[8 * s + 2], ds[8 * s + 3]),
+                                                                        pack_bf16x2(ds[8 * s + 4], ds[8 * s + 5]), pack_bf16x2(ds[8 * s + 6], ds[8 * s + 7])));
 #pragma unroll
-                for (int dt = 0; dt < 2; ++dt) {
-                    const char* kb = base + (2 * t + s) * 2048;
-                    bf16x8 kf = rb_read_tr(kb + toff[dt][0], kb + toff[dt][1]);
-                    if (part) kf = rb_keep(kf, (unsigned)(w >> (32 * t + 16 * s + 8 * hi)) & 0xffu);
-                    dq[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, ds, dq[dt], 0, 0, 0);
-                }
+                for (int dt = 0; dt < 2; ++dt) dq[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[s][dt], df, dq[dt], 0, 0, 0);
             }
             __builtin_amdgcn_s_setprio(0);
-        }
-        drain_and_barrier();
-        j = j_next;
-        w = w_next;
-        buf ^= 1;
+        };
+        half(std::integral_constant<int, 0>{});
+        half(std::integral_constant<int, 1>{});
+        rb_tiles_landed();                                            // tile j1, issued one tile ago
+        if (j2 < nkv) stage(j2, rb_next(rb_next(buf)));               // its buffer was last read before the previous barrier
+        rb_reads_done_barrier();
+        j = j1; w = w1;
+        j1 = j2; w1 = w2;
+        buf = rb_next(buf);
     }
     rb_store(dq, args.scale, const_cast<bf16_t*>(args.dq.p) + (size_t)b * args.dq.sb + (size_t)h * args.dq.sh + (size_t)qc * args.dq.ss, hi, qrow < S);
 
     if (args.part == nullptr) return;
     // ---- dT of this workgroup: the far sums join the outermost entries, then the copies are added up, then each bucket's run of distances ----
+    if (carry_at >= 0) put(carry_at + 8 * hi - q0 - l32 + p.reach + RB_PAD, carry);
     sum_r = wave_sum(sum_r);
     sum_l = wave_sum(sum_l);
     if (lane == 0) {                                                  // (wave-private, and behind the wave's own adds)
@@ -243,11 +285,11 @@ __global__ __launch_bounds__(1024) void relbias_attn_dtable_kernel(const float* 
 }
 
 template <int NW>
-__global__ __launch_bounds__(NW * 64) void relbias_attn_dkv_kernel(RbBwdArgs args) {
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void relbias_attn_dkv_kernel(RbBwdArgs args) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const RbArgs& p = args.a;
-    float* const rows = (float*)(smem + 2 * RB_BUF);                  // [buffer][L | δ][64]
-    float* const tab = (float*)(smem + 2 * RB_BUF + 1024);
+    float* const rows = (float*)(smem + RB_RING);                  // [buffer of three][L | δ][64]
+    float* const tab = (float*)(smem + RB_RING + 1536);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5, l32 = lane & 31;
     const int wave_s = __builtin_amdgcn_readfirstlane(wave);
     const int S = p.S;
@@ -284,7 +326,7 @@ __global__ __launch_bounds__(NW * 64) void relbias_attn_dkv_kernel(RbBwdArgs arg
         float next_l = 0.f, next_d = 0.f;
         // rows behind the last one repeat it: their P is 0 (L = +inf), and what they are multiplied with has to be a number
         auto stage = [&](int j, int buf) {
-            char* const dst = smem + buf * RB_BUF + wave_s * 1024;
+            char* const dst = smem + buf + wave_s * 1024;
 #pragma unroll
             for (int ps = 0; ps < 8 / NW; ++ps) {
                 const int r = (ps * NW + wave) * 8 + (lane >> 3), sw = ((lane & 7) ^ rb_swz(r)) << 4;
@@ -300,10 +342,13 @@ __global__ __launch_bounds__(NW * 64) void relbias_attn_dkv_kernel(RbBwdArgs arg
         };
         auto put_rows = [&](int buf) {
             if (tid < RB_KV) {
-                rows[buf * 128 + tid] = next_l;
-                rows[buf * 128 + 64 + tid] = next_d;
+                float* const to = rows + buf / RB_BUF * 128 + tid;
+                to[0] = next_l;
+                to[64] = next_d;
             }
         };
+        rb_arrived(kf);
+        rb_arrived(vf);
         int roff[4], toff[2][2];
         rb_row_offsets(lane, roff);
         rb_tr_offsets(lane, toff);
@@ -311,17 +356,19 @@ __global__ __launch_bounds__(NW * 64) void relbias_attn_dkv_kernel(RbBwdArgs arg
         const int nq = (S + RB_KV - 1) / RB_KV;
         stage(0, 0);
         put_rows(0);
+        if (nq > 1) stage(1, RB_BUF);
         drain_and_barrier();
+        int buf = 0;
         for (int j = 0; j < nq; ++j) {
-            const int buf = j & 1;
-            if (j + 1 < nq) stage(j + 1, buf ^ 1);
             if (some) {
-                const char* base = smem + buf * RB_BUF;
+                const char* base = smem + buf;
                 const int d_lo = k0 - (j * RB_KV + 63), d_hi = k0 + 31 - j * RB_KV;
                 const bool right = d_lo >= p.reach, left = d_hi <= -p.reach;
                 const float far = right ? far_r : far_l;
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
+                auto half = [&](auto t_tag, auto far_tag) {
+                    constexpr int t = decltype(t_tag)::value;
+                    constexpr bool FAR = decltype(far_tag)::value;
+                    // x[r], dp[r]: key l32, query 64j + 32t + 16(r >> 3) + 8hi + (r & 7)
                     f32x16 x, dp;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) { x[i] = 0.f; dp[i] = 0.f; }
@@ -332,43 +379,57 @@ __global__ __launch_bounds__(NW * 64) void relbias_attn_dkv_kernel(RbBwdArgs arg
                         dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(base + RB_TILE + t * 4096 + roff[ks]), vf[ks], dp, 0, 0, 0);
                     }
                     __builtin_amdgcn_s_setprio(0);
-                    // x[r], dp[r]: key l32, query 64j + 32t + 16(r >> 3) + 8hi + (r & 7)
-                    const float* lp = rows + buf * 128 + 32 * t + 8 * hi;
+                    const float* lp = rows + buf / RB_BUF * 128 + 32 * t + 8 * hi;
                     const float* tb = tab + (key - (j * RB_KV + 32 * t + 8 * hi) - 23 + p.reach + RB_PAD);   // of the last of the 16 queries
-                    f32x16 pr;
+                    unsigned pf[2][4], df[2][4];
 #pragma unroll
                     for (int s = 0; s < 2; ++s) {
                         const f32x4 l0 = *(const f32x4*)(lp + 16 * s), l1 = *(const f32x4*)(lp + 16 * s + 4);
                         const f32x4 e0 = *(const f32x4*)(lp + 64 + 16 * s), e1 = *(const f32x4*)(lp + 64 + 16 * s + 4);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const int r = 8 * s + e;
-                            const float l = e < 4 ? l0[e] : l1[e - 4], dl = e < 4 ? e0[e] : e1[e - 4];
-                            const float bias = right || left ? far : tb[23 - 16 * s - e];
-                            const float y = counts ? fmaf(x[r], p.c, bias - l) : -INFINITY;
-                            pr[r] = __builtin_amdgcn_exp2f(y);
-                            x[r] = pr[r] * (dp[r] - dl);
+                        for (int e = 0; e < 8; e += 2) {
+                            float pr[2], ds[2];
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                const int r = 8 * s + e + i;
+                                const float l = e < 4 ? l0[e + i] : l1[e + i - 4], dl = e < 4 ? e0[e + i] : e1[e + i - 4];
+                                const float bias = FAR ? far : tb[23 - 16 * s - e - i];
+                                pr[i] = __builtin_amdgcn_exp2f(counts ? fmaf(x[r], p.c, bias - l) : -INFINITY);
+                                ds[i] = pr[i] * (dp[r] - dl);
+                            }
+                            pf[s][e / 2] = pack_bf16x2(pr[0], pr[1]);
+                            df[s][e / 2] = pack_bf16x2(ds[0], ds[1]);
                         }
                     }
+                    bf16x8 qt[2][2], gt[2][2];
+                    rb_read_tr(gt, base + RB_TILE + t * 4096, toff);
+                    rb_read_tr(qt, base + t * 4096, toff);
                     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
                     for (int s = 0; s < 2; ++s) {
-                        const bf16x8 pf = __builtin_bit_cast(bf16x8, make_uint4(pack_bf16x2(pr[8 * s], pr[8 * s + 1]), pack_bf16x2(pr[8 * s + 2], pr[8 * s + 3]),
-                                                                                pack_bf16x2(pr[8 * s + 4], pr[8 * s + 5]), pack_bf16x2(pr[8 * s + 6], pr[8 * s + 7])));
-                        const bf16x8 ds = __builtin_bit_cast(bf16x8, make_uint4(pack_bf16x2(x[8 * s], x[8 * s + 1]), pack_bf16x2(x[8 * s + 2], x[8 * s + 3]),
-                                                                                pack_bf16x2(x[8 * s + 4], x[8 * s + 5]), pack_bf16x2(x[8 * s + 6], x[8 * s + 7])));
+                        const bf16x8 pv = __builtin_bit_cast(bf16x8, make_uint4(pf[s][0], pf[s][1], pf[s][2], pf[s][3]));
+                        const bf16x8 dv_ = __builtin_bit_cast(bf16x8, make_uint4(df[s][0], df[s][1], df[s][2], df[s][3]));
 #pragma unroll
                         for (int dt = 0; dt < 2; ++dt) {
-                            const char* qb = base + (2 * t + s) * 2048;
-                            dv[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(rb_read_tr(qb + RB_TILE + toff[dt][0], qb + RB_TILE + toff[dt][1]), pf, dv[dt], 0, 0, 0);
-                            dk[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(rb_read_tr(qb + toff[dt][0], qb + toff[dt][1]), ds, dk[dt], 0, 0, 0);
+                            dv[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(gt[s][dt], pv, dv[dt], 0, 0, 0);
+                            dk[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qt[s][dt], dv_, dk[dt], 0, 0, 0);
                         }
                     }
                     __builtin_amdgcn_s_setprio(0);
+                };
+                if (right || left) {
+                    half(std::integral_constant<int, 0>{}, std::true_type{});
+                    half(std::integral_constant<int, 1>{}, std::true_type{});
+                } else {
+                    half(std::integral_constant<int, 0>{}, std::false_type{});
+                    half(std::integral_constant<int, 1>{}, std::false_type{});
                 }
             }
-            if (j + 1 < nq) put_rows(buf ^ 1);
-            drain_and_barrier();
+            rb_tiles_landed();                                        // tile j + 1, issued one tile ago, and its rows' L and δ
+            put_rows(rb_next(buf));
+            if (j + 2 < nq) stage(j + 2, rb_next(rb_next(buf)));      // its buffer was last read before the previous barrier
+            rb_reads_done_barrier();
+            buf = rb_next(buf);
         }
     }
     // a key that does not count has P = dS = 0; times a NaN of some row's dO that would be a NaN
@@ -383,7 +444,7 @@ __global__ __launch_bounds__(NW * 64) void relbias_attn_dkv_kernel(RbBwdArgs arg
 static int rb_bwd_waves(const RbArgs& p, bool dtable) {
     // a wave's two tables of the distances have to fit beside the tiles
     int nw = rb_waves(p);
-    while (dtable && nw > 1 && 2 * RB_BUF + rb_table_bytes(p.reach) * (1 + 2 * nw) + rb_words_bytes(p) > 64 * 1024) nw /= 2;
+    while (dtable && nw > 1 && RB_RING + rb_table_bytes(p.reach) * (1 + 2 * nw) + rb_words_bytes(p) > 160 * 1024) nw /= 2;
     return nw;
 }
 
@@ -430,8 +491,8 @@ extern "C" int aether_relbias_attn_bwd(const AetherRelbias* d, const void* go, c
         nw = rb_bwd_waves(p, dtable != nullptr);
         p.nqb = (p.S + nw * 32 - 1) / (nw * 32);
         const dim3 grid((unsigned)((long)p.B * p.H * p.nqb));
-        const size_t lds_q = 2 * RB_BUF + rb_table_bytes(p.reach) * (dtable ? 1 + 2 * nw : 1) + rb_words_bytes(p);
-        const size_t lds_k = 2 * RB_BUF + 1024 + rb_table_bytes(p.reach);
+        const size_t lds_q = RB_RING + rb_table_bytes(p.reach) * (dtable ? 1 + 2 * nw : 1) + rb_words_bytes(p);
+        const size_t lds_k = RB_RING + 1536 + rb_table_bytes(p.reach);
 #define RB_LAUNCH(NW)                                                                                       \
     do {                                                                                                    \
         if (lds_q > 64 * 1024 && hipFuncSetAttribute((const void*)relbias_attn_dq_kernel<NW>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_q) != hipSuccess) \
