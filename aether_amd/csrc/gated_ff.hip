@@ -218,6 +218,177 @@ __global__ __launch_bounds__(512) void gated_ff_kernel(FfArgs p) {
     for (int mt = 0; mt < MT; ++mt) ff_finish<ET, ACT>(p, acc[mt][0], acc[mt][1], m0 + (wm * MT + mt) * 32 + l32, n, hi);
 }
 
+// ---- few rows: 16 pairs of columns a workgroup, straight from memory ----------------------------------------------------------------------------
+// Bound by reading the weights: every lane loads its 16 bytes of a weight row in the matrix unit's operand layout, with no LDS and no barrier in between.
+// A K tile is 128 bytes of 16 rows of Wg and of Wu; the workgroup's waves take every NW-th tile, many loads in flight each, and add up at the end through
+// LDS in the order of the waves.  x comes from the caches: MB blocks of 16 rows on v_mfma_f32_16x16x32_bf16 / v_mfma_..._16x16x128_f8f6f4; rows behind the last one
+// repeat it.
+typedef f32x4 FfAcc;
+AE_DEV FfAcc ff_mfma16(const i32x4 (&a)[2], const i32x4 (&b)[2], FfAcc c, bf16_t*) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a[s]), __builtin_bit_cast(bf16x8, b[s]), c, 0, 0, 0);
+    return c;
+}
+AE_DEV FfAcc ff_mfma16(const i32x4 (&a)[2], const i32x4 (&b)[2], FfAcc c, u8_t*) {
+    const i32x8 x = {a[0][0], a[0][1], a[0][2], a[0][3], a[1][0], a[1][1], a[1][2], a[1][3]};
+    const i32x8 y = {b[0][0], b[0][1], b[0][2], b[0][3], b[1][0], b[1][1], b[1][2], b[1][3]};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+}
+
+template <class ET, int MB, int ACT>      // MB: blocks of 16 rows
+__global__ __launch_bounds__(256) void gated_ff_rows_kernel(FfArgs p) {
+    constexpr int NW = 4, ES = FfType<ET>::SIZE, UNROLL = MB == 1 ? 4 : 2;
+    __shared__ __attribute__((aligned(16))) float part[NW][2][MB][64][4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, quad = lane >> 4;
+    const int n0 = blockIdx.x * 16;
+    const int nk = p.K * ES / 128;
+    // 16-byte chunks 4s + quad of a 128-byte tile (bf16: k = 32s + 8 quad ... of step s; e4m3: any order will do, the same in both operands)
+    const char* const g = (const char*)p.wg + (size_t)(n0 + l16) * p.ldw * ES + quad * 16;
+    const char* const u = (const char*)p.wu + (size_t)(n0 + l16) * p.ldw * ES + quad * 16;
+    const char* x[MB];
+#pragma unroll
+    for (int b = 0; b < MB; ++b) x[b] = (const char*)p.x + (size_t)min(b * 16 + l16, p.M - 1) * p.ldx * ES + quad * 16;
+    FfAcc ag[MB], au[MB];
+#pragma unroll
+    for (int b = 0; b < MB; ++b) { ag[b] = FfAcc{0.f, 0.f, 0.f, 0.f}; au[b] = ag[b]; }
+    auto step = [&](int kt, auto n_tag) {
+        constexpr int N = decltype(n_tag)::value;
+        i32x4 wg[N][2], wu[N][2], xv[N][MB][2];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const size_t at = (size_t)(kt + i * NW) * 128;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                wg[i][s] = *(const i32x4*)(g + at + 64 * s);
+                wu[i][s] = *(const i32x4*)(u + at + 64 * s);
+            }
+#pragma unroll
+            for (int b = 0; b < MB; ++b)
+#pragma unroll
+                for (int s = 0; s < 2; ++s) xv[i][b][s] = *(const i32x4*)(x[b] + at + 64 * s);
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int b = 0; b < MB; ++b) {
+                ag[b] = ff_mfma16(wg[i], xv[i][b], ag[b], (ET*)nullptr);
+                au[b] = ff_mfma16(wu[i], xv[i][b], au[b], (ET*)nullptr);
+            }
+    };
+    int kt = wave;
+    for (; kt + (UNROLL - 1) * NW < nk; kt += UNROLL * NW) step(kt, std::integral_constant<int, UNROLL>{});
+    for (; kt < nk; kt += NW) step(kt, std::integral_constant<int, 1>{});
+    // lane (token l16 of block b, columns 4 quad ... + 3)
+#pragma unroll
+    for (int b = 0; b < MB; ++b) {
+        *(FfAcc*)part[wave][0][b][lane] = ag[b];
+        *(FfAcc*)part[wave][1][b][lane] = au[b];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < MB * 64; i += 256) {
+        const int b = i >> 6, l = i & 63, m = b * 16 + (l & 15), n = n0 + 4 * (l >> 4);
+        if (m >= p.M) continue;
+        FfAcc a = *(const FfAcc*)part[0][0][b][l], c = *(const FfAcc*)part[0][1][b][l];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) { a += *(const FfAcc*)part[w][0][b][l]; c += *(const FfAcc*)part[w][1][b][l]; }
+        if constexpr (std::is_same<ET, u8_t>::value) {
+            const float sx = p.sx[m];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { a[e] *= sx * p.sg[n + e]; c[e] *= sx * p.su[n + e]; }
+        }
+        if (p.gu) {
+            *(FfAcc*)(p.gu + (size_t)m * 2 * p.F + n) = a;
+            *(FfAcc*)(p.gu + (size_t)m * 2 * p.F + p.F + n) = c;
+        }
+        *(uint2*)(p.h + (size_t)m * p.ldh + n) = make_uint2(pack_bf16x2(ff_act<ACT>(a[0]) * c[0], ff_act<ACT>(a[1]) * c[1]),
+                                                            pack_bf16x2(ff_act<ACT>(a[2]) * c[2], ff_act<ACT>(a[3]) * c[3]));
+    }
+}
+
+// ---- some rows: small tiles, several workgroups a CU ---------------------------------------------------------------------------------------------
+// 4 waves as WM x WN over (WM MT 32) rows x (WN 32) pairs of columns; the loads of the next K tile are in flight while this one is worked on, one barrier a tile.
+template <class ET, int WM, int WN, int MT, int NS, int ACT>
+__global__ __launch_bounds__(WM * WN * 64) void gated_ff_small_kernel(FfArgs p) {
+    constexpr int NW = WM * WN;
+    static_assert(NW == 4 || NW == 8, "4 or 8 wavefronts per workgroup");
+    constexpr int BM = WM * MT * 32, BN = WN * 32;
+    constexpr int X_TILE = BM * 128, W_TILE = WN * 64 * 128, BUF = X_TILE + W_TILE;
+    constexpr int X_ROUNDS = BM / (8 * NW), W_ROUNDS = WN * 8 / NW;   // 8 rows a wave-instruction
+    constexpr int SLOTS = FfType<ET>::SLOTS, CH = FfType<ET>::CHUNKS, ES = FfType<ET>::SIZE;
+    extern __shared__ __attribute__((aligned(16))) char smem_small[];
+    char* const smem = smem_small;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / WN, wn = wave % WN, hi = lane >> 5, l32 = lane & 31;
+    const int wave_s = __builtin_amdgcn_readfirstlane(wave);
+    const int id = xcd_remap((int)blockIdx.x, p.tiles_m * p.tiles_n);
+    const int tile_n = id / p.tiles_m, tile_m = id - tile_n * p.tiles_m;   // the row tiles of a column tile one after the other: its weights are read once
+    const int m0 = tile_m * BM, n0 = tile_n * BN;
+    const int srow = wave * 8 + (lane >> 3);
+    const unsigned schunk = ((lane & 7) ^ ((srow >> 1) & 7)) * 16;
+    unsigned x_off[X_ROUNDS], w_off[W_ROUNDS];
+#pragma unroll
+    for (int r = 0; r < X_ROUNDS; ++r) x_off[r] = (unsigned)min(m0 + r * (8 * NW) + srow, p.M - 1) * (unsigned)(p.ldx * ES) + schunk;
+    // rows 64 c ... + 31 of the W tile are rows 32 c ... of Wg, + 32 ... + 63 the same of Wu: a wave-instruction carries rows of one of them
+#pragma unroll
+    for (int r = 0; r < W_ROUNDS; ++r) {
+        const int row = r * (8 * NW) + srow;
+        w_off[r] = (unsigned)min(n0 + (row >> 6) * 32 + (row & 31), p.F - 1) * (unsigned)(p.ldw * ES) + schunk;
+    }
+    const buf_rsrc_t x_rsrc = make_buf_rsrc(p.x, p.x_bytes), g_rsrc = make_buf_rsrc(p.wg, p.w_bytes), u_rsrc = make_buf_rsrc(p.wu, p.w_bytes);
+    const int nk = p.K * ES / 128;
+    auto stage = [&](int kt, int buf) {
+        const unsigned soff = 128u * (unsigned)kt;
+        char* const dst = smem + buf * BUF + wave_s * 1024;
+#pragma unroll
+        for (int r = 0; r < W_ROUNDS; ++r) {
+            const bool up = ((r * NW + wave_s) & 4) != 0;
+            bglds16(up ? u_rsrc : g_rsrc, w_off[r], soff, dst + X_TILE + r * (NW * 1024));
+        }
+#pragma unroll
+        for (int r = 0; r < X_ROUNDS; ++r) bglds16(x_rsrc, x_off[r], soff, dst + r * (NW * 1024));
+    };
+    const int swz = (lane >> 1) & 7;
+    const int x_row = (wm * MT * 32 + l32) * 128, w_row = X_TILE + (wn * 64 + l32) * 128;
+    f32x16 acc[MT][2];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) { acc[mt][0][i] = 0.f; acc[mt][1][i] = 0.f; }
+    // a ring of NS buffers; past the last K tile it is fetched again, into a buffer that nobody reads any more, so that the counts of loads stay the same
+    constexpr int PIECES = W_ROUNDS + X_ROUNDS;
+#pragma unroll
+    for (int i = 0; i < NS - 1; ++i) stage(min(i, nk - 1), i);
+    int buf = 0;
+    for (int kt = 0; kt < nk; ++kt) {
+        wait_vmcnt<(NS - 2) * PIECES>();                              // this wave's part of tile kt has landed
+        block_barrier();                                              // everybody's; and tile kt - 1 has been read by all
+        stage(min(kt + NS - 1, nk - 1), buf == 0 ? NS - 1 : buf - 1);
+        const char* base = smem + buf * BUF;
+        buf = buf == NS - 1 ? 0 : buf + 1;
+#pragma unroll
+        for (int sl = 0; sl < SLOTS; ++sl) {
+            i32x4 wf[2][CH], xf[MT][CH];
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                const int off = ((2 * (sl * CH + c) + hi) ^ swz) << 4;
+#pragma unroll
+                for (int t = 0; t < 2; ++t) wf[t][c] = *(const i32x4*)(base + w_row + t * 4096 + off);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) xf[mt][c] = *(const i32x4*)(base + x_row + mt * 4096 + off);
+            }
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) acc[mt][t] = ff_mfma(wf[t], xf[mt], acc[mt][t]);
+        }
+        wait_lgkmcnt0();
+    }
+    wait_vmcnt<0>();                                                  // nothing arrives in LDS behind the workgroup's end
+    const int n = n0 + wn * 32;
+    if (n >= p.F) return;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) ff_finish<ET, ACT>(p, acc[mt][0], acc[mt][1], m0 + (wm * MT + mt) * 32 + l32, n, hi);
+}
+
 // ---- backward ------------------------------------------------------------------------------------------------------------------------------
 // dg = dh u act'(g), du = dh act(g), as [M][2F] for the product with the weights and transposed, [2F][Mp], for the one with x.  A workgroup turns a
 // 64 x 64 piece through LDS.  Columns M ... Mp − 1 of the transposed form are zeros.
@@ -293,6 +464,28 @@ static int ff_check(const void* x, long ldx, const void* wg, const void* wu, lon
     return AETHER_OK;
 }
 
+// Which kernel, from the sizes alone.  A tile kernel runs its workgroups in rounds of one a CU; a round's time is that of one workgroup's K loop, measured per
+// K tile of 128 bytes (K = 4096, F = 1024 ... 10240, µs): 64 x 64 (rows x pairs of columns) 0.42, 128 x 64 0.6, 128 x 128 and 256 x 64 0.9, the 256 x 128
+// kernel with alternating waves 1.45.  The least rounds x time wins; for instance, bf16, F = 10240: 64 rows 37 µs (256 x 128: 91), 128 rows 46 (91), 226 rows
+// 59 (92), 300 rows 65 (96), 400 rows 95 with 256 x 128 (the others 110 and more), 1024 rows 184 (199), 2048 rows 300.
+// The kernel without tiles splits K over its waves and needs no round: up to 32 rows it is ahead where F / 64 workgroups of the smallest tile leave most CUs
+// idle (F = 2048, K = 4096: 1 row 12 µs against 23, 32 rows 18.5 against 23.5; F = 8192, K = 2048: 16 rows 14.5 against 15.3, 32 rows 18.6 against 15.6).
+enum FfVariant { FF_ROWS_16, FF_ROWS_32, FF_64X64, FF_128X64, FF_128X128, FF_256X64, FF_256X128 };
+static FfVariant ff_variant(int M, int F) {
+    if (M <= 16 && F <= 8192) return FF_ROWS_16;
+    if (M <= 32 && F <= 4096) return FF_ROWS_32;
+    static const struct { FfVariant v; int rows, pairs; float us; } tile[] = {
+        {FF_64X64, 64, 64, 0.42f}, {FF_128X64, 128, 64, 0.6f}, {FF_256X64, 256, 64, 0.9f}, {FF_128X128, 128, 128, 0.9f}, {FF_256X128, 256, 128, 1.45f}};
+    FfVariant best = FF_256X128;
+    float least = 3e38f;
+    for (const auto& t : tile) {
+        const long groups = (long)((M + t.rows - 1) / t.rows) * ((F + t.pairs - 1) / t.pairs);
+        const float us = (float)((groups + 255) / 256) * t.us;
+        if (us < least) { least = us; best = t.v; }
+    }
+    return best;
+}
+
 template <class ET>
 static int ff_forward(FfArgs p, int act, hipStream_t s) {
     constexpr int ES = FfType<ET>::SIZE;
@@ -315,7 +508,38 @@ static int ff_forward(FfArgs p, int act, hipStream_t s) {
         if (act == ACT_SILU) hipLaunchKernelGGL((gated_ff_kernel<ET, WM, WN, MT, ACT_SILU>), grid, dim3(512), 0, s, p);                \
         else hipLaunchKernelGGL((gated_ff_kernel<ET, WM, WN, MT, ACT_GELU_TANH>), grid, dim3(512), 0, s, p);                           \
     } while (0)
-        FF_LAUNCH(2, 4, 4);
+#define FF_SMALL(WM, WN, MT)                                                                                                           \
+    do {                                                                                                                               \
+        constexpr int NS = 3, LDS = NS * (WM * MT * 32 + WN * 64) * 128;                                                               \
+        p.tiles_m = (p.M + WM * MT * 32 - 1) / (WM * MT * 32);                                                                         \
+        p.tiles_n = (p.F + WN * 32 - 1) / (WN * 32);                                                                                   \
+        const dim3 grid(p.tiles_m * p.tiles_n), block(WM * WN * 64);                                                                   \
+        const void* f = act == ACT_SILU ? (const void*)gated_ff_small_kernel<ET, WM, WN, MT, NS, ACT_SILU>                             \
+                                        : (const void*)gated_ff_small_kernel<ET, WM, WN, MT, NS, ACT_GELU_TANH>;                       \
+        if (LDS > 64 * 1024 && hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) {                \
+            (void)hipGetLastError();                                                                                                   \
+            return aether_set_error(AETHER_ERR_LAUNCH, "gated_ff: the workgroup's LDS could not be set");                              \
+        }                                                                                                                              \
+        if (act == ACT_SILU) hipLaunchKernelGGL((gated_ff_small_kernel<ET, WM, WN, MT, NS, ACT_SILU>), grid, block, LDS, s, p);        \
+        else hipLaunchKernelGGL((gated_ff_small_kernel<ET, WM, WN, MT, NS, ACT_GELU_TANH>), grid, block, LDS, s, p);                   \
+    } while (0)
+#define FF_ROWS(MB)                                                                                                                    \
+    do {                                                                                                                               \
+        const dim3 grid(p.F / 16);                                                                                                     \
+        if (act == ACT_SILU) hipLaunchKernelGGL((gated_ff_rows_kernel<ET, MB, ACT_SILU>), grid, dim3(256), 0, s, p);                   \
+        else hipLaunchKernelGGL((gated_ff_rows_kernel<ET, MB, ACT_GELU_TANH>), grid, dim3(256), 0, s, p);                              \
+    } while (0)
+        switch (ff_variant(p.M, p.F)) {
+            case FF_ROWS_16: FF_ROWS(1); break;
+            case FF_ROWS_32: FF_ROWS(2); break;
+            case FF_64X64: FF_SMALL(2, 2, 1); break;
+            case FF_128X64: FF_SMALL(4, 2, 1); break;
+            case FF_128X128: FF_SMALL(2, 4, 2); break;
+            case FF_256X64: FF_SMALL(4, 2, 2); break;
+            default: FF_LAUNCH(2, 4, 4); break;
+        }
+#undef FF_ROWS
+#undef FF_SMALL
 #undef FF_LAUNCH
         int rc = aether_check_launch("gated_ff");
         if (rc) return rc;

@@ -68,6 +68,25 @@ def test_rows_e4m3(cuda, hip_lib, M, act):
         assert ((got.double() - ref).norm() / ref.norm()).item() < 0.15
 
 
+# each way the work is cut into tiles, whole and ragged ones (which way is chosen goes by rows and columns; K may stay small)
+TILINGS = [(1, 10240), (16, 8192), (17, 10240), (64, 10240), (65, 10240), (100, 10272), (128, 10240), (129, 10240), (200, 10240), (226, 10240), (256, 10272), (257, 10240),
+           (300, 10240), (383, 10272), (400, 10240), (513, 10240), (1024, 4096), (1100, 1056)]
+
+
+@pytest.mark.parametrize("M,F", TILINGS)
+def test_tilings(cuda, hip_lib, M, F):
+    from aether_amd import ops
+    K = 256
+    x, wg, wu, dh = _inputs(M, K, F, cuda, seed=9)
+    for act in ("gelu_tanh", "silu"):
+        h, lim = _forward(x.double(), wg.double(), wu.double(), act)[:2]
+        _within(ops.gated_ff(x, wg, wu, act), h, lim, (M, K, F))
+        (xq, xs), (gq, gs), (uq, us) = (ops.quantize_rows_e4m3(t) for t in (x, wg, wu))
+        h, lim = _forward(*(q.float().double() * s.double()[:, None] for q, s in ((xq, xs), (gq, gs), (uq, us))), act, 2.0 ** -12)[:2]
+        _within(ops.gated_ff_e4m3(xq, xs, gq, gs, uq, us, act), h, lim, (M, K, F))
+    _check_backward(x, wg, wu, dh, "gelu_tanh")
+
+
 @pytest.mark.parametrize("M,K,F", [(300, 4096, 1056), (1, 4096, 10240), (33, 2048, 4128), (700, 64, 2080), (2049, 128, 544), (226, 1024, 2848)])
 def test_larger(cuda, hip_lib, M, K, F):
     """Grids of many workgroups and long sums; every element is compared."""
