@@ -24,8 +24,11 @@ namespace aether {
 
 struct RbFwdArgs { RbArgs a; bf16_t* o; bf16_t* o_low; float* lse; };   // o_low, lse: for a backward pass
 
-template <int NW, bool TRAIN>
-__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(3, 3))) void relbias_attn_fwd_kernel(RbFwdArgs args) {
+// tiles from which the pipelined loop is used: its start and end cost about two tiles' time, its registers the third wave of a SIMD
+constexpr int RB_PIPE_TILES = 7;
+
+template <int NW, bool TRAIN, bool PIPE>
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(PIPE ? 2 : 3, PIPE ? 2 : 3))) void relbias_attn_fwd_kernel(RbFwdArgs args) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const RbArgs& p = args.a;
     float* const tab = (float*)(smem + RB_RING);
@@ -51,8 +54,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(3, 3)))
     }
     // ---- staging: a wave-instruction moves 8 rows x 128 bytes; rows at or beyond S are outside the descriptor and their keys do not count ----
     const unsigned k_row = (unsigned)p.k.ss * 2, v_row = (unsigned)p.v.ss * 2;
-    const buf_rsrc_t k_rsrc = make_buf_rsrc(p.k.p + (size_t)b * p.k.sb + (size_t)h * p.k.sh, (unsigned)(S - 1) * k_row + 128);
-    const buf_rsrc_t v_rsrc = make_buf_rsrc(p.v.p + (size_t)b * p.v.sb + (size_t)h * p.v.sh, (unsigned)(S - 1) * v_row + 128);
+    const i32x4 k_rsrc = rb_rsrc(p.k.p + (size_t)b * p.k.sb + (size_t)h * p.k.sh, (unsigned)(S - 1) * k_row + 128);
+    const i32x4 v_rsrc = rb_rsrc(p.v.p + (size_t)b * p.v.sb + (size_t)h * p.v.sh, (unsigned)(S - 1) * v_row + 128);
     unsigned k_off[8 / NW], v_off[8 / NW];
 #pragma unroll
     for (int ps = 0; ps < 8 / NW; ++ps) {
@@ -60,13 +63,19 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(3, 3)))
         k_off[ps] = r * k_row + ((ch ^ rb_swz(r)) << 4);
         v_off[ps] = r * v_row + ((ch ^ rb_swz(r)) << 4);
     }
-    auto stage = [&](int j, int buf) {
-        char* const dst = smem + buf + wave_s * 1024;
+    auto stage_k = [&](int j, int buf) {
+        const unsigned dst = rb_lds(smem) + buf + wave_s * 1024;
 #pragma unroll
-        for (int ps = 0; ps < 8 / NW; ++ps) {
-            bglds16(k_rsrc, k_off[ps], (unsigned)j * (RB_KV * k_row), dst + ps * (NW * 1024));
-            bglds16(v_rsrc, v_off[ps], (unsigned)j * (RB_KV * v_row), dst + RB_TILE + ps * (NW * 1024));
-        }
+        for (int ps = 0; ps < 8 / NW; ++ps) rb_dma16(k_rsrc, k_off[ps], (unsigned)j * (RB_KV * k_row), dst + ps * (NW * 1024));
+    };
+    auto stage_v = [&](int j, int buf) {
+        const unsigned dst = rb_lds(smem) + buf + RB_TILE + wave_s * 1024;
+#pragma unroll
+        for (int ps = 0; ps < 8 / NW; ++ps) rb_dma16(v_rsrc, v_off[ps], (unsigned)j * (RB_KV * v_row), dst + ps * (NW * 1024));
+    };
+    auto stage = [&](int j, int buf) {
+        stage_k(j, buf);
+        stage_v(j, buf);
     };
     int koff[4], voff[2][2];
     rb_row_offsets(lane, koff);
@@ -87,126 +96,285 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(3, 3)))
             if ((w = rb_word(p, words, j)) != 0) break;
         return j;
     };
-    uint64_t w = 0, w1 = 0, w2 = 0;
-    int j = next_tile(0, w), j1 = next_tile(j + 1, w1);
-    int buf = 0;
-    if (j < nkv) stage(j, 0);
-    if (j1 < nkv) stage(j1, RB_BUF);
-    drain_and_barrier();
-    while (j < nkv) {
-        const char* base = smem + buf;
-        const int j2 = next_tile(j1 + 1, w2);
-        f32x16 x[2];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) { x[0][i] = 0.f; x[1][i] = 0.f; }
-        __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int ks = 0; ks < 4; ++ks)
-                x[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(base + t * 4096 + koff[ks]), qf[ks], x[t], 0, 0, 0);
-        __builtin_amdgcn_s_setprio(0);
-        // x[t][r]: query l32, key 64j + 32t + 16(r >> 3) + 8hi + (r & 7)
-        const int d_lo = j * RB_KV - (q0 + 31), d_hi = j * RB_KV + 63 - q0;
-        const bool right = d_lo >= p.reach, left = d_hi <= -p.reach;
-        const bool part = w != ~0ull;
-        // One half of the tile: soft-max, then its share of Oᵀ += Vᵀ·Pᵀ.  The first half's soft-max runs behind the second half's scores on the matrix pipe,
-        // the second half's behind the first half's products.
-        auto half = [&](auto t_tag) {
-            constexpr int t = decltype(t_tag)::value;
-            const unsigned wt = (unsigned)(w >> (32 * t));
-            if (part && wt == 0) return;                              // (wave-uniform) no key in this half
-            if (right || left) {
-                const float add = (right ? far_r : far_l) - m_run;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) x[t][r] = fmaf(x[t][r], p.c, add);
-            } else {
-                // |d| <= reach + 94 here: inside the padded table.  A query row beyond the last one reads inside it too (its wave's own range).
-                const float* tb = tab + (j * RB_KV + 32 * t + 8 * hi - qrow + p.reach + RB_PAD);
-#pragma unroll
-                for (int r = 0; r < 16; ++r) x[t][r] = fmaf(x[t][r], p.c, tb[16 * (r >> 3) + (r & 7)] - m_run);
-            }
-            if (__builtin_expect(part, 0)) {
-                const unsigned mine = wt >> (8 * hi);
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (!((mine >> (16 * (r >> 3) + (r & 7))) & 1)) x[t][r] = -INFINITY;
-            }
-            unsigned pf[2][4], pl[2][4];
-            float tsum = 0.f;
-            auto expo = [&]() {
-                float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-                for (int s = 0; s < 2; ++s)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float pa = __builtin_amdgcn_exp2f(x[t][8 * s + 2 * e]), pb = __builtin_amdgcn_exp2f(x[t][8 * s + 2 * e + 1]);
-                        pf[s][e] = pack_bf16x2(pa, pb);
-                        if constexpr (TRAIN) {
-                            pl[s][e] = pack_bf16x2(pa - __uint_as_float(pf[s][e] << 16), pb - __uint_as_float(pf[s][e] & 0xffff0000u));
-                            s0 += pa;
-                            s1 += pb;
-                        } else {                                      // the sum of the rounded values: numerator and denominator round alike, one instruction a pair
-                            bf16x2 ones;
-                            ones[0] = (__bf16)1.0f; ones[1] = (__bf16)1.0f;
-                            if (e & 1) s1 = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pf[s][e]), ones, s1, false);
-                            else s0 = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pf[s][e]), ones, s0, false);
+    // Tile by tile from `first` on, any tile: the tiles in front of it are done.
+    auto sweep = [&](int first) {
+        uint64_t w = 0, w1 = 0, w2 = 0;
+        int j = next_tile(first, w), j1 = next_tile(j + 1, w1);
+        int buf = 0;
+        if (j < nkv) stage(j, 0);
+        if (j1 < nkv) stage(j1, RB_BUF);
+        drain_and_barrier();
+        while (j < nkv) {
+            const char* base = smem + buf;
+            const int j2 = next_tile(j1 + 1, w2);
+            f32x16 x[2];
+    #pragma unroll
+            for (int i = 0; i < 16; ++i) { x[0][i] = 0.f; x[1][i] = 0.f; }
+    #pragma unroll
+            for (int t = 0; t < 2; ++t)
+    #pragma unroll
+                for (int ks = 0; ks < 4; ++ks)
+                    x[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(base + t * 4096 + koff[ks]), qf[ks], x[t], 0, 0, 0);
+            // x[t][r]: query l32, key 64j + 32t + 16(r >> 3) + 8hi + (r & 7)
+            const int d_lo = j * RB_KV - (q0 + 31), d_hi = j * RB_KV + 63 - q0;
+            const bool right = d_lo >= p.reach, left = d_hi <= -p.reach;
+            const bool part = w != ~0ull;
+            // One half of the tile: soft-max, then its share of Oᵀ += Vᵀ·Pᵀ.  The first half's soft-max runs behind the second half's scores on the matrix pipe,
+            // the second half's behind the first half's products.
+            auto half = [&](auto t_tag) {
+                constexpr int t = decltype(t_tag)::value;
+                const unsigned wt = (unsigned)(w >> (32 * t));
+                if (part && wt == 0) return;                              // (wave-uniform) no key in this half
+                if (right || left) {
+                    const float add = (right ? far_r : far_l) - m_run;
+    #pragma unroll
+                    for (int r = 0; r < 16; ++r) x[t][r] = fmaf(x[t][r], p.c, add);
+                } else {
+                    // |d| <= reach + 94 here: inside the padded table.  A query row beyond the last one reads inside it too (its wave's own range).
+                    const float* tb = tab + (j * RB_KV + 32 * t + 8 * hi - qrow + p.reach + RB_PAD);
+    #pragma unroll
+                    for (int r = 0; r < 16; ++r) x[t][r] = fmaf(x[t][r], p.c, tb[16 * (r >> 3) + (r & 7)] - m_run);
+                }
+                if (__builtin_expect(part, 0)) {
+                    const unsigned mine = wt >> (8 * hi);
+    #pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (!((mine >> (16 * (r >> 3) + (r & 7))) & 1)) x[t][r] = -INFINITY;
+                }
+                unsigned pf[2][4], pl[2][4];
+                float tsum = 0.f;
+                auto expo = [&]() {
+                    float s0 = 0.f, s1 = 0.f;
+    #pragma unroll
+                    for (int s = 0; s < 2; ++s)
+    #pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float pa = __builtin_amdgcn_exp2f(x[t][8 * s + 2 * e]), pb = __builtin_amdgcn_exp2f(x[t][8 * s + 2 * e + 1]);
+                            pf[s][e] = pack_bf16x2(pa, pb);
+                            if constexpr (TRAIN) {
+                                pl[s][e] = pack_bf16x2(pa - __uint_as_float(pf[s][e] << 16), pb - __uint_as_float(pf[s][e] & 0xffff0000u));
+                                s0 += pa;
+                                s1 += pb;
+                            } else {                                      // the sum of the rounded values: numerator and denominator round alike, one instruction a pair
+                                bf16x2 ones;
+                                ones[0] = (__bf16)1.0f; ones[1] = (__bf16)1.0f;
+                                if (e & 1) s1 = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pf[s][e]), ones, s1, false);
+                                else s0 = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pf[s][e]), ones, s0, false);
+                            }
                         }
+                    tsum = s0 + s1;
+                };
+                bool redo = !started;
+                if (!redo) {
+                    expo();
+                    redo = __any(!(tsum <= 1.2676506e30f)) != 0;          // 2^100
+                }
+                if (__builtin_expect(redo, 0)) {
+                    float top = x[t][0];
+    #pragma unroll
+                    for (int r = 1; r < 16; ++r) top = fmaxf(top, x[t][r]);
+                    top = fmaxf(top, __shfl_xor(top, 32, 64));
+                    const float up = started ? fmaxf(top, 0.f) : top == -INFINITY ? 0.f : top;
+                    if (started) {
+                        const float alpha = __builtin_amdgcn_exp2f(-up);
+    #pragma unroll
+                        for (int i = 0; i < 16; ++i) { o[0][i] *= alpha; o[1][i] *= alpha; }
+                        l_run *= alpha;
                     }
-                tsum = s0 + s1;
-            };
-            bool redo = !started;
-            if (!redo) {
-                expo();
-                redo = __any(!(tsum <= 1.2676506e30f)) != 0;          // 2^100
-            }
-            if (__builtin_expect(redo, 0)) {
-                float top = x[t][0];
-#pragma unroll
-                for (int r = 1; r < 16; ++r) top = fmaxf(top, x[t][r]);
-                top = fmaxf(top, __shfl_xor(top, 32, 64));
-                const float up = started ? fmaxf(top, 0.f) : top == -INFINITY ? 0.f : top;
-                if (started) {
-                    const float alpha = __builtin_amdgcn_exp2f(-up);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) { o[0][i] *= alpha; o[1][i] *= alpha; }
-                    l_run *= alpha;
+                    m_run += up;
+    #pragma unroll
+                    for (int i = 0; i < 16; ++i) x[t][i] -= up;
+                    expo();
+                    started = true;
                 }
-                m_run += up;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) x[t][i] -= up;
-                expo();
-                started = true;
-            }
-            l_run += tsum;
-            bf16x8 vf[2][2];
-            rb_read_tr(vf, base + RB_TILE + t * 4096, voff);
-            if (__builtin_expect(part, 0)) {
-#pragma unroll
+                l_run += tsum;
+                bf16x8 vf[2][2];
+                rb_read_tr(vf, base + RB_TILE + t * 4096, voff);
+                if (__builtin_expect(part, 0)) {
+    #pragma unroll
+                    for (int s = 0; s < 2; ++s)
+    #pragma unroll
+                        for (int dt = 0; dt < 2; ++dt) vf[s][dt] = rb_keep(vf[s][dt], (wt >> (16 * s + 8 * hi)) & 0xffu);
+                }
+    #pragma unroll
                 for (int s = 0; s < 2; ++s)
+    #pragma unroll
+                    for (int dt = 0; dt < 2; ++dt) {
+                        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[s][dt], __builtin_bit_cast(bf16x8, make_uint4(pf[s][0], pf[s][1], pf[s][2], pf[s][3])), o[dt], 0, 0, 0);
+                        if constexpr (TRAIN)
+                            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[s][dt], __builtin_bit_cast(bf16x8, make_uint4(pl[s][0], pl[s][1], pl[s][2], pl[s][3])), o[dt], 0, 0, 0);
+                    }
+            };
+            half(std::integral_constant<int, 0>{});
+            half(std::integral_constant<int, 1>{});
+            rb_tiles_landed();                                            // tile j1, issued one tile ago
+            if (j2 < nkv) stage(j2, rb_next(rb_next(buf)));               // its buffer was last read before the previous barrier
+            rb_reads_done_barrier();
+            j = j1; w = w1;
+            j1 = j2; w1 = w2;
+            buf = rb_next(buf);
+        }
+    };
+
+    // ---- the run of whole tiles at the front, in a pipeline --------------------------------------------------------------------------------------------
+    // VALU issued between a wave's own matrix instructions runs behind them, that of the SIMD's other waves mostly does not: the soft-max of one half of a tile
+    // is spread over eight matrix instructions, four of the other half's scores and four of the previous half's products.  Iteration j:
+    //   scores of (j, half 1) and products of (j − 1, half 1)  behind them the soft-max of (j, half 0)
+    //   products of (j, half 0) and scores of (j + 1, half 0)   behind them the soft-max of (j, half 1)
+    // K runs one tile ahead of V.  The shift is the maximum of the row's first 32 scores throughout; whether an exp2 left fp32's range shows in the finished
+    // row (a sum or an output that is not finite): the workgroup then starts over with the tile-by-tile loop.
+    auto pipeline = [&](int n) {
+        constexpr int KO = 0, VO = RB_TILE;
+        int kb = 0, kb1 = RB_BUF, kb2 = 2 * RB_BUF;                   // buffers of K(j), K(j + 1), K(j + 2); V(j) is in the same as K(j)
+        stage_k(0, kb);
+        stage_v(0, kb);
+        stage_k(1, kb1);
+        drain_and_barrier();
+        if (n > 2) stage_k(2, kb2);
+        stage_v(1, kb1);
+        f32x16 x0, x1;
+        bf16x8 ka[4], kc[4], va[2][2], vc[2][2];                      // fragments for the first and the second half of an iteration
+        unsigned p0[2][4], p1[2][4], l0[2][4], l1[2][4];
+        auto scores = [&](int ks, const bf16x8& k, f32x16& x) {
+            if (ks == 0) {
 #pragma unroll
-                    for (int dt = 0; dt < 2; ++dt) vf[s][dt] = rb_keep(vf[s][dt], (wt >> (16 * s + 8 * hi)) & 0xffu);
+                for (int i = 0; i < 16; ++i) x[i] = 0.f;
             }
-            __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int dt = 0; dt < 2; ++dt) {
-                    o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[s][dt], __builtin_bit_cast(bf16x8, make_uint4(pf[s][0], pf[s][1], pf[s][2], pf[s][3])), o[dt], 0, 0, 0);
-                    if constexpr (TRAIN)
-                        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[s][dt], __builtin_bit_cast(bf16x8, make_uint4(pl[s][0], pl[s][1], pl[s][2], pl[s][3])), o[dt], 0, 0, 0);
-                }
-            __builtin_amdgcn_s_setprio(0);
+            x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, qf[ks], x, 0, 0, 0);
         };
-        half(std::integral_constant<int, 0>{});
-        half(std::integral_constant<int, 1>{});
-        rb_tiles_landed();                                            // tile j1, issued one tile ago
-        if (j2 < nkv) stage(j2, rb_next(rb_next(buf)));               // its buffer was last read before the previous barrier
-        rb_reads_done_barrier();
-        j = j1; w = w1;
-        j1 = j2; w1 = w2;
-        buf = rb_next(buf);
+        auto frag = [&](const unsigned (&f)[4]) { return __builtin_bit_cast(bf16x8, make_uint4(f[0], f[1], f[2], f[3])); };
+        auto product = [&](int i, const bf16x8 (&v)[2][2], const unsigned (&p)[2][4], const unsigned (&l)[2][4]) {   // i: 2 s + dt
+            o[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[i >> 1][i & 1], frag(p[i >> 1]), o[i & 1], 0, 0, 0);
+            if constexpr (TRAIN) o[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[i >> 1][i & 1], frag(l[i >> 1]), o[i & 1], 0, 0, 0);
+        };
+        float s0 = 0.f, s1 = 0.f;
+        auto soft = [&](int e, const f32x16& x, unsigned (&p)[2][4], unsigned (&l)[2][4], float add, auto near_tag) {   // elements 2e, 2e + 1
+            const bool NEAR = decltype(near_tag)::value;
+            const float a = __builtin_amdgcn_exp2f(NEAR ? x[2 * e] : fmaf(x[2 * e], args.a.c, add));
+            const float b = __builtin_amdgcn_exp2f(NEAR ? x[2 * e + 1] : fmaf(x[2 * e + 1], args.a.c, add));
+            const unsigned pk = pack_bf16x2(a, b);
+            p[e >> 2][e & 3] = pk;
+            if constexpr (TRAIN) {
+                l[e >> 2][e & 3] = pack_bf16x2(a - __uint_as_float(pk << 16), b - __uint_as_float(pk & 0xffff0000u));
+                s0 += a;
+                s1 += b;
+            } else {
+                bf16x2 ones;
+                ones[0] = (__bf16)1.0f; ones[1] = (__bf16)1.0f;
+                if (e & 1) s1 = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pk), ones, s1, false);
+                else s0 = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pk), ones, s0, false);
+            }
+        };
+        auto biased = [&](f32x16& x, int at) {                        // scale, bias and shift of 16 scores near the diagonal
+            const float* tb = tab + (at + 8 * hi - qrow + p.reach + RB_PAD);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x[r] = fmaf(x[r], p.c, tb[16 * (r >> 3) + (r & 7)] - m_run);
+        };
+        auto sides = [&](int j, bool& right, bool& left) {
+            right = j * RB_KV - (q0 + 31) >= p.reach;
+            left = j * RB_KV + 63 - q0 <= -p.reach;
+        };
+        // scores of (0, half 0): their maximum is the rows' shift
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) scores(ks, *(const bf16x8*)(smem + kb + KO + koff[ks]), x0);
+        {
+            f32x16 y = x0;
+            bool right, left;
+            sides(0, right, left);
+            if (right || left) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) y[r] = fmaf(y[r], p.c, right ? far_r : far_l);
+            } else biased(y, 0);
+            float top = y[0];
+#pragma unroll
+            for (int r = 1; r < 16; ++r) top = fmaxf(top, y[r]);
+            m_run = fmaxf(top, __shfl_xor(top, 32, 64));
+        }
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) ka[ks] = *(const bf16x8*)(smem + kb + KO + 4096 + koff[ks]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) va[i >> 1][i & 1] = bf16x8{};
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { p1[s][e] = 0; l1[s][e] = 0; }   // (0, half 1) has no predecessor: zeros times zeros
+        auto turn = [&](int j, float add, auto near_tag) {
+            if constexpr (decltype(near_tag)::value) biased(x0, j * RB_KV);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                vc[i >> 1][i & 1] = rb_read_tr1(smem + kb + VO + 2048 * (i >> 1), voff[i & 1]);      // for the second half of the iteration
+                kc[i] = *(const bf16x8*)(smem + kb1 + KO + koff[i]);
+                scores(i, ka[i], x1);
+                soft(2 * i, x0, p0, l0, add, near_tag);
+                __builtin_amdgcn_sched_barrier(0);
+                product(i, va, p1, l1);
+                soft(2 * i + 1, x0, p0, l0, add, near_tag);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if constexpr (decltype(near_tag)::value) biased(x1, j * RB_KV + 32);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                va[i >> 1][i & 1] = rb_read_tr1(smem + kb + VO + 4096 + 2048 * (i >> 1), voff[i & 1]);   // for the next iteration's first half
+                ka[i] = *(const bf16x8*)(smem + kb1 + KO + 4096 + koff[i]);
+                product(i, vc, p0, l0);
+                soft(2 * i, x1, p1, l1, add, near_tag);
+                __builtin_amdgcn_sched_barrier(0);
+                scores(i, kc[i], x0);
+                soft(2 * i + 1, x1, p1, l1, add, near_tag);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            // K(j + 2) and V(j + 1) have landed.  V(j)'s and K(j + 1)'s reads above may still be on their way; K(j)'s and V(j - 1)'s, whose buffers are
+            // filled now, have been used.
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            block_barrier();
+            if (j + 3 < n) stage_k(j + 3, kb);
+            if (j + 2 < n) stage_v(j + 2, kb2);
+            const int was = kb;
+            kb = kb1; kb1 = kb2; kb2 = was;
+        };
+        // three loops, so that each has one body: tiles left of the wave's diagonal, along it, right of it.  The workgroup's waves change over at
+        // different tiles; every iteration has the same one barrier.
+        const int near_from = min(n, max(0, (q0 - p.reach - 63) / RB_KV + (q0 - p.reach - 63 >= 0 ? 1 : 0)));   // the first tile with 64j + 63 - q0 > -reach
+        const int near_to = min(n, (q0 + 31 + p.reach + RB_KV - 1) / RB_KV);                                    // the first with 64j - q0 - 31 >= reach
+        int j = 0;
+        for (; j < near_from; ++j) turn(j, far_l - m_run, std::false_type{});
+        for (; j < near_to; ++j) turn(j, 0.f, std::true_type{});
+        for (; j < n; ++j) turn(j, far_r - m_run, std::false_type{});
+#pragma unroll
+        for (int i = 0; i < 4; ++i) product(i, va, p1, l1);
+        l_run = s0 + s1;
+        started = true;
+        drain_and_barrier();
+    };
+    int whole = 0;                                                    // tiles at the front whose keys all count
+    if (PIPE && p.mask == nullptr) whole = S / RB_KV;
+    else if (PIPE) {
+        for (int at = 0;; at += 64) {
+            const uint64_t less = __ballot(at + lane >= nkv || words[min(at + lane, nkv - 1)] != ~0ull);
+            if (less) { whole = at + __builtin_ctzll(less); break; }
+        }
     }
+    if (PIPE && whole >= RB_PIPE_TILES) {
+        pipeline(whole);
+        if (whole < nkv) sweep(whole);
+        float worst = fabsf(l_run);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) worst = fmaxf(worst, fmaxf(fabsf(o[0][i]), fabsf(o[1][i])));
+        bool bad = !(worst <= 3.4e38f);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) bad |= o[0][i] != o[0][i] || o[1][i] != o[1][i];   // (fmaxf passes over a NaN)
+        bad |= l_run != l_run;
+        if (__syncthreads_or(bad ? 1 : 0)) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) { o[0][i] = 0.f; o[1][i] = 0.f; }
+            m_run = 0.f;
+            l_run = 0.f;
+            started = false;
+            sweep(0);
+        }
+    } else sweep(0);
     // ---- epilogue: O[b][q][h][d], d = 32dt + 8(r >> 2) + 4hi + (r & 3) ----
     const float l_tot = l_run + __shfl_xor(l_run, 32, 64);
     const float inv = started ? 1.0f / l_tot : 0.f;
@@ -285,15 +453,18 @@ extern "C" int aether_relbias_attn(const AetherRelbias* d, void* o, void* o_low,
     p.nqb = (p.S + nw * 32 - 1) / (nw * 32);
     const dim3 grid((unsigned)((long)p.B * p.H * p.nqb));
     hipStream_t s = (hipStream_t)stream;
-#define RB_LAUNCH(NW)                                                                                                \
+#define RB_LAUNCH(NW, PIPE)                                                                                          \
     do {                                                                                                             \
-        if (lse) hipLaunchKernelGGL((relbias_attn_fwd_kernel<NW, true>), grid, dim3(NW * 64), lds, s, args);         \
-        else hipLaunchKernelGGL((relbias_attn_fwd_kernel<NW, false>), grid, dim3(NW * 64), lds, s, args);            \
+        if (lse) hipLaunchKernelGGL((relbias_attn_fwd_kernel<NW, true, PIPE>), grid, dim3(NW * 64), lds, s, args);   \
+        else hipLaunchKernelGGL((relbias_attn_fwd_kernel<NW, false, PIPE>), grid, dim3(NW * 64), lds, s, args);      \
     } while (0)
     switch (nw) {
-        case 4: RB_LAUNCH(4); break;
-        case 2: RB_LAUNCH(2); break;
-        default: RB_LAUNCH(1); break;
+        case 4:
+            if (p.S >= RB_PIPE_TILES * RB_KV) RB_LAUNCH(4, true);
+            else RB_LAUNCH(4, false);
+            break;
+        case 2: RB_LAUNCH(2, false); break;
+        default: RB_LAUNCH(1, false); break;
     }
 #undef RB_LAUNCH
     return aether_check_launch("relbias_attn");

@@ -70,6 +70,18 @@ AE_DEV uint64_t rb_word(const RbArgs& p, const uint64_t* words, int j) {
     return left >= 64 ? ~0ull : (1ull << left) - 1;
 }
 
+// 16-byte LDS-DMA as in common.hpp (LDS destination: wave-uniform base + lane · 16; bytes beyond the descriptor are not fetched), in assembly: the compiler
+// waits for every LDS-DMA it knows of before a transposing LDS read, the next tile's included.  The loops wait for their tiles themselves.
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+AE_DEV i32x4 rb_rsrc(const void* base, unsigned bytes) {
+    const uint64_t a = (uint64_t)base;
+    return i32x4{__builtin_amdgcn_readfirstlane((int)(unsigned)a), __builtin_amdgcn_readfirstlane((int)(unsigned)(a >> 32) & 0xffff), __builtin_amdgcn_readfirstlane((int)bytes), 0x00020000};
+}
+AE_DEV unsigned rb_lds(const void* p) { return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) char*)p; }
+AE_DEV void rb_dma16(i32x4 rsrc, unsigned voff, unsigned soff, unsigned lds_wave_base) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds_wave_base), "v"(voff), "s"(rsrc), "s"(soff) : "memory", "m0");
+}
+
 // A 64 x 64 tile in LDS: 128-byte rows, the 16-byte chunk c of row r stands at c ^ swz(r).  swz takes all eight values over r's bits 1 ... 3, so that 32 rows
 // read at one chunk spread over the banks; and rows r, r + 2 differ in its bit 1, so that the 4 x 32-byte pieces of a transposing read do too.
 AE_DEV int rb_swz(int r) { return (((r >> 1) & 3) << 1) | ((r >> 3) & 1); }
@@ -131,20 +143,21 @@ AE_DEV void rb_store(const f32x16 (&o)[2], float f, bf16_t* row, int hi, bool ok
     }
 }
 
-// The transposed fragments of 32 rows of a tile: f[s][dt] holds column 32 dt + (lane & 31), rows 16 s + 8hi ... + 7.  The transposing LDS read moves a 4 x 16 piece
-// per 16 lanes: lane 4r + c names row r, elements 4c ... 4c + 3, and lane i receives column i.  Before these reads the compiler waits for every LDS-DMA in
-// flight; the loops therefore issue the tile after the next behind them.
-AE_DEV void rb_read_tr(bf16x8 (&f)[2][2], const char* at, const int (&off)[2][2]) {
+// One transposed fragment: 16 rows from `at`, columns by off (rb_tr_offsets of a 32-column half)
+AE_DEV bf16x8 rb_read_tr1(const char* at, const int (&off)[2]) {
     typedef short s16x4 __attribute__((ext_vector_type(4)));
     typedef short s16x8 __attribute__((ext_vector_type(8)));
+    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + off[0]));
+    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + off[1]));
+    return __builtin_bit_cast(bf16x8, s16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]});
+}
+// The transposed fragments of 32 rows of a tile: f[s][dt] holds column 32 dt + (lane & 31), rows 16 s + 8hi ... + 7.  The transposing LDS read moves a 4 x 16 piece
+// per 16 lanes: lane 4r + c names row r, elements 4c ... 4c + 3, and lane i receives column i.
+AE_DEV void rb_read_tr(bf16x8 (&f)[2][2], const char* at, const int (&off)[2][2]) {
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
-        for (int dt = 0; dt < 2; ++dt) {
-            const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + 2048 * s + off[dt][0]));
-            const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + 2048 * s + off[dt][1]));
-            f[s][dt] = __builtin_bit_cast(bf16x8, s16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]});
-        }
+        for (int dt = 0; dt < 2; ++dt) f[s][dt] = rb_read_tr1(at + 2048 * s, off[dt]);
 }
 
 // Three buffers of two tiles: while one is worked on, the next one is complete or arriving, and the one after it is issued.
@@ -165,6 +178,6 @@ inline size_t rb_table_bytes(int reach) { return (size_t)((2 * (reach + RB_PAD) 
 inline size_t rb_words_bytes(const RbArgs& p) { return p.mask ? (size_t)(p.S + 63) / 64 * 8 : 0; }
 int rb_setup(RbArgs& p, const AetherRelbias* d);   // fills the arguments; an error code and its message where the call is refused
 int rb_tensor(RbTensor& t, const void* ptr, const long* strides, int S);
-// waves of a workgroup (32 rows each): four where that still gives every CU a workgroup, else fewer
-inline int rb_waves(const RbArgs& p) { return p.S <= 32 ? 1 : p.S > 64 && (long)p.B * p.H * ((p.S + 127) / 128) >= 256 ? 4 : 2; }
+// waves of a workgroup (32 rows each): four where that still gives every CU a workgroup or the sequence is long enough for the pipelined loop, else fewer
+inline int rb_waves(const RbArgs& p) { return p.S <= 32 ? 1 : p.S >= 448 || (p.S > 64 && (long)p.B * p.H * ((p.S + 127) / 128) >= 256) ? 4 : 2; }
 }  // namespace aether

@@ -87,8 +87,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     const float lse = qrow < S ? args.lse[(size_t)bh * S + qc] : INFINITY;   // rows behind the last one: P = 0, they add nothing to dT
 
     const unsigned k_row = (unsigned)p.k.ss * 2, v_row = (unsigned)p.v.ss * 2;
-    const buf_rsrc_t k_rsrc = make_buf_rsrc(p.k.p + (size_t)b * p.k.sb + (size_t)h * p.k.sh, (unsigned)(S - 1) * k_row + 128);
-    const buf_rsrc_t v_rsrc = make_buf_rsrc(p.v.p + (size_t)b * p.v.sb + (size_t)h * p.v.sh, (unsigned)(S - 1) * v_row + 128);
+    const i32x4 k_rsrc = rb_rsrc(p.k.p + (size_t)b * p.k.sb + (size_t)h * p.k.sh, (unsigned)(S - 1) * k_row + 128);
+    const i32x4 v_rsrc = rb_rsrc(p.v.p + (size_t)b * p.v.sb + (size_t)h * p.v.sh, (unsigned)(S - 1) * v_row + 128);
     unsigned k_off[8 / NW], v_off[8 / NW];
 #pragma unroll
     for (int ps = 0; ps < 8 / NW; ++ps) {
@@ -97,11 +97,11 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
         v_off[ps] = r * v_row + ((ch ^ rb_swz(r)) << 4);
     }
     auto stage = [&](int j, int buf) {
-        char* const dst = smem + buf + wave_s * 1024;
+        const unsigned dst = rb_lds(smem) + buf + wave_s * 1024;
 #pragma unroll
         for (int ps = 0; ps < 8 / NW; ++ps) {
-            bglds16(k_rsrc, k_off[ps], (unsigned)j * (RB_KV * k_row), dst + ps * (NW * 1024));
-            bglds16(v_rsrc, v_off[ps], (unsigned)j * (RB_KV * v_row), dst + RB_TILE + ps * (NW * 1024));
+            rb_dma16(k_rsrc, k_off[ps], (unsigned)j * (RB_KV * k_row), dst + ps * (NW * 1024));
+            rb_dma16(v_rsrc, v_off[ps], (unsigned)j * (RB_KV * v_row), dst + RB_TILE + ps * (NW * 1024));
         }
     };
     int roff[4], toff[2][2];
@@ -143,7 +143,6 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
         f32x16 x[2], dp[2];
 #pragma unroll
         for (int i = 0; i < 16; ++i) { x[0][i] = 0.f; x[1][i] = 0.f; dp[0][i] = 0.f; dp[1][i] = 0.f; }
-        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -151,7 +150,6 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
                 x[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(base + t * 4096 + roff[ks]), qf[ks], x[t], 0, 0, 0);
                 dp[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(base + RB_TILE + t * 4096 + roff[ks]), gf[ks], dp[t], 0, 0, 0);
             }
-        __builtin_amdgcn_s_setprio(0);
         // x[t][r], dp[t][r]: query l32, key 64j + 32t + 16(r >> 3) + 8hi + (r & 7)
         auto half = [&](auto t_tag) {
             constexpr int t = decltype(t_tag)::value;
@@ -211,7 +209,6 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 #pragma unroll
                     for (int dt = 0; dt < 2; ++dt) kf[s][dt] = rb_keep(kf[s][dt], (wt >> (16 * s + 8 * hi)) & 0xffu);
             }
-            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 const bf16x8 df = __builtin_bit_cast(bf16x8, make_uint4(pack_bf16x2(ds[8 * s], ds[8 * s + 1]), pack_bf16x2(ds[8 * s + 2], ds[8 * s + 3]),
@@ -219,7 +216,6 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 #pragma unroll
                 for (int dt = 0; dt < 2; ++dt) dq[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[s][dt], df, dq[dt], 0, 0, 0);
             }
-            __builtin_amdgcn_s_setprio(0);
         };
         half(std::integral_constant<int, 0>{});
         half(std::integral_constant<int, 1>{});
@@ -321,18 +317,18 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 
     if (__syncthreads_or(some ? 1 : 0)) {                             // (and the table is there)
         const unsigned q_row = (unsigned)p.q.ss * 2, g_row = (unsigned)args.go.ss * 2;
-        const buf_rsrc_t q_rsrc = make_buf_rsrc(p.q.p + (size_t)b * p.q.sb + (size_t)h * p.q.sh, (unsigned)(S - 1) * q_row + 128);
-        const buf_rsrc_t g_rsrc = make_buf_rsrc(args.go.p + (size_t)b * args.go.sb + (size_t)h * args.go.sh, (unsigned)(S - 1) * g_row + 128);
+        const i32x4 q_rsrc = rb_rsrc(p.q.p + (size_t)b * p.q.sb + (size_t)h * p.q.sh, (unsigned)(S - 1) * q_row + 128);
+        const i32x4 g_rsrc = rb_rsrc(args.go.p + (size_t)b * args.go.sb + (size_t)h * args.go.sh, (unsigned)(S - 1) * g_row + 128);
         float next_l = 0.f, next_d = 0.f;
         // rows behind the last one repeat it: their P is 0 (L = +inf), and what they are multiplied with has to be a number
         auto stage = [&](int j, int buf) {
-            char* const dst = smem + buf + wave_s * 1024;
+            const unsigned dst = rb_lds(smem) + buf + wave_s * 1024;
 #pragma unroll
             for (int ps = 0; ps < 8 / NW; ++ps) {
                 const int r = (ps * NW + wave) * 8 + (lane >> 3), sw = ((lane & 7) ^ rb_swz(r)) << 4;
                 const unsigned row = min(j * RB_KV + r, S - 1);
-                bglds16(q_rsrc, row * q_row + sw, 0u, dst + ps * (NW * 1024));
-                bglds16(g_rsrc, row * g_row + sw, 0u, dst + RB_TILE + ps * (NW * 1024));
+                rb_dma16(q_rsrc, row * q_row + sw, 0u, dst + ps * (NW * 1024));
+                rb_dma16(g_rsrc, row * g_row + sw, 0u, dst + RB_TILE + ps * (NW * 1024));
             }
             if (tid < RB_KV) {
                 const int row = j * RB_KV + tid;
@@ -372,13 +368,11 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
                     f32x16 x, dp;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) { x[i] = 0.f; dp[i] = 0.f; }
-                    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
                     for (int ks = 0; ks < 4; ++ks) {
                         x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(base + t * 4096 + roff[ks]), kf[ks], x, 0, 0, 0);
                         dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(base + RB_TILE + t * 4096 + roff[ks]), vf[ks], dp, 0, 0, 0);
                     }
-                    __builtin_amdgcn_s_setprio(0);
                     const float* lp = rows + buf / RB_BUF * 128 + 32 * t + 8 * hi;
                     const float* tb = tab + (key - (j * RB_KV + 32 * t + 8 * hi) - 23 + p.reach + RB_PAD);   // of the last of the 16 queries
                     unsigned pf[2][4], df[2][4];
@@ -404,7 +398,6 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
                     bf16x8 qt[2][2], gt[2][2];
                     rb_read_tr(gt, base + RB_TILE + t * 4096, toff);
                     rb_read_tr(qt, base + t * 4096, toff);
-                    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
                     for (int s = 0; s < 2; ++s) {
                         const bf16x8 pv = __builtin_bit_cast(bf16x8, make_uint4(pf[s][0], pf[s][1], pf[s][2], pf[s][3]));
@@ -415,7 +408,6 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
                             dk[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qt[s][dt], dv_, dk[dt], 0, 0, 0);
                         }
                     }
-                    __builtin_amdgcn_s_setprio(0);
                 };
                 if (right || left) {
                     half(std::integral_constant<int, 0>{}, std::true_type{});
