@@ -43,9 +43,6 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(PIPE ? 
     const int q0 = qb * (NW * 32) + wave_s * 32;                      // this wave's first query
     const int qrow = q0 + l32;
 
-    rb_fill_table(p, h, tab, NW * 64);
-    if (p.mask) rb_fill_words(p.mask + (size_t)b * p.mask_sb, S, words8, NW * 64);
-
     bf16x8 qf[4];
     {
         const bf16_t* qp = p.q.p + (size_t)b * p.q.sb + (size_t)h * p.q.sh + (size_t)min(qrow, S - 1) * p.q.ss;
@@ -77,6 +74,11 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(PIPE ? 
         stage_k(j, buf);
         stage_v(j, buf);
     };
+    const int nkv = (S + RB_KV - 1) / RB_KV;
+    stage(0, 0);                                                      // on their way while the table and the mask are read; whether their keys count shows later
+    if (nkv > 1) stage(1, RB_BUF);
+    rb_fill_table(p, h, tab, NW * 64);
+    if (p.mask) rb_fill_words(p.mask + (size_t)b * p.mask_sb, S, words8, NW * 64);
     int koff[4], voff[2][2];
     rb_row_offsets(lane, koff);
     rb_tr_offsets(lane, voff);
@@ -88,22 +90,23 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(PIPE ? 
     bool started = false;
 
     rb_arrived(qf);
-    __syncthreads();                                                  // table and words are there
+    drain_and_barrier();                                              // table and words are there, and the first two tiles
     const float far_r = tab[2 * (p.reach + RB_PAD)], far_l = tab[0];
-    const int nkv = (S + RB_KV - 1) / RB_KV;
     auto next_tile = [&](int j, uint64_t& w) {                        // the next tile from j on that holds a key, nkv if none does
         for (; j < nkv; ++j)
             if ((w = rb_word(p, words, j)) != 0) break;
         return j;
     };
-    // Tile by tile from `first` on, any tile: the tiles in front of it are done.
-    auto sweep = [&](int first) {
+    // Tile by tile from `first` on, any tile: the tiles in front of it are done.  fresh: tiles 0 and 1 are in the first two buffers.
+    auto sweep = [&](int first, bool fresh) {
         uint64_t w = 0, w1 = 0, w2 = 0;
         int j = next_tile(first, w), j1 = next_tile(j + 1, w1);
         int buf = 0;
-        if (j < nkv) stage(j, 0);
-        if (j1 < nkv) stage(j1, RB_BUF);
-        drain_and_barrier();
+        if (!fresh || j != 0 || j1 != 1) {                            // not the tiles that were staged at the start
+            if (j < nkv) stage(j, 0);
+            if (j1 < nkv) stage(j1, RB_BUF);
+            drain_and_barrier();
+        }
         while (j < nkv) {
             const char* base = smem + buf;
             const int j2 = next_tile(j1 + 1, w2);
@@ -226,12 +229,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(PIPE ? 
     auto pipeline = [&](int n) {
         constexpr int KO = 0, VO = RB_TILE;
         int kb = 0, kb1 = RB_BUF, kb2 = 2 * RB_BUF;                   // buffers of K(j), K(j + 1), K(j + 2); V(j) is in the same as K(j)
-        stage_k(0, kb);
-        stage_v(0, kb);
-        stage_k(1, kb1);
-        drain_and_barrier();
-        if (n > 2) stage_k(2, kb2);
-        stage_v(1, kb1);
+        if (n > 2) stage_k(2, kb2);                                   // tiles 0 and 1 are there
         f32x16 x0, x1;
         bf16x8 ka[4], kc[4], va[2][2], vc[2][2];                      // fragments for the first and the second half of an iteration
         unsigned p0[2][4], p1[2][4], l0[2][4], l1[2][4];
@@ -358,7 +356,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(PIPE ? 
     }
     if (PIPE && whole >= RB_PIPE_TILES) {
         pipeline(whole);
-        if (whole < nkv) sweep(whole);
+        if (whole < nkv) sweep(whole, false);
         float worst = fabsf(l_run);
 #pragma unroll
         for (int i = 0; i < 16; ++i) worst = fmaxf(worst, fmaxf(fabsf(o[0][i]), fabsf(o[1][i])));
@@ -372,9 +370,9 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(PIPE ? 
             m_run = 0.f;
             l_run = 0.f;
             started = false;
-            sweep(0);
+            sweep(0, false);
         }
-    } else sweep(0);
+    } else sweep(0, true);
     // ---- epilogue: O[b][q][h][d], d = 32dt + 8(r >> 2) + 4hi + (r & 3) ----
     const float l_tot = l_run + __shfl_xor(l_run, 32, 64);
     const float inv = started ? 1.0f / l_tot : 0.f;

@@ -34,27 +34,34 @@ struct RbArgs {
 // reach read past it without a clamp.
 AE_DEV void rb_fill_table(const RbArgs& p, int h, float* tab, int nthreads) {
     const int n_tab = 2 * (p.reach + RB_PAD) + 1;
-    for (int i = threadIdx.x; i < n_tab; i += nthreads) {
-        const int d = i - p.reach - RB_PAD, n = d < 0 ? -d : d;
-        int b = n;
-        if (n >= p.near_n) {
-            b = p.near_n;
-            for (int j = 0; j < p.n_border; ++j) b += p.border[j] <= n;
+    for (int i0 = threadIdx.x; i0 < n_tab; i0 += 2 * nthreads) {          // two entries at a time: their loads travel together
+        bf16_t v[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int d = min(i0 + k * nthreads, n_tab - 1) - p.reach - RB_PAD, n = d < 0 ? -d : d;
+            int b = n;
+            if (n >= p.near_n) {
+                b = p.near_n;
+                for (int j = 0; j < p.n_border; ++j) b += p.border[j] <= n;
+            }
+            b += d > 0 ? p.half : 0;
+            v[k] = p.table[(size_t)b * p.H + h];
         }
-        b += d > 0 ? p.half : 0;
-        tab[i] = (float)p.table[(size_t)b * p.H + h] * RB_LOG2E;
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            if (i0 + k * nthreads < n_tab) tab[i0 + k * nthreads] = (float)v[k] * RB_LOG2E;
     }
 }
 
 // One bit per key, 64 keys a word.  A lane reads eight mask bytes and writes their bits as one byte.
 AE_DEV void rb_fill_words(const unsigned char* mask, int S, unsigned char* words, int nthreads) {
     for (int i = threadIdx.x; i < (S + 63) / 64 * 8; i += nthreads) {
+        unsigned char m[8];                                               // all eight loads before the first is looked at
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m[e] = mask[min(i * 8 + e, S - 1)];
         unsigned bits = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int key = i * 8 + e;
-            bits |= (key < S && mask[min(key, S - 1)] != 0 ? 1u : 0u) << e;
-        }
+        for (int e = 0; e < 8; ++e) bits |= (m[e] != 0 && i * 8 + e < S ? 1u : 0u) << e;
         words[i] = (unsigned char)bits;
     }
 }

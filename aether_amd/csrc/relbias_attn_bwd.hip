@@ -54,10 +54,6 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     const int q0 = qb * (NW * 32) + wave_s * 32;
     const int qrow = q0 + l32, qc = min(qrow, S - 1);
 
-    rb_fill_table(p, h, tab, NW * 64);
-    if (p.mask) rb_fill_words(p.mask + (size_t)b * p.mask_sb, S, words8, NW * 64);
-    if (args.part)
-        for (int i = tid; i < tab_bytes / 4 * 2 * NW; i += NW * 64) hist[i] = 0.f;
     float* const my_hist = hist + (wave * 2 + hi) * (tab_bytes / 4);
 
     bf16x8 qf[4], gf[4];
@@ -104,6 +100,13 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
             rb_dma16(v_rsrc, v_off[ps], (unsigned)j * (RB_KV * v_row), dst + RB_TILE + ps * (NW * 1024));
         }
     };
+    const int nkv = (S + RB_KV - 1) / RB_KV;
+    stage(0, 0);                                                      // on their way while the table and the mask are read; whether their keys count shows later
+    if (nkv > 1) stage(1, RB_BUF);
+    rb_fill_table(p, h, tab, NW * 64);
+    if (p.mask) rb_fill_words(p.mask + (size_t)b * p.mask_sb, S, words8, NW * 64);
+    if (args.part)
+        for (int i = tid; i < tab_bytes / 4 * 2 * NW; i += NW * 64) hist[i] = 0.f;
     int roff[4], toff[2][2];
     rb_row_offsets(lane, roff);
     rb_tr_offsets(lane, toff);
@@ -120,9 +123,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
         if (at < n_tab) my_hist[at] = v;                              // (beyond it there are only zeros: no pair of the wave is that far apart)
     };
 
-    __syncthreads();
+    drain_and_barrier();                                              // table, words and tables of distances are there, and the first two tiles
     const float far_r = tab[2 * (p.reach + RB_PAD)], far_l = tab[0];
-    const int nkv = (S + RB_KV - 1) / RB_KV;
     auto next_tile = [&](int j, uint64_t& w) {
         for (; j < nkv; ++j)
             if ((w = rb_word(p, words, j)) != 0) break;
@@ -131,9 +133,11 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     uint64_t w = 0, w1 = 0, w2 = 0;
     int j = next_tile(0, w), j1 = next_tile(j + 1, w1);
     int buf = 0;
-    if (j < nkv) stage(j, 0);
-    if (j1 < nkv) stage(j1, RB_BUF);
-    drain_and_barrier();
+    if (j != 0 || j1 != 1) {                                          // not the tiles that were staged at the start
+        if (j < nkv) stage(j, 0);
+        if (j1 < nkv) stage(j1, RB_BUF);
+        drain_and_barrier();
+    }
     while (j < nkv) {
         const int j2 = next_tile(j1 + 1, w2);
         const char* base = smem + buf;
@@ -299,7 +303,6 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     bf16_t* const dkp = const_cast<bf16_t*>(args.dk.p) + (size_t)b * args.dk.sb + (size_t)h * args.dk.sh + (size_t)kc * args.dk.ss;
     bf16_t* const dvp = const_cast<bf16_t*>(args.dv.p) + (size_t)b * args.dv.sb + (size_t)h * args.dv.sh + (size_t)kc * args.dv.ss;
 
-    rb_fill_table(p, h, tab, NW * 64);
     bf16x8 kf[4], vf[4];
     {
         const bf16_t* kp = p.k.p + (size_t)b * p.k.sb + (size_t)h * p.k.sh + (size_t)kc * p.k.ss;
@@ -315,7 +318,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 #pragma unroll
     for (int i = 0; i < 16; ++i) { dk[0][i] = 0.f; dk[1][i] = 0.f; dv[0][i] = 0.f; dv[1][i] = 0.f; }
 
-    if (__syncthreads_or(some ? 1 : 0)) {                             // (and the table is there)
+    if (__syncthreads_or(some ? 1 : 0)) {
         const unsigned q_row = (unsigned)p.q.ss * 2, g_row = (unsigned)args.go.ss * 2;
         const i32x4 q_rsrc = rb_rsrc(p.q.p + (size_t)b * p.q.sb + (size_t)h * p.q.sh, (unsigned)(S - 1) * q_row + 128);
         const i32x4 g_rsrc = rb_rsrc(args.go.p + (size_t)b * args.go.sb + (size_t)h * args.go.sh, (unsigned)(S - 1) * g_row + 128);
@@ -343,17 +346,22 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
                 to[64] = next_d;
             }
         };
+        const int nq = (S + RB_KV - 1) / RB_KV;
+        stage(0, 0);
+        const float first_l = next_l, first_d = next_d;
+        if (nq > 1) stage(1, RB_BUF);
+        rb_fill_table(p, h, tab, NW * 64);
+        if (tid < RB_KV) {
+            rows[tid] = first_l;
+            rows[64 + tid] = first_d;
+        }
         rb_arrived(kf);
         rb_arrived(vf);
         int roff[4], toff[2][2];
         rb_row_offsets(lane, roff);
         rb_tr_offsets(lane, toff);
-        const float far_r = tab[2 * (p.reach + RB_PAD)], far_l = tab[0];
-        const int nq = (S + RB_KV - 1) / RB_KV;
-        stage(0, 0);
-        put_rows(0);
-        if (nq > 1) stage(1, RB_BUF);
         drain_and_barrier();
+        const float far_r = tab[2 * (p.reach + RB_PAD)], far_l = tab[0];
         int buf = 0;
         for (int j = 0; j < nq; ++j) {
             if (some) {
