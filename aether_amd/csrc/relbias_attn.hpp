@@ -85,9 +85,12 @@ AE_DEV i32x4 rb_rsrc(const void* base, unsigned bytes) {
     return i32x4{__builtin_amdgcn_readfirstlane((int)(unsigned)a), __builtin_amdgcn_readfirstlane((int)(unsigned)(a >> 32) & 0xffff), __builtin_amdgcn_readfirstlane((int)bytes), 0x00020000};
 }
 AE_DEV unsigned rb_lds(const void* p) { return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) char*)p; }
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"       // (that m0 is not preserved is what is meant)
 AE_DEV void rb_dma16(i32x4 rsrc, unsigned voff, unsigned soff, unsigned lds_wave_base) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds_wave_base), "v"(voff), "s"(rsrc), "s"(soff) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 
 // A 64 x 64 tile in LDS: 128-byte rows, the 16-byte chunk c of row r stands at c ^ swz(r).  swz takes all eight values over r's bits 1 ... 3, so that 32 rows
 // read at one chunk spread over the banks; and rows r, r + 2 differ in its bit 1, so that the 4 x 32-byte pieces of a transposing read do too.

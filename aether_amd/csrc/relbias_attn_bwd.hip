@@ -8,8 +8,7 @@
 // (7 products instead of 5), and every sum has an order that depends on the sizes alone.  A lane holds 16 scores of ONE query (first sweep) or of
 // ONE key (second) at a time, and dS / P leave the registers as the B operand of the next product; the transposed A operands come out of
 // row-major tiles by ds_read_b64_tr_b16.
-// δ is a product with O on the matrix pipe like dP is one with v, in the same order of sums: a row that has one key has O = v, so that its dP − δ is 0, not the
-// difference of two roundings.
+// Where one key alone counts, P is 1 whatever its score and dS is 0: those gradients are set to 0 instead of the difference of two roundings of one number.
 // dT: beyond `reach` a tile's dS go into one number per lane.  Near the diagonal dS is summed along its diagonals in registers: the 16 values of a lane are
 // rotated over the 32 queries by their key's place (ds_swizzle, a constant each), which brings a diagonal into one lane; what wraps around joins the next
 // 32 keys' diagonals, so that every entry of a wave's table of distances is stored once, by plain stores.  (LDS float atomics in their place: 200 cycles an
@@ -92,7 +91,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
         k_off[ps] = r * k_row + ((ch ^ rb_swz(r)) << 4);
         v_off[ps] = r * v_row + ((ch ^ rb_swz(r)) << 4);
     }
-    auto stage = [&](int j, int buf) {
+    auto stage = [&](int j, int buf) __attribute__((always_inline)) {
         const unsigned dst = rb_lds(smem) + buf + wave_s * 1024;
 #pragma unroll
         for (int ps = 0; ps < 8 / NW; ++ps) {
@@ -113,10 +112,10 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 
     rb_arrived(qf);
     rb_arrived(gf);
-    f32x16 dq[2];
+    f32x16 dq[2], minus_delta;                                        // dP starts from −δ
 #pragma unroll
-    for (int i = 0; i < 16; ++i) { dq[0][i] = 0.f; dq[1][i] = 0.f; }
-    float sum_r = 0.f, sum_l = 0.f;                                   // dS beyond the reach, on either side
+    for (int i = 0; i < 16; ++i) { dq[0][i] = 0.f; dq[1][i] = 0.f; minus_delta[i] = -delta; }
+    float sum_r = 0.f, sum_l = 0.f, far_sum = 0.f;                    // dS beyond the reach, on either side
     float carry = 0.f;                                                // diagonals that go on into the keys from carry_at on (wave-uniform; < 0: none)
     int carry_at = -1;
     auto put = [&](int at, float v) {
@@ -125,6 +124,12 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 
     drain_and_barrier();                                              // table, words and tables of distances are there, and the first two tiles
     const float far_r = tab[2 * (p.reach + RB_PAD)], far_l = tab[0];
+    bool lone = S == 1;
+    if (p.mask) {
+        int n = 0;
+        for (int i = lane; i < nkv; i += 64) n += __popcll(words[i]);
+        lone = wave_sum((float)n) == 1.f;
+    }
     auto next_tile = [&](int j, uint64_t& w) {
         for (; j < nkv; ++j)
             if ((w = rb_word(p, words, j)) != 0) break;
@@ -138,97 +143,125 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
         if (j1 < nkv) stage(j1, RB_BUF);
         drain_and_barrier();
     }
-    while (j < nkv) {
-        const int j2 = next_tile(j1 + 1, w2);
-        const char* base = smem + buf;
-        const bool part = w != ~0ull;
-        const int d_lo = j * RB_KV - (q0 + 31), d_hi = j * RB_KV + 63 - q0;
-        const bool right = d_lo >= p.reach, left = d_hi <= -p.reach;
-        f32x16 x[2], dp[2];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) { x[0][i] = 0.f; x[1][i] = 0.f; dp[0][i] = 0.f; dp[1][i] = 0.f; }
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int ks = 0; ks < 4; ++ks) {
-                x[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(base + t * 4096 + roff[ks]), qf[ks], x[t], 0, 0, 0);
-                dp[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(base + RB_TILE + t * 4096 + roff[ks]), gf[ks], dp[t], 0, 0, 0);
+    // dS of one half, near the diagonal: summed along its diagonals
+    auto diagonals = [&](const f32x16& ds, int k_at) __attribute__((always_inline)) {
+        // element (query l32, key k_at + kr + 8hi), kr = 16(r >> 3) + (r & 7): rotated by kr it is in lane i = l32 - kr of its half (of 32 lanes), distance
+        // k_at + 8hi - q0 - i; or, wrapped, in lane i = l32 - kr + 32, distance 32 more
+        float whole = 0.f, wrap = 0.f;
+        rb_static_for<16>([&](auto r_tag) __attribute__((always_inline)) {
+            constexpr int r = decltype(r_tag)::value, kr = 16 * (r >> 3) + (r & 7);
+            const float y = kr ? __int_as_float(__builtin_amdgcn_ds_swizzle(__float_as_int(ds[r]), 0xc000 | (kr << 5))) : ds[r];
+            const float z = l32 > 31 - kr ? y : 0.f;
+            wrap += z;
+            whole += y - z;
+        });
+        if (k_at != carry_at) {                                       // the diagonals carried here do not continue where this begins
+            if (carry_at >= 0) put(carry_at + 8 * hi - q0 - l32 + p.reach + RB_PAD, carry);
+            carry = 0.f;
+        }
+        put(k_at + 8 * hi - q0 - l32 + p.reach + RB_PAD, whole + carry);
+        carry = wrap;
+        carry_at = k_at + 32;
+    };
+    // One tile.  VALU issued between a wave's own matrix instructions runs behind them: the first half's dS is spread over the second half's scores and dP, the
+    // second half's over the first half's products.
+    auto tile = [&](float add, auto near_tag, auto part_tag) __attribute__((always_inline)) {
+        constexpr bool NEAR = decltype(near_tag)::value, PART = decltype(part_tag)::value;
+        const char* const base = smem + buf;
+        // the A fragment of matrix instruction i of 24: scores and dP of the first half, of the second half, products of the first, of the second
+        auto fragment = [&](auto i_tag) __attribute__((always_inline)) -> bf16x8 {
+            constexpr int i = decltype(i_tag)::value;
+            if constexpr (i < 16) return *(const bf16x8*)(base + (i & 1) * RB_TILE + (i >> 3) * 4096 + roff[(i >> 1) & 3]);
+            else if constexpr (PART)
+                return rb_keep(rb_read_tr1(base + ((i >> 2) & 1) * 4096 + 2048 * ((i >> 1) & 1), toff[i & 1]), (unsigned)(w >> (32 * ((i >> 2) & 1) + 16 * ((i >> 1) & 1) + 8 * hi)) & 0xffu);
+            else return rb_read_tr1(base + ((i >> 2) & 1) * 4096 + 2048 * ((i >> 1) & 1), toff[i & 1]);
+        };
+        f32x16 x[2], dp[2];                                           // x[t][r], dp[t][r]: query l32, key 64j + 32t + 16(r >> 3) + 8hi + (r & 7)
+        unsigned df[2][2][4];
+        const float* const tb = tab + (j * RB_KV + 8 * hi - qrow + p.reach + RB_PAD);
+        const unsigned keep0 = (unsigned)w >> (8 * hi), keep1 = (unsigned)(w >> 32) >> (8 * hi);
+        auto weigh = [&](auto e_tag, auto t_tag) __attribute__((always_inline)) {                    // elements 2e, 2e + 1
+            constexpr int e = decltype(e_tag)::value, t = decltype(t_tag)::value, at = 16 * (e >> 2) + 2 * (e & 3);
+            float d0 = __builtin_amdgcn_exp2f(fmaf(x[t][2 * e], p.c, NEAR ? tb[32 * t + at] + add : add)) * dp[t][2 * e];
+            float d1 = __builtin_amdgcn_exp2f(fmaf(x[t][2 * e + 1], p.c, NEAR ? tb[32 * t + at + 1] + add : add)) * dp[t][2 * e + 1];
+            if constexpr (PART) {
+                d0 = ((t ? keep1 : keep0) >> at) & 1 ? d0 : 0.f;
+                d1 = ((t ? keep1 : keep0) >> (at + 1)) & 1 ? d1 : 0.f;
             }
-        // x[t][r], dp[t][r]: query l32, key 64j + 32t + 16(r >> 3) + 8hi + (r & 7)
-        auto half = [&](auto t_tag) {
-            constexpr int t = decltype(t_tag)::value;
-            const unsigned wt = (unsigned)(w >> (32 * t));
-            if (part && wt == 0) return;                              // (wave-uniform) no key in this half
-            const int k_at = j * RB_KV + 32 * t;
-            const int d0 = k_at + 8 * hi - qrow + p.reach + RB_PAD;   // the distance of r = 0, as an index of tab
-            f32x16& ds = x[t];
-            if (right || left) {
-                const float add = (right ? far_r : far_l) - lse;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) ds[r] = fmaf(ds[r], p.c, add);
-            } else {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) ds[r] = fmaf(ds[r], p.c, tab[d0 + 16 * (r >> 3) + (r & 7)] - lse);
-            }
-#pragma unroll
-            for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(ds[r]) * (dp[t][r] - delta);
-            if (__builtin_expect(part, 0)) {
-                const unsigned mine = wt >> (8 * hi);
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (!((mine >> (16 * (r >> 3) + (r & 7))) & 1)) ds[r] = 0.f;
-            }
-            if (args.part) {
-                if (right || left) {
-                    float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-                    for (int r = 0; r < 16; r += 2) { s0 += ds[r]; s1 += ds[r + 1]; }
-                    if (right) sum_r += s0 + s1;
-                    else sum_l += s0 + s1;
-                } else {
-                    // element (query l32, key k_at + kr + 8hi), kr = 16(r >> 3) + (r & 7): rotated by kr it is in lane i = l32 - kr of its half (of 32
-                    // lanes), distance k_at + 8hi - q0 - i; or, wrapped, in lane i = l32 - kr + 32, distance 32 more
-                    float whole = 0.f, wrap = 0.f;
-                    rb_static_for<16>([&](auto r_tag) {
-                        constexpr int r = decltype(r_tag)::value, kr = 16 * (r >> 3) + (r & 7);
-                        const float y = kr ? __int_as_float(__builtin_amdgcn_ds_swizzle(__float_as_int(ds[r]), 0xc000 | (kr << 5))) : ds[r];
-                        const float z = l32 > 31 - kr ? y : 0.f;
-                        wrap += z;
-                        whole += y - z;
-                    });
-                    if (k_at != carry_at) {                           // the diagonals carried here do not continue where this begins
-                        if (carry_at >= 0) put(carry_at + 8 * hi - q0 - l32 + p.reach + RB_PAD, carry);
-                        carry = 0.f;
-                    }
-                    put(d0 + qrow - q0 - l32, whole + carry);
-                    carry = wrap;
-                    carry_at = k_at + 32;
-                }
-            }
-            bf16x8 kf[2][2];
-            rb_read_tr(kf, base + t * 4096, toff);
-            if (__builtin_expect(part, 0)) {
-#pragma unroll
-                for (int s = 0; s < 2; ++s)
-#pragma unroll
-                    for (int dt = 0; dt < 2; ++dt) kf[s][dt] = rb_keep(kf[s][dt], (wt >> (16 * s + 8 * hi)) & 0xffu);
-            }
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const bf16x8 df = __builtin_bit_cast(bf16x8, make_uint4(pack_bf16x2(ds[8 * s], ds[8 * s + 1]), pack_bf16x2(ds[8 * s + 2], ds[8 * s + 3]),
-                                                                        pack_bf16x2(ds[8 * s + 4], ds[8 * s + 5]), pack_bf16x2(ds[8 * s + 6], ds[8 * s + 7])));
-#pragma unroll
-                for (int dt = 0; dt < 2; ++dt) dq[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[s][dt], df, dq[dt], 0, 0, 0);
+            x[t][2 * e] = d0;
+            x[t][2 * e + 1] = d1;
+            const unsigned pk = pack_bf16x2(d0, d1);
+            df[t][e >> 2][e & 3] = pk;
+            if constexpr (!NEAR) {                                    // a far bucket's share, from the rounded values: one instruction a pair
+                bf16x2 ones;
+                ones[0] = (__bf16)1.0f; ones[1] = (__bf16)1.0f;
+                far_sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pk), ones, far_sum, false);
             }
         };
-        half(std::integral_constant<int, 0>{});
-        half(std::integral_constant<int, 1>{});
+        constexpr int AHEAD = 3;                                      // fragments are read this many instructions before they are used
+        bf16x8 f[AHEAD + 1];
+        rb_static_for<AHEAD>([&](auto i_tag) { f[decltype(i_tag)::value] = fragment(i_tag); });
+        rb_static_for<24>([&](auto i_tag) __attribute__((always_inline)) {
+            constexpr int i = decltype(i_tag)::value, t = (i >> 3) & 1, ks = (i >> 1) & 3;
+            if constexpr (i + AHEAD < 24) f[(i + AHEAD) % (AHEAD + 1)] = fragment(std::integral_constant<int, i + AHEAD>{});
+            const bf16x8& a = f[i % (AHEAD + 1)];
+            if constexpr (i < 16 && (i & 1) == 0) {
+                if constexpr (ks == 0) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) x[t][r] = 0.f;
+                }
+                x[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, qf[ks], x[t], 0, 0, 0);
+            } else if constexpr (i < 16) {
+                dp[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, gf[ks], ks == 0 ? minus_delta : dp[t], 0, 0, 0);
+            } else {
+                constexpr int ht = (i >> 2) & 1, s = (i >> 1) & 1, dt = i & 1;
+                dq[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, __builtin_bit_cast(bf16x8, make_uint4(df[ht][s][0], df[ht][s][1], df[ht][s][2], df[ht][s][3])), dq[dt], 0, 0, 0);
+            }
+            if constexpr (i >= 8 && i < 16) weigh(std::integral_constant<int, i - 8>{}, std::integral_constant<int, 0>{});
+            if constexpr (i >= 16 && i < 20) {
+                weigh(std::integral_constant<int, 2 * (i - 16)>{}, std::integral_constant<int, 1>{});
+                weigh(std::integral_constant<int, 2 * (i - 16) + 1>{}, std::integral_constant<int, 1>{});
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        if constexpr (NEAR) {
+            if (args.part) {
+                diagonals(x[0], j * RB_KV);
+                diagonals(x[1], j * RB_KV + 32);
+            }
+        }
+    };
+    auto advance = [&]() __attribute__((always_inline)) {
+        const int j2 = next_tile(j1 + 1, w2);
         rb_tiles_landed();                                            // tile j1, issued one tile ago
         if (j2 < nkv) stage(j2, rb_next(rb_next(buf)));               // its buffer was last read before the previous barrier
         rb_reads_done_barrier();
         j = j1; w = w1;
         j1 = j2; w1 = w2;
         buf = rb_next(buf);
+    };
+    // three loops: keys left of the wave's queries, around them, right of them.  The workgroup's waves change over at different tiles; every iteration has the
+    // same one barrier.
+    const int near_from = q0 - p.reach - 63 >= 0 ? (q0 - p.reach - 63) / RB_KV + 1 : 0;   // the first tile with 64j + 63 - q0 > -reach
+    const int near_to = (q0 + 31 + p.reach + RB_KV - 1) / RB_KV;                          // the first with 64j - q0 - 31 >= reach
+    auto far = [&](float add) __attribute__((always_inline)) {
+        if (__builtin_expect(w != ~0ull, 0)) tile(add, std::false_type{}, std::true_type{});
+        else tile(add, std::false_type{}, std::false_type{});
+        advance();
+    };
+    while (j < min(near_from, nkv)) far(far_l - lse);
+    sum_l = far_sum;
+    far_sum = 0.f;
+    while (j < min(near_to, nkv)) {
+        if (__builtin_expect(w != ~0ull, 0)) tile(-lse, std::true_type{}, std::true_type{});
+        else tile(-lse, std::true_type{}, std::false_type{});
+        advance();
+    }
+    while (j < nkv) far(far_r - lse);
+    sum_r = far_sum;
+    if (lone) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) { dq[0][i] = 0.f; dq[1][i] = 0.f; }
     }
     rb_store(dq, args.scale, const_cast<bf16_t*>(args.dq.p) + (size_t)b * args.dq.sb + (size_t)h * args.dq.sh + (size_t)qc * args.dq.ss, hi, qrow < S);
 
@@ -261,7 +294,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
         s += __shfl_xor(s, 1, 64);
         s += __shfl_xor(s, 2, 64);
         s += __shfl_xor(s, 4, 64);
-        if (sub == 0) out[bk] = s;
+        if (sub == 0) out[bk] = lone ? 0.f : s;
     }
 }
 
@@ -288,7 +321,7 @@ template <int NW>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void relbias_attn_dkv_kernel(RbBwdArgs args) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const RbArgs& p = args.a;
-    float* const rows = (float*)(smem + RB_RING);                  // [buffer of three][L | δ][64]
+    float* const rows = (float*)(smem + RB_RING);                  // [buffer of three][−L / c | −δ][64]
     float* const tab = (float*)(smem + RB_RING + 1536);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5, l32 = lane & 31;
     const int wave_s = __builtin_amdgcn_readfirstlane(wave);
@@ -300,6 +333,9 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     const int key = k0 + l32, kc = min(key, S - 1);
     const bool counts = key < S && (p.mask == nullptr || p.mask[(size_t)b * p.mask_sb + kc] != 0);
     const bool some = __any(counts) != 0;                             // of this wave; the others keep it company at the barriers
+    int mine = 0;                                                     // keys of the batch item that count, as far as this thread looked
+    if (p.mask)
+        for (int i = tid; i < S; i += NW * 64) mine += p.mask[(size_t)b * p.mask_sb + i] != 0;
     bf16_t* const dkp = const_cast<bf16_t*>(args.dk.p) + (size_t)b * args.dk.sb + (size_t)h * args.dk.sh + (size_t)kc * args.dk.ss;
     bf16_t* const dvp = const_cast<bf16_t*>(args.dv.p) + (size_t)b * args.dv.sb + (size_t)h * args.dv.sh + (size_t)kc * args.dv.ss;
 
@@ -310,21 +346,24 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
         const bf16x8 zero = {};
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {                              // what stands at a key that does not count is not looked at
-            kf[ks] = counts ? *(const bf16x8*)(kp + 16 * ks + 8 * hi) : zero;
+            kf[ks] = counts && p.c != 0.f ? *(const bf16x8*)(kp + 16 * ks + 8 * hi) : zero;
             vf[ks] = counts ? *(const bf16x8*)(vp + 16 * ks + 8 * hi) : zero;
         }
     }
+    // a scale of 0 is a scale of 1 on keys of 0
+    const float c = p.c != 0.f ? p.c : 1.f, inv_c = 1.f / c;
     f32x16 dk[2], dv[2];
 #pragma unroll
     for (int i = 0; i < 16; ++i) { dk[0][i] = 0.f; dk[1][i] = 0.f; dv[0][i] = 0.f; dv[1][i] = 0.f; }
 
+    const bool lone = p.mask ? __syncthreads_count(mine != 0) == 1 && !__syncthreads_or(mine > 1) : S == 1;
     if (__syncthreads_or(some ? 1 : 0)) {
         const unsigned q_row = (unsigned)p.q.ss * 2, g_row = (unsigned)args.go.ss * 2;
         const i32x4 q_rsrc = rb_rsrc(p.q.p + (size_t)b * p.q.sb + (size_t)h * p.q.sh, (unsigned)(S - 1) * q_row + 128);
         const i32x4 g_rsrc = rb_rsrc(args.go.p + (size_t)b * args.go.sb + (size_t)h * args.go.sh, (unsigned)(S - 1) * g_row + 128);
         float next_l = 0.f, next_d = 0.f;
         // rows behind the last one repeat it: their P is 0 (L = +inf), and what they are multiplied with has to be a number
-        auto stage = [&](int j, int buf) {
+        auto stage = [&](int j, int buf) __attribute__((always_inline)) {
             const unsigned dst = rb_lds(smem) + buf + wave_s * 1024;
 #pragma unroll
             for (int ps = 0; ps < 8 / NW; ++ps) {
@@ -342,8 +381,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
         auto put_rows = [&](int buf) {
             if (tid < RB_KV) {
                 float* const to = rows + buf / RB_BUF * 128 + tid;
-                to[0] = next_l;
-                to[64] = next_d;
+                to[0] = next_l * -inv_c;
+                to[64] = -next_d;
             }
         };
         const int nq = (S + RB_KV - 1) / RB_KV;
@@ -352,8 +391,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
         if (nq > 1) stage(1, RB_BUF);
         rb_fill_table(p, h, tab, NW * 64);
         if (tid < RB_KV) {
-            rows[tid] = first_l;
-            rows[64 + tid] = first_d;
+            rows[tid] = first_l * -inv_c;
+            rows[64 + tid] = -first_d;
         }
         rb_arrived(kf);
         rb_arrived(vf);
@@ -362,81 +401,104 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
         rb_tr_offsets(lane, toff);
         drain_and_barrier();
         const float far_r = tab[2 * (p.reach + RB_PAD)], far_l = tab[0];
+        // One tile of 64 queries.  The scores start from −L / c, so that one fma with the bias gives the exponent, and dP from −δ.  VALU issued between a wave's own matrix
+        // instructions runs behind them: the first half's P and dS are spread over the second half's scores and dP, the second half's over the first half's
+        // products.
+        const float off = counts ? 0.f : -INFINITY;
         int buf = 0;
-        for (int j = 0; j < nq; ++j) {
-            if (some) {
-                const char* base = smem + buf;
-                const int d_lo = k0 - (j * RB_KV + 63), d_hi = k0 + 31 - j * RB_KV;
-                const bool right = d_lo >= p.reach, left = d_hi <= -p.reach;
-                const float far = right ? far_r : far_l;
-                auto half = [&](auto t_tag, auto far_tag) {
-                    constexpr int t = decltype(t_tag)::value;
-                    constexpr bool FAR = decltype(far_tag)::value;
-                    // x[r], dp[r]: key l32, query 64j + 32t + 16(r >> 3) + 8hi + (r & 7)
-                    f32x16 x, dp;
+        auto tile = [&](int j, float add, auto near_tag) __attribute__((always_inline)) {             // add: what every score of the tile gets, −inf at keys that do not count
+            constexpr bool NEAR = decltype(near_tag)::value;
+            const char* const base = smem + buf;
+            const float* const lp = rows + buf / RB_BUF * 128 + 8 * hi;
+            // x[r], dp[r] of half t: key l32, query 64j + 32t + 16(r >> 3) + 8hi + (r & 7)
+            auto begin = [&](int t, f32x16& x, f32x16& dp) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) { x[i] = 0.f; dp[i] = 0.f; }
+                for (int s = 0; s < 2; ++s) {
+                    const f32x4 l0 = *(const f32x4*)(lp + 32 * t + 16 * s), l1 = *(const f32x4*)(lp + 32 * t + 16 * s + 4);
+                    const f32x4 e0 = *(const f32x4*)(lp + 64 + 32 * t + 16 * s), e1 = *(const f32x4*)(lp + 64 + 32 * t + 16 * s + 4);
 #pragma unroll
-                    for (int ks = 0; ks < 4; ++ks) {
-                        x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(base + t * 4096 + roff[ks]), kf[ks], x, 0, 0, 0);
-                        dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(base + RB_TILE + t * 4096 + roff[ks]), vf[ks], dp, 0, 0, 0);
-                    }
-                    const float* lp = rows + buf / RB_BUF * 128 + 32 * t + 8 * hi;
-                    const float* tb = tab + (key - (j * RB_KV + 32 * t + 8 * hi) - 23 + p.reach + RB_PAD);   // of the last of the 16 queries
-                    unsigned pf[2][4], df[2][4];
-#pragma unroll
-                    for (int s = 0; s < 2; ++s) {
-                        const f32x4 l0 = *(const f32x4*)(lp + 16 * s), l1 = *(const f32x4*)(lp + 16 * s + 4);
-                        const f32x4 e0 = *(const f32x4*)(lp + 64 + 16 * s), e1 = *(const f32x4*)(lp + 64 + 16 * s + 4);
-#pragma unroll
-                        for (int e = 0; e < 8; e += 2) {
-                            float pr[2], ds[2];
-#pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                const int r = 8 * s + e + i;
-                                const float l = e < 4 ? l0[e + i] : l1[e + i - 4], dl = e < 4 ? e0[e + i] : e1[e + i - 4];
-                                const float bias = FAR ? far : tb[23 - 16 * s - e - i];
-                                pr[i] = __builtin_amdgcn_exp2f(counts ? fmaf(x[r], p.c, bias - l) : -INFINITY);
-                                ds[i] = pr[i] * (dp[r] - dl);
-                            }
-                            pf[s][e / 2] = pack_bf16x2(pr[0], pr[1]);
-                            df[s][e / 2] = pack_bf16x2(ds[0], ds[1]);
-                        }
-                    }
-                    bf16x8 qt[2][2], gt[2][2];
-                    rb_read_tr(gt, base + RB_TILE + t * 4096, toff);
-                    rb_read_tr(qt, base + t * 4096, toff);
-#pragma unroll
-                    for (int s = 0; s < 2; ++s) {
-                        const bf16x8 pv = __builtin_bit_cast(bf16x8, make_uint4(pf[s][0], pf[s][1], pf[s][2], pf[s][3]));
-                        const bf16x8 dv_ = __builtin_bit_cast(bf16x8, make_uint4(df[s][0], df[s][1], df[s][2], df[s][3]));
-#pragma unroll
-                        for (int dt = 0; dt < 2; ++dt) {
-                            dv[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(gt[s][dt], pv, dv[dt], 0, 0, 0);
-                            dk[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qt[s][dt], dv_, dk[dt], 0, 0, 0);
-                        }
-                    }
-                };
-                if (right || left) {
-                    half(std::integral_constant<int, 0>{}, std::true_type{});
-                    half(std::integral_constant<int, 1>{}, std::true_type{});
-                } else {
-                    half(std::integral_constant<int, 0>{}, std::false_type{});
-                    half(std::integral_constant<int, 1>{}, std::false_type{});
+                    for (int e = 0; e < 4; ++e) { x[8 * s + e] = l0[e]; x[8 * s + 4 + e] = l1[e]; dp[8 * s + e] = e0[e]; dp[8 * s + 4 + e] = e1[e]; }
                 }
-            }
+            };
+            // the A fragment of matrix instruction i of 32: scores and dP of the first half, of the second half, products of the first, of the second
+            auto fragment = [&](int i) {
+                if (i < 16) return *(const bf16x8*)(base + (i & 1) * RB_TILE + (i >> 3) * 4096 + roff[(i >> 1) & 3]);
+                return rb_read_tr1(base + (i & 1 ? 0 : RB_TILE) + ((i >> 3) & 1) * 4096 + 2048 * ((i >> 2) & 1), toff[(i >> 1) & 1]);
+            };
+            auto score = [&](int i, const bf16x8& a, f32x16& x, f32x16& dp) {
+                if (i & 1) dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, vf[(i >> 1) & 3], dp, 0, 0, 0);
+                else x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, kf[(i >> 1) & 3], x, 0, 0, 0);
+            };
+            auto product = [&](int i, const bf16x8& a, const unsigned (&pf)[2][4], const unsigned (&df)[2][4]) {
+                const int s = (i >> 2) & 1, dt = (i >> 1) & 1;
+                const unsigned (&f)[4] = i & 1 ? df[s] : pf[s];
+                const bf16x8 v = __builtin_bit_cast(bf16x8, make_uint4(f[0], f[1], f[2], f[3]));
+                if (i & 1) dk[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, v, dk[dt], 0, 0, 0);
+                else dv[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, v, dv[dt], 0, 0, 0);
+            };
+            auto weigh = [&](int e, int t, const f32x16& x, const f32x16& dp, unsigned (&pf)[2][4], unsigned (&df)[2][4]) {   // elements 2e, 2e + 1
+                const float* const tb = tab + (key - (j * RB_KV + 32 * t + 8 * hi) - 23 + p.reach + RB_PAD);   // of the last of the 16 queries
+                float pr[2], ds[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int r = 2 * e + i;
+                    pr[i] = __builtin_amdgcn_exp2f(fmaf(x[r], c, NEAR ? tb[23 - 16 * (r >> 3) - (r & 7)] + add : add));
+                    ds[i] = pr[i] * dp[r];
+                }
+                pf[e >> 2][e & 3] = pack_bf16x2(pr[0], pr[1]);
+                df[e >> 2][e & 3] = pack_bf16x2(ds[0], ds[1]);
+            };
+            f32x16 x0, dp0, x1, dp1;
+            unsigned p0[2][4], d0[2][4], p1[2][4], d1[2][4];
+            constexpr int AHEAD = 3;                                  // fragments are read this many instructions before they are used
+            bf16x8 f[AHEAD + 1];
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) f[i] = fragment(i);
+            begin(0, x0, dp0);
+            rb_static_for<32>([&](auto i_tag) __attribute__((always_inline)) {
+                constexpr int i = decltype(i_tag)::value;
+                if constexpr (i + AHEAD < 32) f[(i + AHEAD) % (AHEAD + 1)] = fragment(i + AHEAD);
+                const bf16x8& a = f[i % (AHEAD + 1)];
+                if constexpr (i < 8) score(i, a, x0, dp0);
+                else if constexpr (i < 16) score(i, a, x1, dp1);
+                else if constexpr (i < 24) product(i, a, p0, d0);
+                else product(i, a, p1, d1);
+                if constexpr (i == 5) begin(1, x1, dp1);
+                if constexpr (i >= 8 && i < 16) weigh(i - 8, 0, x0, dp0, p0, d0);
+                if constexpr (i >= 16 && i < 24) weigh(i - 16, 1, x1, dp1, p1, d1);
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        };
+        auto advance = [&](int j) __attribute__((always_inline)) {
             rb_tiles_landed();                                        // tile j + 1, issued one tile ago, and its rows' L and δ
             put_rows(rb_next(buf));
             if (j + 2 < nq) stage(j + 2, rb_next(rb_next(buf)));      // its buffer was last read before the previous barrier
             rb_reads_done_barrier();
             buf = rb_next(buf);
+        };
+        // three loops, so that each has one body: queries left of the wave's keys, around them, right of them.  The workgroup's waves change over at different
+        // tiles; every iteration has the same one barrier.
+        const int near_from = k0 - 63 - p.reach >= 0 ? min(nq, (k0 - 63 - p.reach) / RB_KV + 1) : 0;   // the first tile with k0 - 64j - 63 < reach
+        const int near_to = min(nq, (k0 + 31 + p.reach + RB_KV - 1) / RB_KV);                          // the first with k0 + 31 - 64j <= -reach
+        int j = 0;
+        for (; j < near_from; ++j) {
+            if (some) tile(j, far_r + off, std::false_type{});
+            advance(j);
+        }
+        for (; j < near_to; ++j) {
+            if (some) tile(j, off, std::true_type{});
+            advance(j);
+        }
+        for (; j < nq; ++j) {
+            if (some) tile(j, far_l + off, std::false_type{});
+            advance(j);
         }
     }
     // a key that does not count has P = dS = 0; times a NaN of some row's dO that would be a NaN
 #pragma unroll
     for (int i = 0; i < 16; ++i)
 #pragma unroll
-        for (int dt = 0; dt < 2; ++dt) { dk[dt][i] = counts ? dk[dt][i] : 0.f; dv[dt][i] = counts ? dv[dt][i] : 0.f; }
+        for (int dt = 0; dt < 2; ++dt) { dk[dt][i] = counts && !lone ? dk[dt][i] : 0.f; dv[dt][i] = counts ? dv[dt][i] : 0.f; }
     rb_store(dk, args.scale, dkp, hi, key < S);
     rb_store(dv, 1.f, dvp, hi, key < S);
 }
