@@ -9,9 +9,9 @@
 //   * The bias depends on key − query alone and is constant beyond `reach` (91 positions for 32 buckets up to 128): a tile that lies beyond it adds ONE
 //     number, folded into the fma that scales the scores.  Only the few tiles along the diagonal look their bias up, in a table of 2·reach + 1 floats
 //     in LDS, whose addresses are consecutive over the lanes (no bank conflicts).
-//   * Soft-max over one pass: the shift of a row is the true maximum of its first tile; later tiles are exponentiated against it and checked
-//     afterwards (a lane's partial sum above 2^100, or NaN, makes the wave take the classic online step on the scores it still holds).  Any shift
-//     gives the same soft-max; the check keeps exp2 inside fp32.  Sums are fp32; P is rounded to bf16 once, as the operand of P·V.
+//   * Soft-max over one pass: the shift of a row is the maximum of its first 32 scores that holds one above -inf; later scores are exponentiated against it
+//     and checked afterwards (a lane's partial sum above 2^40, or NaN, makes the wave compute these scores again and take the classic online step).  Any
+//     shift gives the same soft-max; the check keeps P·V inside fp32 for |v| up to 1e22.  Sums are fp32; P is rounded to bf16 once, as the operand of P·V.
 //   * For a backward pass the output is needed beyond bf16: δ = dO·O is subtracted from numbers that may be nearly equal to it.  TRAIN multiplies V with P in
 //     two bf16 parts (P = hi + lo to 2^-17) and also stores what the rounding of O left (o_low), so that O + o_low is good to 2^-16.
 //   * Keys that do not count: whole tiles are skipped; in a tile that holds some, their scores become −inf and their V elements 0 (a NaN or an infinity
@@ -27,8 +27,11 @@ struct RbFwdArgs { RbArgs a; bf16_t* o; bf16_t* o_low; float* lse; };   // o_low
 // tiles from which the pipelined loop is used: its start and end cost about two tiles' time, its registers the third wave of a SIMD
 constexpr int RB_PIPE_TILES = 7;
 
+// beyond this a row's shift is taken off the rounded sum of score and bias, as it was found, so that all of a row's scores round alike
+constexpr float RB_FAR_SHIFT = 16384.f;
+
 template <int NW, bool TRAIN, bool PIPE>
-__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(PIPE ? 2 : 3, PIPE ? 2 : 3))) void relbias_attn_fwd_kernel(RbFwdArgs args) {
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(PIPE || NW == 1 ? 2 : 3, PIPE || NW == 1 ? 2 : 3))) void relbias_attn_fwd_kernel(RbFwdArgs args) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const RbArgs& p = args.a;
     float* const tab = (float*)(smem + RB_RING);
@@ -87,7 +90,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(PIPE ? 
 #pragma unroll
     for (int i = 0; i < 16; ++i) { o[0][i] = 0.f; o[1][i] = 0.f; }
     float m_run = 0.f, l_run = 0.f;
-    bool started = false;
+    bool started = false, fresh = true;                               // (of the wave) a key was met; (of the row) only scores of -inf were
 
     rb_arrived(qf);
     drain_and_barrier();                                              // table and words are there, and the first two tiles
@@ -97,12 +100,12 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(PIPE ? 
             if ((w = rb_word(p, words, j)) != 0) break;
         return j;
     };
-    // Tile by tile from `first` on, any tile: the tiles in front of it are done.  fresh: tiles 0 and 1 are in the first two buffers.
-    auto sweep = [&](int first, bool fresh) {
+    // Tile by tile from `first` on, any tile: the tiles in front of it are done.  staged: tiles 0 and 1 are in the first two buffers.
+    auto sweep = [&](int first, bool staged) {
         uint64_t w = 0, w1 = 0, w2 = 0;
         int j = next_tile(first, w), j1 = next_tile(j + 1, w1);
         int buf = 0;
-        if (!fresh || j != 0 || j1 != 1) {                            // not the tiles that were staged at the start
+        if (!staged || j != 0 || j1 != 1) {                            // not the tiles that were staged at the start
             if (j < nkv) stage(j, 0);
             if (j1 < nkv) stage(j1, RB_BUF);
             drain_and_barrier();
@@ -128,22 +131,29 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(PIPE ? 
                 constexpr int t = decltype(t_tag)::value;
                 const unsigned wt = (unsigned)(w >> (32 * t));
                 if (part && wt == 0) return;                              // (wave-uniform) no key in this half
-                if (right || left) {
-                    const float add = (right ? far_r : far_l) - m_run;
+                auto weigh = [&](float shift) __attribute__((always_inline)) {   // scale, bias and shift, -inf at keys that do not count
+                    if (right || left) {
+                        const float add = (right ? far_r : far_l) - shift;
     #pragma unroll
-                    for (int r = 0; r < 16; ++r) x[t][r] = fmaf(x[t][r], p.c, add);
-                } else {
-                    // |d| <= reach + 94 here: inside the padded table.  A query row beyond the last one reads inside it too (its wave's own range).
-                    const float* tb = tab + (j * RB_KV + 32 * t + 8 * hi - qrow + p.reach + RB_PAD);
+                        for (int r = 0; r < 16; ++r) x[t][r] = fmaf(x[t][r], p.c, add);
+                    } else {
+                        // |d| <= reach + 94 here: inside the padded table.  A query row beyond the last one reads inside it too (its wave's own range).
+                        const float* tb = tab + (j * RB_KV + 32 * t + 8 * hi - qrow + p.reach + RB_PAD);
     #pragma unroll
-                    for (int r = 0; r < 16; ++r) x[t][r] = fmaf(x[t][r], p.c, tb[16 * (r >> 3) + (r & 7)] - m_run);
-                }
-                if (__builtin_expect(part, 0)) {
-                    const unsigned mine = wt >> (8 * hi);
+                        for (int r = 0; r < 16; ++r) x[t][r] = fmaf(x[t][r], p.c, tb[16 * (r >> 3) + (r & 7)] - shift);
+                    }
+                    if (__builtin_expect(part, 0)) {
+                        const unsigned mine = wt >> (8 * hi);
     #pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (!((mine >> (16 * (r >> 3) + (r & 7))) & 1)) x[t][r] = -INFINITY;
-                }
+                        for (int r = 0; r < 16; ++r)
+                            if (!((mine >> (16 * (r >> 3) + (r & 7))) & 1)) x[t][r] = -INFINITY;
+                    }
+                };
+                if (__builtin_expect(__any(fabsf(m_run) > RB_FAR_SHIFT) != 0, 0)) {   // bias - shift would keep digits that the shift, a sum with the bias, lost
+                    weigh(0.f);
+    #pragma unroll
+                    for (int r = 0; r < 16; ++r) x[t][r] -= m_run;
+                } else weigh(m_run);
                 unsigned pf[2][4], pl[2][4];
                 float tsum = 0.f;
                 auto expo = [&]() {
@@ -170,23 +180,32 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(PIPE ? 
                 bool redo = !started;
                 if (!redo) {
                     expo();
-                    redo = __any(!(tsum <= 1.2676506e30f)) != 0;          // 2^100
+                    redo = __any(fresh || !(tsum <= 1.099511627776e12f)) != 0;   // 2^40
                 }
                 if (__builtin_expect(redo, 0)) {
+                    if (started) {                                        // the scores once more: shifted far, they have lost digits
+    #pragma unroll
+                        for (int r = 0; r < 16; ++r) x[t][r] = 0.f;
+    #pragma unroll
+                        for (int ks = 0; ks < 4; ++ks)
+                            x[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(base + t * 4096 + koff[ks]), qf[ks], x[t], 0, 0, 0);
+                        weigh(0.f);
+                    }
                     float top = x[t][0];
     #pragma unroll
                     for (int r = 1; r < 16; ++r) top = fmaxf(top, x[t][r]);
                     top = fmaxf(top, __shfl_xor(top, 32, 64));
-                    const float up = started ? fmaxf(top, 0.f) : top == -INFINITY ? 0.f : top;
+                    const float to = fresh ? (top == -INFINITY ? 0.f : top) : fmaxf(m_run, top);
                     if (started) {
-                        const float alpha = __builtin_amdgcn_exp2f(-up);
+                        const float alpha = fresh ? 1.f : __builtin_amdgcn_exp2f(m_run - to);
     #pragma unroll
                         for (int i = 0; i < 16; ++i) { o[0][i] *= alpha; o[1][i] *= alpha; }
                         l_run *= alpha;
                     }
-                    m_run += up;
+                    m_run = to;
+                    fresh = fresh && top == -INFINITY;
     #pragma unroll
-                    for (int i = 0; i < 16; ++i) x[t][i] -= up;
+                    for (int i = 0; i < 16; ++i) x[t][i] -= to;
                     expo();
                     started = true;
                 }
@@ -344,6 +363,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(PIPE ? 
         for (int i = 0; i < 4; ++i) product(i, va, p1, l1);
         l_run = s0 + s1;
         started = true;
+        fresh = false;
         drain_and_barrier();
     };
     int whole = 0;                                                    // tiles at the front whose keys all count
@@ -358,6 +378,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(PIPE ? 
         pipeline(whole);
         if (whole < nkv) sweep(whole, false);
         float worst = fabsf(l_run);
+        if (fabsf(m_run) > RB_FAR_SHIFT) worst = INFINITY;
 #pragma unroll
         for (int i = 0; i < 16; ++i) worst = fmaxf(worst, fmaxf(fabsf(o[0][i]), fabsf(o[1][i])));
         bool bad = !(worst <= 3.4e38f);
@@ -370,6 +391,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(PIPE ? 
             m_run = 0.f;
             l_run = 0.f;
             started = false;
+            fresh = true;
             sweep(0, false);
         }
     } else sweep(0, true);
@@ -378,8 +400,10 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(PIPE ? 
     const float inv = started ? 1.0f / l_tot : 0.f;
     const size_t at = (((size_t)b * S + min(qrow, S - 1)) * p.H + h) * RB_D;
     if constexpr (TRAIN) {
-        if (hi == 0 && qrow < S)              // +inf: the backward pass gets P = 0 everywhere in such a row
-            args.lse[(size_t)bh * S + qrow] = started ? m_run + __builtin_amdgcn_logf(l_tot) : INFINITY;
+        if (hi == 0 && qrow < S) {            // +inf: the backward pass gets P = 0 everywhere in such a row; beyond 2^20 a log-sum's digits do not tell P any more
+            const float l = m_run + __builtin_amdgcn_logf(l_tot);
+            args.lse[(size_t)bh * S + qrow] = !started || fabsf(l) > 1048576.f ? INFINITY : l;
+        }
         f32x16 low[2];
 #pragma unroll
         for (int dt = 0; dt < 2; ++dt)
@@ -415,6 +439,8 @@ int rb_setup(RbArgs& p, const AetherRelbias* d) {
         p.border[i] = last;
     }
     if (last > RB_MAX_REACH) return fail(AETHER_ERR_SHAPE, "relbias_attn: the last bucket must begin at 1024 or before");
+    if (!(d->scale == 0.f || (fabsf(d->scale) >= 1e-20f && fabsf(d->scale) <= 1e20f)))    // (a backward pass divides by it)
+        return fail(AETHER_ERR_ARG, "relbias_attn: the scale must be 0 or of a magnitude in [1e-20, 1e20]");
     p.B = d->B; p.S = d->S; p.H = d->H;
     p.half = half; p.near_n = near_n; p.n_border = d->n_borders; p.reach = last;
     p.c = d->scale * RB_LOG2E;

@@ -49,7 +49,10 @@ AE_DEV void rb_fill_table(const RbArgs& p, int h, float* tab, int nthreads) {
         }
 #pragma unroll
         for (int k = 0; k < 2; ++k)
-            if (i0 + k * nthreads < n_tab) tab[i0 + k * nthreads] = (float)v[k] * RB_LOG2E;
+            if (i0 + k * nthreads < n_tab) {
+                const float t = (float)v[k];                              // a finite entry stays finite in log2 units: rows that hold only the type's lowest value are uniform
+                tab[i0 + k * nthreads] = fabsf(t) < INFINITY ? fminf(fmaxf(t * RB_LOG2E, -3.3e38f), 3.3e38f) : t;
+            }
     }
 }
 

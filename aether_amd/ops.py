@@ -297,6 +297,8 @@ def _relbias(name, q, k, v, table, max_distance, scale, key_mask):
         raise ValueError(f"{name}: no heads")
     if table.dtype != torch.bfloat16 or table.dim() != 2 or table.shape[1] != H:
         raise ValueError(f"{name}: the table is bfloat16 [num_buckets, {H}], got {table.dtype} {list(table.shape)}")
+    if not (scale == 0 or 1e-20 <= abs(scale) <= 1e20):
+        raise ValueError(f"{name}: the scale is 0 or of a magnitude in [1e-20, 1e20], got {scale}")
     borders = relbias_borders(table.shape[0], max_distance)
     q, k, v, table = _heads(q), _heads(k), _heads(v), table.contiguous()
     if key_mask is not None:
@@ -314,7 +316,8 @@ def relbias_attn(q, k, v, table, max_distance=128, scale=1.0, key_mask=None, nee
     """Self-attention with a learned bias by relative position: S_ij = scale q_i·k_j + table[bucket(j − i), h], O = softmax(S) V over the keys that count.
     q, k, v bfloat16 [B, S, H, 64] (views of a packed projection included), table bfloat16 [num_buckets, H] (buckets of both directions, exact up to
     num_buckets / 4, logarithmic up to max_distance), key_mask bool [B, S], True where a key counts.  A row without keys gives 0; what stands at
-    keys that do not count reaches nothing.  -> o bfloat16 [B, S, H, 64]; with need_lse (o, lse), where lse (float32, flat) is what
+    keys that do not count reaches nothing.  |v| up to 1e22: weighted sums are held in float32 before they are normalized.
+    -> o bfloat16 [B, S, H, 64]; with need_lse (o, lse), where lse (float32, flat) is what
     `relbias_attn_backward` needs besides o: the rows' log-sums to base 2 [B, H, S], then, from the next 16 bytes on, o's rounding remainders
     (bfloat16 [B, S, H, 64]).  P then multiplies v in two parts, and o is a little more exact than without."""
     dev, d, keep = _relbias("relbias_attn", q, k, v, table, max_distance, scale, key_mask)
@@ -335,7 +338,8 @@ _Strides = C.c_long * 3
 
 def relbias_attn_backward(do, q, k, v, o, lse, table, max_distance=128, scale=1.0, key_mask=None, need_dtable=True):
     """Gradients of `relbias_attn` from its inputs, its output o and its lse: -> (dq, dk, dv bfloat16 [B, S, H, 64], thirds of one packed
-    [B, S, 3, H, 64] buffer; dtable bfloat16 [num_buckets, H] or None).  dk and dv are 0 at keys that do not count.  Summed in an order that
+    [B, S, 3, H, 64] buffer; dtable bfloat16 [num_buckets, H] or None).  dk and dv are 0 at keys that do not count.  P comes from
+    the log-sums again: a row whose largest score lies beyond ±7e5 has no gradient.  Summed in an order that
     depends on the sizes alone."""
     name = "relbias_attn_backward"
     dev, d, keep = _relbias(name, q, k, v, table, max_distance, scale, key_mask)

@@ -23,7 +23,7 @@ def _run(q, k, v, table, do, **kw):
     return ops.relbias_attn_backward(do, q, k, v, o, lse, table, **kw)
 
 
-def _check(got, q, k, v, table, do, scale=1.0, **kw):
+def _check(got, q, k, v, table, do, scale=1.0, S32=S32, **kw):
     leaf = [t.double().requires_grad_(True) for t in (q, k, v, table)]
     o, p = attention(*leaf, scale=scale, **kw)
     want = torch.autograd.grad((o * do.double()).sum(), leaf)
@@ -120,6 +120,70 @@ def test_masks(cuda, hip_lib, kind, S):
         bad[:, :, 1:][at] = val
     again = _run(q, bad[:, :, 1], bad[:, :, 2], table, do, key_mask=mask)
     assert all(torch.equal(x, y) for x, y in zip(got, again)), "what stands behind the mask reaches nothing"
+
+
+@pytest.mark.parametrize("kind", ["right", "left", "holes", "blocks"])
+def test_masks_long(cuda, hip_lib, kind):
+    B, S, H = 2, 1030, 2
+    qkv, table = inputs(B, S, H, device=cuda, seed=34)
+    mask = _masks(B, S, cuda)[kind]
+    q, k, v = qkv.unbind(2)
+    do = _do(q)
+    got = _run(q, k, v, table, do, key_mask=mask)
+    _check(got, q, k, v, table, do, key_mask=mask)
+    bad = qkv.clone()
+    bad[:, :, 1:][~mask] = math.nan
+    assert all(torch.equal(x, y) for x, y in zip(got, _run(q, bad[:, :, 1], bad[:, :, 2], table, do, key_mask=mask)))
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1, 0.02])
+@pytest.mark.parametrize("S", [70, 500])
+def test_scales(cuda, hip_lib, scale, S):
+    qkv, table = inputs(2, S, 2, device=cuda, seed=35, qk=4.0)
+    q, k, v = qkv.unbind(2)
+    do = _do(q)
+    got = _run(q, k, v, table, do, scale=scale)
+    _check(got, q, k, v, table, do, scale=scale)
+    if scale == 0:
+        assert not got[0].any() and not got[1].any()
+
+
+@pytest.mark.parametrize("order", ["early", "late", "rising", "far_below"])
+@pytest.mark.parametrize("S", [200, 700])
+def test_score_ranges(cuda, hip_lib, order, S):
+    """Scores of several hundred: they and the log-sum carry 66 · 2^-24 · 800 < 2^-8 each."""
+    qkv, table = inputs(1, S, 2, device=cuda, seed=36)
+    at = torch.arange(S, device=cuda, dtype=torch.float32)
+    level = dict(early=400 * (at < 5), late=400 * (at > S - 9), rising=at * (400 / S), far_below=at * 0 - 400)[order]
+    q, k, v = (t.clone() for t in qkv.unbind(2))
+    q[..., 0], k[..., 0] = 4.0, (level / 4).to(torch.bfloat16)[None, :, None]
+    do = _do(q)
+    _check(_run(q, k, v, table, do), q, k, v, table, do, S32=2.0 ** -6)
+
+
+@pytest.mark.parametrize("low", [-math.inf, torch.finfo(torch.bfloat16).min, -1e9])
+@pytest.mark.parametrize("S", [70, 500])
+@pytest.mark.parametrize("scale", [1.0, 0.1])
+def test_one_side_switched_off(cuda, hip_lib, low, S, scale):
+    """Buckets at −inf or the type's lowest value: rows see the keys up to their own.  Rows of the padding in front, which see the lowest value alone, have no
+    gradient and bring none."""
+    qkv, table = inputs(2, S, 2, device=cuda, seed=37)
+    table[table.shape[0] // 2:] = low
+    q, k, v = qkv.unbind(2)
+    do = _do(q)
+    got = _run(q, k, v, table, do, scale=scale)
+    want = table.clone()
+    want[table.shape[0] // 2:] = -2000.0         # exp of it is 0 in float64 too, and its gradient a number
+    _check(got, q, k, v, want, do, scale=scale)
+    if low != -math.inf:
+        mask = torch.ones(2, S, dtype=torch.bool, device=cuda)
+        mask[1, :25] = False
+        do[1, :25] = 0
+        got = _run(q, k, v, table, do, scale=scale, key_mask=mask)
+        assert all(bool(torch.isfinite(x.float()).all()) for x in got) and not got[0][1, :25].any()
+        part = _run(q[1:, 25:], k[1:, 25:], v[1:, 25:], table, do[1:, 25:], scale=scale)
+        for x, y in zip(got[:3], part[:3]):
+            assert bool(((x[1, 25:].double() - y[0].double()).norm() <= 4 * BF16 * y.double().norm()))
 
 
 def test_empty_row_with_non_finite_gradient(cuda, hip_lib):

@@ -170,6 +170,98 @@ def test_score_ranges(cuda, hip_lib, order):
     _check_o(ops.relbias_attn(q, k, v, table), q, k, v, table, extra=2.0 ** -6)
 
 
+@pytest.mark.parametrize("order", ["early", "late", "middle", "rising", "falling", "far_below"])
+@pytest.mark.parametrize("masked", [False, True])
+def test_score_ranges_long(cuda, hip_lib, order, masked):
+    """The same over many tiles, with and without what a backward pass needs; the mask takes keys at the end and a few in between."""
+    from aether_amd import ops
+    B, S, H = 2, 1100, 2
+    qkv, table = inputs(B, S, H, device=cuda, seed=17)
+    at = torch.arange(S, device=cuda, dtype=torch.float32)
+    level = dict(early=400 * (at < 5), late=400 * (at > S - 60), middle=400 * ((at > 500) & (at < 510)), rising=at * (400 / S), falling=(S - at) * (400 / S), far_below=at * 0 - 400)[order]
+    q = qkv[:, :, 0].clone()
+    k = qkv[:, :, 1].clone()
+    q[..., 0], k[..., 0] = 4.0, (level / 4).to(torch.bfloat16)[None, :, None]
+    q[1, ::2, :, 0] = 0.25                    # every other row of the second item has ordinary scores
+    v = qkv[:, :, 2]
+    mask = None
+    if masked:
+        mask = torch.ones(B, S, dtype=torch.bool, device=cuda)
+        mask[0, 1070:], mask[1, 700:720], mask[1, 1099:] = False, False, False
+    o = ops.relbias_attn(q, k, v, table, key_mask=mask)
+    _check_o(o, q, k, v, table, extra=2.0 ** -6, key_mask=mask)
+    o2, _ = ops.relbias_attn(q, k, v, table, key_mask=mask, need_lse=True)
+    _check_o(o2, q, k, v, table, extra=2.0 ** -6, key_mask=mask)
+
+
+@pytest.mark.parametrize("low", [-math.inf, torch.finfo(torch.bfloat16).min, -1e9, -300.0])
+@pytest.mark.parametrize("which", ["right", "left", "far", "near"])
+@pytest.mark.parametrize("S", [70, 600])
+def test_buckets_that_are_switched_off(cuda, hip_lib, low, which, S):
+    """A table that holds the lowest value, −inf or a very negative number for one side, for the far buckets or for the near ones; scores of −200 where the
+    others are.  Every row has a key with an ordinary bucket."""
+    from aether_amd import ops
+    qkv, table = inputs(2, S, 2, device=cuda, seed=18)
+    half = table.shape[0] // 2
+    if which == "right":
+        table[half:] = low
+    elif which == "left":
+        table[1:half] = low
+    elif which == "far":
+        table[12:half], table[half + 12:] = low, low
+    else:
+        table[1:5], table[half:half + 5] = low, low
+    q, k, v = (t.clone() for t in qkv.unbind(2))
+    q[..., 0], k[..., 0] = 4.0, -50.0
+    for train in (False, True):
+        o = ops.relbias_attn(q, k, v, table, need_lse=train)
+        _check_o(o[0] if train else o, q, k, v, table, extra=2.0 ** -7)     # 66 · 2^-24 · 2 · (200 + 60 + 300) < 2^-7
+
+
+@pytest.mark.parametrize("S", [40, 500])
+def test_rows_of_the_lowest_value_are_uniform(cuda, hip_lib, S):
+    """Every key of a row at the type's lowest value: all scores are the same number, as they are in a sum with it in float32."""
+    from aether_amd import ops
+    qkv, table = inputs(1, S, 2, device=cuda, seed=19)
+    q, k, v = qkv.unbind(2)
+    o = ops.relbias_attn(q, k, v, torch.full_like(table, torch.finfo(torch.bfloat16).min))
+    want, T = v.double().mean(1, keepdim=True), v.double().abs().mean(1, keepdim=True)
+    assert bool(((o.double() - want).abs() <= (BF16 + 2.0 ** -10) * T + BF16 * want.abs()).all())
+
+
+@pytest.mark.parametrize("S", [64, 700])
+def test_large_values(cuda, hip_lib, S):
+    """v at the documented limit, scores that rise over the sequence."""
+    from aether_amd import ops
+    qkv, table = inputs(1, S, 2, device=cuda, seed=20)
+    q, k, v = (t.clone() for t in qkv.unbind(2))
+    q[..., 0], k[..., 0] = 4.0, (torch.arange(S, device=cuda) * (80 / S)).to(torch.bfloat16)[None, :, None]
+    v = (v.clamp(-4, 4) * 2.5e21).contiguous()
+    for train in (False, True):
+        o = ops.relbias_attn(q, k, v, table, need_lse=train)
+        _check_o(o[0] if train else o, q, k, v, table, extra=2.0 ** -6)
+
+
+@pytest.mark.parametrize("where", [0, 77, 599])
+def test_non_finite_inputs_long(cuda, hip_lib, where):
+    """A NaN in one query of a long sequence makes that row NaN and no other; one in a key makes its head's rows NaN and no other head's."""
+    from aether_amd import ops
+    qkv, table = inputs(1, 600, 2, device=cuda, seed=21)
+    q, k, v = qkv.unbind(2)
+    o = ops.relbias_attn(q, k, v, table)
+    bad = q.clone()
+    bad[0, where, 1, 5] = math.nan
+    got = ops.relbias_attn(bad, k, v, table)
+    assert bool(torch.isnan(got[0, where, 1].float()).all())
+    keep = torch.ones(600, 2, dtype=torch.bool, device=cuda)
+    keep[where, 1] = False
+    assert bool(((got[0][keep].float() - o[0][keep].float()).abs() <= 2 * BF16 * o[0][keep].float().abs() + 1e-2).all())
+    bad = k.clone()
+    bad[0, where, 1, 5] = math.nan
+    got = ops.relbias_attn(q, bad, v, table)
+    assert torch.equal(got[:, :, 0], o[:, :, 0]) and bool(torch.isnan(got[:, :, 1].float()).all())
+
+
 def test_scale(cuda, hip_lib):
     from aether_amd import ops
     qkv, table = inputs(2, 150, 2, device=cuda, seed=8, qk=8.0)
@@ -221,7 +313,7 @@ def test_refusals(cuda, hip_lib):
                 lambda: ops.relbias_attn(q, k, v, table.float()), lambda: ops.relbias_attn(q, k, v, table[:, :1]), lambda: ops.relbias_attn(q, k, v, table[:31]),
                 lambda: ops.relbias_attn(q, k, v, table[:2]), lambda: ops.relbias_attn(q, k, v, table, max_distance=8), lambda: ops.relbias_attn(q, k, v, table, max_distance=5000),
                 lambda: ops.relbias_attn(q, k, v, table, key_mask=mask.float()), lambda: ops.relbias_attn(q, k, v, table, key_mask=mask[:, :8]),
-                lambda: ops.relbias_attn(q[0], k[0], v[0], table)):
+                lambda: ops.relbias_attn(q[0], k[0], v[0], table), lambda: ops.relbias_attn(q, k, v, table, scale=math.nan), lambda: ops.relbias_attn(q, k, v, table, scale=1e-25)):
         with pytest.raises(ValueError):
             bad()
     with pytest.raises(RuntimeError, match="device tensors"):

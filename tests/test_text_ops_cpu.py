@@ -80,7 +80,7 @@ def _relbias(lib, o=4096, **kw):
     a.update(kw)
     b = a["borders"]
     arr = (C.c_int * len(b))(*b) if b is not None else None
-    d = _lib.AetherRelbias(a["q"], a["k"], a["v"], a["st"], a["st"], a["st"], a["table"], a["mask"], 0, a["B"], a["S"], a["H"], 1.0, a["num_buckets"], arr, len(b or ()))
+    d = _lib.AetherRelbias(a["q"], a["k"], a["v"], a["st"], a["st"], a["st"], a["table"], a["mask"], 0, a["B"], a["S"], a["H"], a.get("scale", 1.0), a["num_buckets"], arr, len(b or ()))
     return lib.aether_relbias_attn(C.byref(d), o, a["low"], a["lse"], None)
 
 
@@ -92,7 +92,7 @@ def _relbias(lib, o=4096, **kw):
     (dict(table=None), -1, b"table"), (dict(q=None), -1, b"operand"), (dict(v=None), -1, b"operand"), (dict(k=4104), -3, b"aligned"),
     (dict(st=(4096, 60, 64)), -3, b"aligned"), (dict(st=(4096, -64, 64)), -2, b"stride"), (dict(st=(-4096, 64, 64)), -2, b"stride"),
     (dict(st=(0, 1 << 15, 64), S=65536), -2, b"4 GiB"), (dict(o=None), -1, b"output"), (dict(low=4096), -1, b"together"), (dict(lse=4096), -1, b"together"), (dict(low=4104, lse=4096), -3, b"aligned"), (dict(o=4104), -3, b"aligned"),
-    (dict(B=1 << 20, H=1 << 10, S=65536), -2, b"blocks"),
+    (dict(B=1 << 20, H=1 << 10, S=65536), -2, b"blocks"), (dict(scale=float("nan")), -1, b"scale"), (dict(scale=float("inf")), -1, b"scale"), (dict(scale=1e-30), -1, b"scale"),
 ])
 def test_relbias_entry_refuses(hip_lib, kw, code, text):
     assert _relbias(hip_lib, **kw) == code and text in hip_lib.aether_last_error()
