@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import struct
 
 import torch
 
@@ -169,6 +170,11 @@ def _vector(t):
     return t if t.stride(0) == 1 and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
+def _like(t, dtype):
+    """An output of t's shape (half the time of torch.empty with a device)."""
+    return torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
+
+
 _STREAMS = {torch.bfloat16: _lib.AETHER_STREAM_BF16, torch.float32: _lib.AETHER_STREAM_FP32}
 
 
@@ -192,12 +198,12 @@ def _rms_norm(x, w, eps, delta, e4m3):
     D = _norm_operands(x, w, delta, name)
     x2, w = _rows(x, D), _vector(w)
     rows = x2.shape[0]
-    y = torch.empty(x.shape, dtype=torch.float8_e4m3fn if e4m3 else torch.bfloat16, device=dev)
+    y = _like(x, torch.float8_e4m3fn if e4m3 else torch.bfloat16)
     scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev) if e4m3 else None
     if delta is None:
         d2, res = None, None
     else:
-        d2, res = _rows(delta, D), torch.empty(x.shape, dtype=x.dtype, device=dev)
+        d2, res = _rows(delta, D), _like(x, x.dtype)
     if rows:
         _run(name, dev, _lib.load().aether_rms_norm, x2.data_ptr(), _STREAMS[x.dtype], x2.stride(0), _lib.ptr(d2), d2.stride(0) if d2 is not None else 0,
              _lib.ptr(res), D, w.data_ptr(), float(eps), y.data_ptr(), D, _lib.ptr(scale), rows, D)
@@ -278,6 +284,12 @@ def relbias_borders(num_buckets, max_distance):
     return (C.c_int * len(found))(*found)
 
 
+@functools.lru_cache(maxsize=None)
+def _borders(num_buckets, max_distance):
+    found = relbias_borders(num_buckets, max_distance)
+    return found, C.addressof(found)
+
+
 def _heads(t):
     """[B, S, H, 64] with a dense last dimension, whole 16-byte pieces between rows and an aligned base; copied only where it is not so."""
     sb, ss, sh, one = t.stride()
@@ -289,26 +301,27 @@ def _heads(t):
 def _relbias(name, q, k, v, table, max_distance, scale, key_mask):
     """(device, descriptor, what it points at) of a call."""
     dev = _same_device(q, k, v, table, key_mask)
+    shape = q.shape
     for n, t in (("q", q), ("k", k), ("v", v)):
-        if t.dtype != torch.bfloat16 or t.dim() != 4 or t.shape[3] != 64 or t.shape != q.shape:
+        if t.dtype != torch.bfloat16 or t.shape != shape or len(shape) != 4 or shape[3] != 64:
             raise ValueError(f"{name}: q, k, v are bfloat16 [B, S, H, 64] of one shape; {n} is {t.dtype} {list(t.shape)}")
-    B, S, H, _ = q.shape
+    B, S, H, _ = shape
     if H < 1:
         raise ValueError(f"{name}: no heads")
     if table.dtype != torch.bfloat16 or table.dim() != 2 or table.shape[1] != H:
         raise ValueError(f"{name}: the table is bfloat16 [num_buckets, {H}], got {table.dtype} {list(table.shape)}")
     if not (scale == 0 or 1e-20 <= abs(scale) <= 1e20):
         raise ValueError(f"{name}: the scale is 0 or of a magnitude in [1e-20, 1e20], got {scale}")
-    borders = relbias_borders(table.shape[0], max_distance)
+    borders, borders_at = _borders(table.shape[0], max_distance)
     q, k, v, table = _heads(q), _heads(k), _heads(v), table.contiguous()
     if key_mask is not None:
         if key_mask.dtype != torch.bool or key_mask.shape != (B, S):
             raise ValueError(f"{name}: key_mask is bool [{B}, {S}], True where a key counts, got {key_mask.dtype} {list(key_mask.shape)}")
         if key_mask.stride(1) != 1 or key_mask.stride(0) < 0:
             key_mask = key_mask.contiguous()
-    d = _lib.AetherRelbias(q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride()[:3], k.stride()[:3], v.stride()[:3], table.data_ptr(),
-                           None if key_mask is None else key_mask.data_ptr(), 0 if key_mask is None else key_mask.stride(0), B, S, H, scale,
-                           table.shape[0], borders, len(borders))
+    d = _lib.RELBIAS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], table.data_ptr(),
+                          0 if key_mask is None else key_mask.data_ptr(), 0 if key_mask is None else key_mask.stride(0), B, S, H, scale,
+                          table.shape[0], borders_at, len(borders))
     return dev, d, (q, k, v, table, key_mask)
 
 
@@ -321,11 +334,11 @@ def relbias_attn(q, k, v, table, max_distance=128, scale=1.0, key_mask=None, nee
     `relbias_attn_backward` needs besides o: the rows' log-sums to base 2 [B, H, S], then, from the next 16 bytes on, o's rounding remainders
     (bfloat16 [B, S, H, 64]).  P then multiplies v in two parts, and o is a little more exact than without."""
     dev, d, keep = _relbias("relbias_attn", q, k, v, table, max_distance, scale, key_mask)
-    o = torch.empty(q.shape, dtype=torch.bfloat16, device=dev)
+    o = _like(q, torch.bfloat16)
     n = o.numel() // 64
     lse = torch.empty(_lse_pad(n) + 32 * n, dtype=torch.float32, device=dev) if need_lse else None
     at = lse.data_ptr() if need_lse else None
-    _run("relbias_attn", dev, _lib.load().aether_relbias_attn, C.byref(d), o.data_ptr(), at + 4 * _lse_pad(n) if need_lse else None, at)
+    _run("relbias_attn", dev, _lib.load().aether_relbias_attn, d, o.data_ptr(), at + 4 * _lse_pad(n) if need_lse else None, at)
     return (o, lse) if need_lse else o
 
 
@@ -333,7 +346,7 @@ def _lse_pad(n):
     return (n + 3) // 4 * 4         # the remainders behind the log-sums begin at whole 16 bytes
 
 
-_Strides = C.c_long * 3
+_strides = struct.Struct("@3l").pack
 
 
 def relbias_attn_backward(do, q, k, v, o, lse, table, max_distance=128, scale=1.0, key_mask=None, need_dtable=True):
@@ -352,14 +365,14 @@ def relbias_attn_backward(do, q, k, v, o, lse, table, max_distance=128, scale=1.
     if lse.dtype != torch.float32 or tuple(lse.shape) != (_lse_pad(n) + 32 * n,):
         raise ValueError(f"{name}: lse is what relbias_attn gave with need_lse, float32 [{_lse_pad(n) + 32 * n}], got {lse.dtype} {list(lse.shape)}")
     do, o, lse = _heads(do), _heads(o), _vector(lse)
-    dqkv = torch.empty(B, S, 3, H, 64, dtype=torch.bfloat16, device=dev)
+    dqkv = q.new_empty(B, S, 3, H, 64)
     dq, dk, dv = dqkv.unbind(2)
-    dtable = torch.empty(table.shape, dtype=torch.bfloat16, device=dev) if need_dtable else None
+    dtable = _like(table, torch.bfloat16) if need_dtable else None
     lib = _lib.load()
-    nbytes = lib.aether_relbias_attn_bwd_workspace_bytes(C.byref(d), need_dtable)
+    nbytes = lib.aether_relbias_attn_bwd_workspace_bytes(d, need_dtable)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    st = _Strides(S * 3 * H * 64, 3 * H * 64, 64)
-    _run(name, dev, lib.aether_relbias_attn_bwd, C.byref(d), do.data_ptr(), _Strides(*do.stride()[:3]), o.data_ptr(), _Strides(*o.stride()[:3]), lse.data_ptr() + 4 * _lse_pad(n), lse.data_ptr(),
+    st = _strides(S * 3 * H * 64, 3 * H * 64, 64)
+    _run(name, dev, lib.aether_relbias_attn_bwd, d, do.data_ptr(), _strides(*do.stride()[:3]), o.data_ptr(), _strides(*o.stride()[:3]), lse.data_ptr() + 4 * _lse_pad(n), lse.data_ptr(),
          dq.data_ptr(), st, dk.data_ptr(), st, dv.data_ptr(), st, _lib.ptr(dtable), ws.data_ptr(), nbytes)
     return dq, dk, dv, dtable
 
@@ -390,8 +403,8 @@ def gated_ff(x, wg, wu, act="gelu_tanh", need_gu=False):
     dev = _same_device(x, wg, wu)
     x2, wg, wu, F, K = _ff_operands("gated_ff", x, wg, wu, act, torch.bfloat16)
     M = x2.shape[0]
-    h = torch.empty(*x.shape[:-1], F, dtype=torch.bfloat16, device=dev)
-    gu = torch.empty(M, 2 * F, dtype=torch.float32, device=dev) if need_gu else None
+    h = x.new_empty(*x.shape[:-1], F)
+    gu = x.new_empty(M, 2 * F, dtype=torch.float32) if need_gu else None
     if M:
         _run("gated_ff", dev, _lib.load().aether_gated_ff, x2.data_ptr(), x2.stride(0), wg.data_ptr(), wu.data_ptr(), wg.stride(0), h.data_ptr(), F, _lib.ptr(gu),
              M, F, K, _ACTS[act])
@@ -408,7 +421,7 @@ def gated_ff_e4m3(x, x_scale, wg, wg_scale, wu, wu_scale, act="gelu_tanh"):
         if t.dtype != torch.float32 or tuple(t.shape) != tuple(shape):
             raise ValueError(f"{name}: {n} is float32 {list(shape)}, got {t.dtype} {list(t.shape)}")
     M = x2.shape[0]
-    h = torch.empty(*x.shape[:-1], F, dtype=torch.bfloat16, device=dev)
+    h = x.new_empty(*x.shape[:-1], F, dtype=torch.bfloat16)
     if M:
         x_scale, wg_scale, wu_scale = x_scale.contiguous(), _vector(wg_scale), _vector(wu_scale)
         _run(name, dev, _lib.load().aether_gated_ff_e4m3, x2.data_ptr(), x2.stride(0), x_scale.data_ptr(), wg.data_ptr(), wg_scale.data_ptr(), wu.data_ptr(),
@@ -428,7 +441,7 @@ def gated_ff_backward(dh, x, wg, wu, gu, act="gelu_tanh", need_dx=True, need_dw=
         raise ValueError(f"{name}: dh is bfloat16 {[*x.shape[:-1], F]}, got {dh.dtype} {list(dh.shape)}")
     if gu.dtype != torch.float32 or tuple(gu.shape) != (M, 2 * F):
         raise ValueError(f"{name}: gu is float32 [{M}, {2 * F}], as gated_ff gave it, got {gu.dtype} {list(gu.shape)}")
-    dx = torch.empty(x.shape, dtype=torch.bfloat16, device=dev) if need_dx else None
+    dx = _like(x, torch.bfloat16) if need_dx else None
     dw = (torch.empty if M else torch.zeros)(2 * F, K, dtype=torch.bfloat16, device=dev) if need_dw else None
     out = dx, dw[:F] if need_dw else None, dw[F:] if need_dw else None
     if M == 0 or not (need_dx or need_dw):

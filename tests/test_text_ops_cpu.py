@@ -103,6 +103,17 @@ def test_relbias_entry_without_rows(hip_lib):
     assert hip_lib.aether_relbias_attn(None, 4096, None, None, None) == -1
 
 
+def test_relbias_descriptor_bytes():
+    """The packed descriptor has the bytes of the declared structure."""
+    import ctypes as C
+    from aether_amd import _lib
+    arr = (C.c_int * 7)(*range(7))
+    st = (2 ** 40 + 1, 2 ** 33, 64), (5, 6, 7), (8, 9, 10)
+    d = _lib.AetherRelbias(2 ** 47 + 4096, 4112, 4128, *st, 8192, None, 2 ** 35, 3, 65536, 64, -0.125, 32, arr, 7)
+    assert _lib.RELBIAS.size == C.sizeof(d)
+    assert _lib.RELBIAS.pack(2 ** 47 + 4096, 4112, 4128, *st[0], *st[1], *st[2], 8192, 0, 2 ** 35, 3, 65536, 64, -0.125, 32, C.addressof(arr), 7) == bytes(d)
+
+
 def test_bucket_borders():
     """The borders against the published definition evaluated in float64 (away from its own roundings) and by counting."""
     import math
