@@ -335,8 +335,12 @@ __global__ __launch_bounds__(WM * WN * 64) void gated_ff_small_kernel(FfArgs p) 
     }
     const buf_rsrc_t x_rsrc = make_buf_rsrc(p.x, p.x_bytes), g_rsrc = make_buf_rsrc(p.wg, p.w_bytes), u_rsrc = make_buf_rsrc(p.wu, p.w_bytes);
     const int nk = p.K * ES / 128;
-    auto stage = [&](int kt, int buf) {
-        const unsigned soff = 128u * (unsigned)kt;
+    // The K tile that is fetched next.  The column tiles begin at places of their own and wrap around: one K tile of rows that lie a power of two apart is a few
+    // memory channels' work, and all workgroups would ask for the same ones (F = 10240, K = 4096: 48 rows 37.7 -> 36.0 µs, 120 rows 47.7 -> 43.6, 226 58.9 -> 57.7).
+    int at = (int)((long)tile_n * nk / p.tiles_n);
+    auto stage = [&](int buf) {
+        const unsigned soff = 128u * (unsigned)at;
+        at = at == nk - 1 ? 0 : at + 1;
         char* const dst = smem + buf * BUF + wave_s * 1024;
 #pragma unroll
         for (int r = 0; r < W_ROUNDS; ++r) {
@@ -353,15 +357,15 @@ __global__ __launch_bounds__(WM * WN * 64) void gated_ff_small_kernel(FfArgs p) 
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int i = 0; i < 16; ++i) { acc[mt][0][i] = 0.f; acc[mt][1][i] = 0.f; }
-    // a ring of NS buffers; past the last K tile it is fetched again, into a buffer that nobody reads any more, so that the counts of loads stay the same
+    // a ring of NS buffers; past the last K tile the first ones come again, into buffers that nobody reads any more, so that the counts of loads stay the same
     constexpr int PIECES = W_ROUNDS + X_ROUNDS;
 #pragma unroll
-    for (int i = 0; i < NS - 1; ++i) stage(min(i, nk - 1), i);
+    for (int i = 0; i < NS - 1; ++i) stage(i);
     int buf = 0;
     for (int kt = 0; kt < nk; ++kt) {
         wait_vmcnt<(NS - 2) * PIECES>();                              // this wave's part of tile kt has landed
         block_barrier();                                              // everybody's; and tile kt - 1 has been read by all
-        stage(min(kt + NS - 1, nk - 1), buf == 0 ? NS - 1 : buf - 1);
+        stage(buf == 0 ? NS - 1 : buf - 1);
         const char* base = smem + buf * BUF;
         buf = buf == NS - 1 ? 0 : buf + 1;
 #pragma unroll
@@ -466,8 +470,8 @@ static int ff_check(const void* x, long ldx, const void* wg, const void* wu, lon
 
 // Which kernel, from the sizes alone.  A tile kernel runs its workgroups in rounds of one a CU; a round's time is that of one workgroup's K loop, measured per
 // K tile of 128 bytes (K = 4096, F = 1024 ... 10240, µs): 64 x 64 (rows x pairs of columns) 0.42, 128 x 64 0.6, 128 x 128 and 256 x 64 0.9, the 256 x 128
-// kernel with alternating waves 1.45.  The least rounds x time wins; for instance, bf16, F = 10240: 64 rows 37 µs (256 x 128: 91), 128 rows 46 (91), 226 rows
-// 59 (92), 300 rows 65 (96), 400 rows 95 with 256 x 128 (the others 110 and more), 1024 rows 184 (199), 2048 rows 300.
+// kernel with alternating waves 1.45.  The least rounds x time wins; for instance, bf16, F = 10240: 64 rows 36 µs (256 x 128: 91), 128 rows 44 (91), 226 rows
+// 58 (92), 300 rows 64 (96), 400 rows 95 with 256 x 128 (the others 110 and more), 1024 rows 184 (199), 2048 rows 300.
 // The kernel without tiles splits K over its waves and needs no round: up to 32 rows it is ahead where F / 64 workgroups of the smallest tile leave most CUs
 // idle (F = 2048, K = 4096: 1 row 12 µs against 23, 32 rows 18.5 against 23.5; F = 8192, K = 2048: 16 rows 14.5 against 15.3, 32 rows 18.6 against 15.6).
 enum FfVariant { FF_ROWS_16, FF_ROWS_32, FF_64X64, FF_128X64, FF_128X128, FF_256X64, FF_256X128 };
