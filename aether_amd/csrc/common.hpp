@@ -64,6 +64,12 @@ AE_DEV void block_barrier() {
     asm volatile("" ::: "memory");
 }
 
+// a·b rounded, then + c rounded: where results must not depend on whether the compiler joins the two into one fma (fmaf says the opposite)
+AE_DEV float mul_then_add(float a, float b, float c) {
+#pragma clang fp contract(off)
+    return a * b + c;
+}
+
 AE_DEV float wave_sum(float v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);

@@ -91,7 +91,7 @@ __global__ __launch_bounds__(256) void layernorm_modulate_kernel(LnArgs p, int b
 #pragma unroll
             for (int c = 0; c < NCH; ++c)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) { const float d = v[c][e] - mean; sq += d * d; }
+                for (int e = 0; e < 8; ++e) { const float d = v[c][e] - mean; sq = mul_then_add(d, d, sq); }
             const float rstd = rsqrtf(wave_sum(sq) / (float)p.D + p.eps);
             bf16_t* yr = p.y + (size_t)row * p.ldy;
 #pragma unroll
@@ -154,7 +154,7 @@ __global__ __launch_bounds__(256) void gemv_rows_kernel(const float* __restrict_
             for (int e = 0; e < 4; ++e) {
                 float a0 = x0[e], a1 = x1[e];
                 if (act_in == 1) { a0 = silu(a0); a1 = silu(a1); }
-                acc[b] += a0 * wv[e] + a1 * wv[e + 4];
+                acc[b] += e < 3 ? fmaf(a0, wv[e], a1 * wv[e + 4]) : mul_then_add(a0, wv[e], a1 * wv[e + 4]);   // (roundings fixed, see mul_then_add)
             }
         }
     }
@@ -243,7 +243,7 @@ AE_DEV uint4 qk_row(const u16x8 raw, const f32x4 (&nw)[2], const f32x4 (&nb)[2],
     const float mean = sum * (1.0f / 64.0f);
     float sq = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) { const float d = v[e] - mean; sq += d * d; }
+    for (int e = 0; e < 8; ++e) { const float d = v[e] - mean; sq = mul_then_add(d, d, sq); }
     sq += __shfl_xor(sq, 1, 64); sq += __shfl_xor(sq, 2, 64); sq += __shfl_xor(sq, 4, 64);
     const float rstd = rsqrtf(sq * (1.0f / 64.0f) + eps);
 #pragma unroll
@@ -252,8 +252,9 @@ AE_DEV uint4 qk_row(const u16x8 raw, const f32x4 (&nw)[2], const f32x4 (&nb)[2],
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
             const float x0 = v[e], x1 = v[e + 1];
-            v[e] = x0 * cs[e >> 2][e & 3] - x1 * sn[e >> 2][e & 3];
-            v[e + 1] = x1 * cs[(e + 1) >> 2][(e + 1) & 3] + x0 * sn[(e + 1) >> 2][(e + 1) & 3];
+            const float c0 = cs[e >> 2][e & 3], s0 = sn[e >> 2][e & 3], c1 = cs[(e + 1) >> 2][(e + 1) & 3], s1 = sn[(e + 1) >> 2][(e + 1) & 3];
+            v[e] = e == 0 ? mul_then_add(x0, c0, -(x1 * s0)) : fmaf(x0, c0, -(x1 * s0));       // (roundings fixed, see mul_then_add)
+            v[e + 1] = e < 6 ? fmaf(x1, c1, x0 * s1) : fmaf(x0, s1, x1 * c1);
         }
     }
     return make_uint4(pack_bf16x2(v[0] * sc, v[1] * sc), pack_bf16x2(v[2] * sc, v[3] * sc), pack_bf16x2(v[4] * sc, v[5] * sc),

@@ -77,12 +77,16 @@ __global__ __launch_bounds__(GN_PT) void groupnorm_partial_kernel(const unsigned
 #pragma unroll
         for (int u = 0; u < 4; ++u)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) { const float f = bf16_bits_to_f32(raw[u][e]); s[e] += f; q[e] += f * f; }
+            for (int e = 0; e < 8; ++e) {                // (roundings fixed, see mul_then_add)
+                const float f = bf16_bits_to_f32(raw[u][e]);
+                s[e] += f;
+                q[e] = e < 6 ? fmaf(f, f, q[e]) : mul_then_add(f, f, q[e]);
+            }
     }
     for (; v < v1; v += vstep) {
         const u16x8 raw = *(const u16x8*)(base + (size_t)v * C);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) { const float f = bf16_bits_to_f32(raw[e]); s[e] += f; q[e] += f * f; }
+        for (int e = 0; e < 8; ++e) { const float f = bf16_bits_to_f32(raw[e]); s[e] += f; q[e] = fmaf(f, f, q[e]); }
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) { red[tid][e] = s[e]; red[tid][8 + e] = q[e]; }
