@@ -158,8 +158,11 @@ class AetherTextEncoder(nn.Module):
 
     def load_state_dict(self, *args, **kwargs):
         """torch's own: this module's parameter names (checkpoints of T5EncoderModel go through `load_t5_state_dict`)."""
-        self._e4m3 = None
         return super().load_state_dict(*args, **kwargs)
+
+    def _load_from_state_dict(self, *args, **kwargs):        # (a module around this one comes in here)
+        self._e4m3 = None
+        return super()._load_from_state_dict(*args, **kwargs)
 
     # ------------------------------------------------------------------------------------------
     def _embed(self, input_ids, inputs_embeds):
@@ -200,7 +203,7 @@ class AetherTextEncoder(nn.Module):
         F = functional if grad else ops
         linear = functional.linear if grad else ops.gemm_bf16
         eps, heads = c.layer_norm_epsilon, c.num_heads
-        h, delta = h.view(B * S, D), None
+        h, delta = h.reshape(B * S, D), None
         for i, b in enumerate(self.blocks):
             y, h = F.rms_norm(h, b.norm1, eps, delta=delta)
             q, k, v = linear(y, b.qkv).view(B, S, 3, heads, 64).unbind(2)

@@ -64,3 +64,15 @@ def test_demo_flag():
     args = demo.parse_args(["--task", "prediction"])
     assert args.native_text_encoder is False
     assert demo.parse_args(["--task", "prediction", "--native_text_encoder"]).native_text_encoder is True
+
+
+def test_loading_drops_the_eight_bit_copies(hip_lib):
+    """New weights by this module's own load_state_dict, or by that of a module around it: 8-bit copies of the old ones do not stay."""
+    import torch
+    from aether_amd.text_encoder import AetherTextEncoder
+    m = AetherTextEncoder(dict(vocab_size=32, d_model=128, num_heads=2, d_ff=128, num_layers=1), device="cpu")
+    outer = torch.nn.ModuleDict({"text": m})
+    for load in (lambda: m.load_state_dict(m.state_dict()), lambda: outer.load_state_dict(outer.state_dict()), lambda: outer.to(torch.device("cpu"))):
+        m._e4m3 = [()]
+        load()
+        assert m._e4m3 is None

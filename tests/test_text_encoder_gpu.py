@@ -198,6 +198,59 @@ def test_graph(cuda, world):
         assert torch.equal(o1, want1) and torch.equal(o2, want2)
 
 
+def test_embeds_of_any_layout(cuda, world):
+    """One learned prompt expanded over the batch, and embeddings that are a transposed view."""
+    m = world.native_frozen
+    e = torch.randn(1, 9, KW["d_model"], generator=torch.Generator().manual_seed(9)).to(cuda)
+    want = m(inputs_embeds=e.repeat(3, 1, 1))[0]
+    assert torch.equal(m(inputs_embeds=e.expand(3, -1, -1))[0], want)
+    assert torch.equal(m(inputs_embeds=e.repeat(3, 1, 1).transpose(0, 1).contiguous().transpose(0, 1))[0], want)
+    leaf = e.clone().requires_grad_(True)
+    grad, = torch.autograd.grad(m(inputs_embeds=leaf.expand(3, -1, -1))[0].float().sum(), leaf)
+    assert grad.shape == e.shape and bool(torch.isfinite(grad).all())
+
+
+def test_captured_gradients(cuda, hip_lib):
+    """A block's three operators forward and backward, captured with torch.autograd.grad and replayed on other values, eager work in between."""
+    from aether_amd import functional as F
+    B, S, H, D, FF = 2, 70, 2, 128, 128
+    g = torch.Generator().manual_seed(11)
+    new = lambda *shape, s=1.0: (torch.randn(*shape, generator=g) * s).to(cuda)  # noqa: E731
+    values = [new(B * S, D), new(B * S, D).bfloat16(), new(D) + 1, new(3 * H * 64, D, s=0.08).bfloat16(), new(32, H).bfloat16(), new(FF, D, s=0.08).bfloat16(), new(FF, D, s=0.08).bfloat16()]
+    mask = torch.arange(S, device=cuda)[None] < torch.tensor([[S], [33]], device=cuda)
+
+    def step(leaves):
+        x, delta, w, wqkv, table, wg, wu = leaves
+        y, h = F.rms_norm(x, w, delta=delta)
+        q, k, v = F.linear(y, wqkv).view(B, S, 3, H, 64).unbind(2)
+        o = F.relbias_attn(q, k, v, table, key_mask=mask).view(B * S, H * 64)
+        y, h = F.rms_norm(h, w, delta=o)
+        out = F.gated_ff(y, wg, wu)
+        return torch.autograd.grad([out, h], leaves, [out.detach(), h.detach()])
+
+    def fresh():
+        return [t.clone().requires_grad_(True) for t in values]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(fresh())
+    torch.cuda.current_stream().wait_stream(side)
+    leaves = fresh()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(leaves)
+    for n in range(3):
+        with torch.no_grad():
+            for t, leaf in zip(values, leaves):
+                t.mul_(-0.9)
+                leaf.copy_(t)
+        graph.replay()
+        want = step(fresh())
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), n
+
+
 def test_pipeline_slot(cuda, hip_lib, world):
     """The pipeline's `encode_prompt` on the native encoder: the empty prompt at construction and any other."""
     from aether_amd.pipelines.aetherv1_pipeline_cogvideox import AetherV1PipelineCogVideoX
