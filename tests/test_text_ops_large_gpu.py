@@ -1,0 +1,111 @@
+"""The text encoder's operators at the largest lengths and with offsets beyond 32 bits, against float64 (rows and keys that are picked out)."""
+import math
+
+import pytest
+import torch
+
+from relbias_reference import bucket
+
+pytestmark = pytest.mark.gpu
+BF16, S32 = 2.0 ** -8, 2.0 ** -10
+
+
+def test_attention_at_its_longest(cuda, hip_lib):
+    """S = 65536.  Bounds as in test_relbias_attn_gpu.py and test_relbias_attn_backward_gpu.py: o of every row, dq, dk and dv of some."""
+    from aether_amd import ops
+    S = 65536
+    g = torch.Generator().manual_seed(1)
+    qkv = torch.randn(1, S, 3, 1, 64, generator=g)
+    qkv[:, :, :2] *= math.sqrt(0.5)
+    qkv = qkv.to(torch.bfloat16).to(cuda)
+    table = (torch.randn(32, 1, generator=g) * 2).to(torch.bfloat16).to(cuda)
+    do = torch.randn(1, S, 1, 64, generator=g).to(torch.bfloat16).to(cuda)
+    mask = torch.ones(1, S, dtype=torch.bool, device=cuda)
+    mask[0, 30000:41000] = False
+    mask[0, -3:] = False
+    q, k, v = qkv.unbind(2)
+    o, lse = ops.relbias_attn(q, k, v, table, key_mask=mask, need_lse=True)
+    dq, dk, dv, dtable = ops.relbias_attn_backward(do, q, k, v, o, lse, table, key_mask=mask)
+    assert not dk[0, 30000:41000].any() and not dv[0, 30000:41000].any()
+
+    qd, kd, vd, gd = (t[0, :, 0].double() for t in (q, k, v, do))
+    of = torch.tensor([bucket(d, 32, 128) for d in range(-200, 201)], device=cuda)
+    td = table[:, 0].double()
+    at = torch.arange(S, device=cuda)
+    rows = torch.tensor([0, 1, 63, 64, 8191, 29999, 30000, 40999, 65532, 65535], device=cuda)
+    keys = torch.tensor([0, 1, 127, 128, 16384, 29999, 41000, 65472, 65532], device=cuda)
+    want = {n: torch.zeros(len(keys), 64, dtype=torch.float64, device=cuda) for n in ("dk", "dv", "lk", "lv")}
+    for at0 in range(0, S, 1024):
+        i = at[at0:at0 + 1024]
+        s = (qd[i] @ kd.t().contiguous()) + td[of[(at[None, :] - i[:, None]).clamp(-200, 200) + 200]]
+        s.masked_fill_(~mask, -math.inf)
+        p = torch.softmax(s, -1)
+        T = p @ vd.abs()
+        oo = p @ vd
+        err = (o[0, i, 0].double() - oo).abs()
+        assert bool((err <= (BF16 + S32) * T + BF16 * oo.abs()).all()), at0
+        delta = (gd[i] * oo).sum(-1, keepdim=True)
+        D = (gd[i].abs() * (2.0 ** -16 + S32) * T).sum(-1, keepdim=True)
+
+        def ds_of(p, j):
+            dP, dPa = gd[i] @ vd[j].t().contiguous(), gd[i].abs() @ vd[j].abs().t().contiguous()
+            ds = p * (dP - delta)
+            return ds, p * (S32 * (dP.abs() + delta.abs()) + D + 66 * 2.0 ** -24 * dPa) + BF16 * ds.abs()
+
+        pj = p[:, keys]
+        ds, E = ds_of(pj, keys)
+        want["dk"] += ds.t().contiguous() @ qd[i]
+        want["lk"] += E.t().contiguous() @ qd[i].abs()
+        want["dv"] += pj.t().contiguous() @ gd[i]
+        want["lv"] += (BF16 + S32) * (pj.t().contiguous() @ gd[i].abs())
+        for r in rows[(rows >= at0) & (rows < at0 + 1024)].tolist():
+            ds, E = ds_of(p, at)
+            x, lim = ds[r - at0] @ kd, E[r - at0] @ kd.abs()
+            assert bool(((dq[0, r, 0].double() - x).abs() <= lim + BF16 * x.abs()).all()), r
+    for n, got in (("k", dk), ("v", dv)):
+        x = want["d" + n]
+        assert bool(((got[0, keys, 0].double() - x).abs() <= want["l" + n] + BF16 * x.abs()).all()), n
+    assert bool(torch.isfinite(dtable.float()).all())
+
+
+def test_batch_items_far_apart(cuda, hip_lib):
+    """The second item begins more than 4 GiB behind the first: the same bits as from packed operands."""
+    from aether_amd import ops
+    S, H, far = 130, 2, (2 ** 32 + 4096) // 2 + 8 * 1000
+    g = torch.Generator().manual_seed(2)
+    qkv = torch.randn(2, S, 3, H, 64, generator=g).to(torch.bfloat16).to(cuda)
+    table = torch.randn(32, H, generator=g).to(torch.bfloat16).to(cuda)
+    store = torch.empty(far + S * 3 * H * 64, dtype=torch.bfloat16, device=cuda)
+    wide = store.as_strided(qkv.shape, (far, *qkv.stride()[1:]))
+    wide.copy_(qkv)
+    do = torch.randn(2, S, H, 64, generator=g).to(torch.bfloat16).to(cuda)
+    out = []
+    for t in (qkv, wide):
+        q, k, v = t.unbind(2)
+        o, lse = ops.relbias_attn(q, k, v, table, need_lse=True)
+        out.append([o, *ops.relbias_attn_backward(do, q, k, v, o, lse, table)])
+    assert all(torch.equal(a, b) for a, b in zip(*out))
+
+
+def test_rows_far_apart(cuda, hip_lib):
+    """Rows of one tensor over more than 4 GiB: the norm and its gradients, and the feed-forward, which goes through them in several launches."""
+    from aether_amd import ops
+    g = torch.Generator().manual_seed(3)
+    M, D, F = 600, 128, 96
+    step = 4 * 2 ** 20                                       # 8 MiB between rows: 600 rows over 4.7 GiB
+    x = torch.randn(M, D, generator=g).to(torch.bfloat16).to(cuda)
+    wide = torch.empty(M * step, dtype=torch.bfloat16, device=cuda).as_strided((M, D), (step, 1))
+    wide.copy_(x)
+    w = torch.randn(D, generator=g).to(cuda)
+    assert all(torch.equal(a, b) for a, b in zip(ops.rms_norm(wide, w, delta=x), ops.rms_norm(x, w, delta=x)))
+    dy = torch.randn(M, D, generator=g).to(torch.bfloat16).to(cuda)
+    assert all(torch.equal(a, b) for a, b in zip(ops.rms_norm_backward(dy, wide, w, need_ddelta=True), ops.rms_norm_backward(dy, x, w, need_ddelta=True)))
+    wg, wu = (torch.randn(F, D, generator=g).to(torch.bfloat16).to(cuda) for _ in range(2))
+    h, gu = ops.gated_ff(wide, wg, wu, need_gu=True)
+    parts = [ops.gated_ff(x[m:m + 256], wg, wu, need_gu=True) for m in range(0, M, 256)]
+    want = torch.cat([p[0] for p in parts])
+    # a launch of other sizes may take another tile, and K in another order: fp32 sums of 128 products on both sides (|act'| < 1.2), one rounding to bf16 each
+    A = [(x.float().abs() @ t.float().abs().t().contiguous()) for t in (wg, wu)]
+    lim = 2 * BF16 * want.float().abs() + 2 * 128 * 2.0 ** -24 * (1.2 * A[0] * gu[:, F:].abs() + A[1] * gu[:, :F].abs())
+    assert bool(((h.float() - want.float()).abs() <= lim).all())
+    assert all(torch.equal(a, b) for a, b in zip(ops.gated_ff_backward(h, wide, wg, wu, gu), ops.gated_ff_backward(h, x, wg, wu, gu)))
