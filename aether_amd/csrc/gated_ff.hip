@@ -11,15 +11,16 @@
 // waves that share a SIMD alternate: one reads its next fragments and issues the next tile's DMA while the other feeds the matrix pipe.
 // Measured, F = 10240, K = 4096: 14464 rows in e4m3 940 µs, 2580 TFLOP/s (a large library product in 8 bits: 2440); 3616 rows in bf16, writing both projections,
 // 620 ... 660 µs, 940 TFLOP/s (library 1390; of these, 75 µs are the projections' 296 MB).
+#include <algorithm>
 #include <type_traits>
 #include "common.hpp"
+#include "turned_tile.hpp"
 #include "../../include/aether_hip.h"
 
 namespace aether {
 
 typedef unsigned char u8_t;
 typedef int i32x8 __attribute__((ext_vector_type(8)));
-typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 struct FfArgs {
     const void* x; long ldx;             // elements
@@ -459,6 +460,150 @@ __global__ __launch_bounds__(256) void transpose_bf16_kernel(const bf16_t* __res
     }
 }
 
+// dx = [dg du] [Wg; Wu] for few rows, without turned copies of the weights: dx[m][c] = Σ_r dgu[m][r] W[r][c], r < F in Wg, the rest in Wu.  The weights' tile, 64 rows
+// of BC columns, goes into LDS as it lies in memory and is read transposed; dgu's rows are read as they are.  The sum over r is split over workgroups so
+// that all CUs work; their parts, in fp32, are added in order by ff_dx_join_kernel.  Bound by reading the weights: F = 10240, K = 4096, 60 rows 29 µs for
+// 168 MB (and 6 to join), 226 rows 56 (and 6).
+struct FfDxArgs {
+    const bf16_t* dgu;                   // [M][2F]
+    const bf16_t *wg, *wu; long ldw;
+    bf16_t* dx; long lddx;
+    float* part;                         // [splits][M][K], or null: dx itself
+    int M, F, K, tiles_m, tiles_c, splits;
+    unsigned dgu_bytes, w_bytes;
+};
+template <int WM, int WC, int MT, int CT>
+__global__ __launch_bounds__(WM * WC * 64) void gated_ff_dx_kernel(FfDxArgs p) {
+    constexpr int NW = WM * WC, NS = 3, BM = WM * MT * 32, BC = WC * CT * 32;
+    constexpr int G_TILE = BM * 128, W_TILE = BC * 128, BUF = G_TILE + W_TILE;
+    constexpr int G_ROUNDS = BM / 8 / NW, W_ROUNDS = BC / 8 / NW;
+    static_assert(BM % (8 * NW) == 0 && BC % (8 * NW) == 0 && BC % 64 == 0 && NW % 2 == 0, "whole wave-instructions");
+    extern __shared__ __attribute__((aligned(16))) char smem_dx[];
+    char* const smem = smem_dx;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5, l32 = lane & 31;
+    const int wave_s = __builtin_amdgcn_readfirstlane(wave), wm = wave_s / WC, wc = wave_s % WC;
+    const int id = xcd_remap((int)blockIdx.x, p.tiles_m * p.tiles_c * p.splits);
+    const int tile_m = id % p.tiles_m, rest = id / p.tiles_m;         // the row tiles of one piece of the weights one after the other
+    const int tile_c = rest % p.tiles_c, split = rest / p.tiles_c;
+    const int m0 = tile_m * BM, c0 = tile_c * BC;
+    const int steps = p.F / 32;                                       // of 64 rows of [Wg; Wu]
+    const int from = (int)((long)steps * split / p.splits), to = (int)((long)steps * (split + 1) / p.splits);
+    const i32x4 g_rsrc = tt_rsrc(p.dgu, p.dgu_bytes), wg_rsrc = tt_rsrc(p.wg, p.w_bytes), wu_rsrc = tt_rsrc(p.wu, p.w_bytes);
+    unsigned g_off[G_ROUNDS], w_off[W_ROUNDS];
+#pragma unroll
+    for (int r = 0; r < G_ROUNDS; ++r) {
+        const int row = (r * NW + wave) * 8 + (lane >> 3);
+        g_off[r] = (unsigned)min(m0 + row, p.M - 1) * (unsigned)(p.F * 4) + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
+    }
+#pragma unroll
+    for (int r = 0; r < W_ROUNDS; ++r) {                              // piece r NW + wave: 8 rows of 64 columns; columns behind the last ones repeat them
+        const int piece = r * NW + wave, row = (piece & 7) * 8 + (lane >> 3);
+        w_off[r] = (unsigned)(lane >> 3) * (unsigned)(p.ldw * 2) + (unsigned)min(c0 + (piece >> 3) * 64, p.K - 64) * 2 + (((lane & 7) ^ tt_swz(row)) << 4);
+    }
+    auto stage = [&](int step, int buf) __attribute__((always_inline)) {
+        const int s = min(step, to - 1);                              // past the last one it is fetched again, into a buffer that nobody reads any more
+        const unsigned dst = tt_lds(smem) + buf * BUF + wave_s * 1024;
+#pragma unroll
+        for (int r = 0; r < W_ROUNDS; ++r) {
+            const int row = s * 64 + ((r * NW + wave_s) & 7) * 8;     // (F is a multiple of 32: eight rows are of one of the two)
+            const bool up = row >= p.F;
+            tt_dma16(up ? wu_rsrc : wg_rsrc, w_off[r], (unsigned)(up ? row - p.F : row) * (unsigned)(p.ldw * 2), dst + G_TILE + r * (NW * 1024));
+        }
+#pragma unroll
+        for (int r = 0; r < G_ROUNDS; ++r) tt_dma16(g_rsrc, g_off[r], (unsigned)s * 128u, dst + r * (NW * 1024));
+    };
+    int toff[2][2];
+    tt_offsets(lane, toff);
+    const int g_row = (wm * MT * 32 + l32) * 128, swz = (lane >> 1) & 7;
+    f32x16 acc[CT][MT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[ct][mt][i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NS - 1; ++i) stage(from + i, i);
+    int buf = 0;
+    for (int step = from; step < to; ++step) {
+        wait_vmcnt<(NS - 2) * (G_ROUNDS + W_ROUNDS)>();               // this wave's part of the tile has landed
+        block_barrier();                                              // everybody's; and the tile before it has been read by all
+        stage(step + NS - 1, buf == 0 ? NS - 1 : buf - 1);
+        const char* const base = smem + buf * BUF;
+        buf = buf == NS - 1 ? 0 : buf + 1;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            bf16x8 w[CT], g[MT];
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+                const int col = wc * CT + ct;                         // of 32 columns
+                const char* const at = base + G_TILE + (col >> 1) * 8192 + 2048 * s;
+                if constexpr (CT == 2) w[ct] = tt_read(at, toff[ct]);
+                else {
+                    const int off[2] = {wc & 1 ? toff[1][0] : toff[0][0], wc & 1 ? toff[1][1] : toff[0][1]};
+                    w[ct] = tt_read(at, off);
+                }
+            }
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) g[mt] = *(const bf16x8*)(base + g_row + mt * 4096 + (((2 * s + hi) ^ swz) << 4));
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) acc[ct][mt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[ct], g[mt], acc[ct][mt], 0, 0, 0);
+        }
+        wait_lgkmcnt0();
+    }
+    wait_vmcnt<0>();                                                  // nothing arrives in LDS behind the workgroup's end
+    // acc[ct][mt][r]: row m of dx, column 8(r >> 2) + 4hi + (r & 3) of 32
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+        const int c = c0 + (wc * CT + ct) * 32;
+        if (c >= p.K) continue;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            const int m = m0 + (wm * MT + mt) * 32 + l32;
+            if (m >= p.M) continue;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const f32x4 v = {acc[ct][mt][4 * q], acc[ct][mt][4 * q + 1], acc[ct][mt][4 * q + 2], acc[ct][mt][4 * q + 3]};
+                if (p.part) *(f32x4*)(p.part + ((size_t)split * p.M + m) * p.K + c + 8 * q + 4 * hi) = v;
+                else *(uint2*)(p.dx + (size_t)m * p.lddx + c + 8 * q + 4 * hi) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+            }
+        }
+    }
+}
+
+__global__ __launch_bounds__(256) void ff_dx_join_kernel(const float* __restrict__ part, int splits, int M, int K, bf16_t* __restrict__ dx, long lddx) {
+    const size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4, n = (size_t)M * K;
+    if (i >= n) return;
+    f32x4 a = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < splits; s0 += 8) {                          // eight loads on their way together
+        f32x4 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = *(const f32x4*)(part + min(s0 + k, splits - 1) * n + i);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (s0 + k < splits) a += v[k];
+    }
+    const size_t m = i / K, c = i - m * K;
+    *(uint2*)(dx + m * lddx + c) = make_uint2(pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]));
+}
+
+// rows of the tile: few rows a small one; the split that fills the CUs (two workgroups of the smallest tile fit one), as far as the parts fit the place of the
+// turned weights
+// Against a large product on turned copies of the weights (F = 10240, K = 4096, µs, copies included): 226 rows 62 against 505, 1800 rows 339 against 505, 3616 rows
+// 631 against 560.  This kernel's tiles are half as wide, so it stays as long as they need one round of the CUs.
+static bool ff_dx_direct(int M, int K) { return (long)((M + 255) / 256) * ((K + 127) / 128) <= 256; }
+struct FfDxPlan { int rows, splits; };
+static FfDxPlan ff_dx_plan(int M, int F, int K) {
+    FfDxPlan q;
+    q.rows = M <= 64 ? 64 : M <= 128 ? 128 : 256;
+    const long tiles = (long)((M + q.rows - 1) / q.rows) * ((K + 127) / 128), want = q.rows == 64 ? 512 : 256;
+    const long most = std::max(1l, std::min({(long)F / M, (long)F / 32 / 4, 64l}));
+    q.splits = (int)std::min(most, std::max(1l, want / tiles));
+    return q;
+}
+
 static int ff_check(const void* x, long ldx, const void* wg, const void* wu, long ldw, int M, int F, int K, int act, int size) {
     if (act != ACT_GELU_TANH && act != ACT_SILU) return aether_set_error(AETHER_ERR_ARG, "gated_ff: unknown activation");
     if (M < 0 || F <= 0 || K <= 0) return aether_set_error(AETHER_ERR_SHAPE, "gated_ff: M must not be negative, F and K must be positive");
@@ -608,7 +753,30 @@ extern "C" int aether_gated_ff_bwd(const void* dh, long lddh, const void* x, lon
     if (act == ACT_SILU) hipLaunchKernelGGL((gated_ff_dgu_kernel<ACT_SILU>), eg, dim3(256), 0, s, gu, (const bf16_t*)dh, lddh, M, F, (int)Mp, dgu, dgut);
     else hipLaunchKernelGGL((gated_ff_dgu_kernel<ACT_GELU_TANH>), eg, dim3(256), 0, s, gu, (const bf16_t*)dh, lddh, M, F, (int)Mp, dgu, dgut);
     rc = aether_check_launch("gated_ff_bwd");
-    if (!rc && dx) {
+    if (!rc && dx && ff_dx_direct(M, K)) {
+        const FfDxPlan plan = ff_dx_plan(M, F, K);
+        FfDxArgs a = {dgu, (const bf16_t*)wg, (const bf16_t*)wu, ldw, (bf16_t*)dx, lddx, plan.splits > 1 ? (float*)wt : nullptr, M, F, K, (M + plan.rows - 1) / plan.rows, (K + 127) / 128,
+                      plan.splits, (unsigned)((size_t)M * 4 * F), (unsigned)(((size_t)(F - 1) * ldw + K) * 2)};
+        const dim3 grid((unsigned)((long)a.tiles_m * a.tiles_c * a.splits));
+#define FF_DX(WM, WC, MT, CT)                                                                                                          \
+    do {                                                                                                                               \
+        constexpr int LDS = 3 * (WM * MT * 32 + WC * CT * 32) * 128;                                                                   \
+        if (hipFuncSetAttribute((const void*)gated_ff_dx_kernel<WM, WC, MT, CT>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) { \
+            (void)hipGetLastError();                                                                                                   \
+            return aether_set_error(AETHER_ERR_LAUNCH, "gated_ff_bwd: the workgroup's LDS could not be set");                          \
+        }                                                                                                                              \
+        hipLaunchKernelGGL((gated_ff_dx_kernel<WM, WC, MT, CT>), grid, dim3(WM * WC * 64), LDS, s, a);                                 \
+    } while (0)
+        if (plan.rows == 64) FF_DX(1, 4, 2, 1);
+        else if (plan.rows == 128) FF_DX(2, 2, 2, 2);
+        else FF_DX(4, 2, 2, 2);
+#undef FF_DX
+        rc = aether_check_launch("gated_ff_dx");
+        if (!rc && plan.splits > 1) {
+            hipLaunchKernelGGL(ff_dx_join_kernel, dim3((unsigned)(((size_t)M * K / 4 + 255) / 256)), dim3(256), 0, s, (const float*)wt, plan.splits, M, K, (bf16_t*)dx, lddx);
+            rc = aether_check_launch("ff_dx_join");
+        }
+    } else if (!rc && dx) {
         hipLaunchKernelGGL(transpose_bf16_kernel, dim3((K + 63) / 64, (F + 63) / 64), dim3(256), 0, s, (const bf16_t*)wg, ldw, F, K, wt, 2 * (long)F, F);
         hipLaunchKernelGGL(transpose_bf16_kernel, dim3((K + 63) / 64, (F + 63) / 64), dim3(256), 0, s, (const bf16_t*)wu, ldw, F, K, wt + F, 2 * (long)F, F);
         rc = aether_check_launch("gated_ff_bwd (weights turned)");

@@ -58,24 +58,24 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(PIPE ||
     }
     // ---- staging: a wave-instruction moves 8 rows x 128 bytes; rows at or beyond S are outside the descriptor and their keys do not count ----
     const unsigned k_row = (unsigned)p.k.ss * 2, v_row = (unsigned)p.v.ss * 2;
-    const i32x4 k_rsrc = rb_rsrc(p.k.p + (size_t)b * p.k.sb + (size_t)h * p.k.sh, (unsigned)(S - 1) * k_row + 128);
-    const i32x4 v_rsrc = rb_rsrc(p.v.p + (size_t)b * p.v.sb + (size_t)h * p.v.sh, (unsigned)(S - 1) * v_row + 128);
+    const i32x4 k_rsrc = tt_rsrc(p.k.p + (size_t)b * p.k.sb + (size_t)h * p.k.sh, (unsigned)(S - 1) * k_row + 128);
+    const i32x4 v_rsrc = tt_rsrc(p.v.p + (size_t)b * p.v.sb + (size_t)h * p.v.sh, (unsigned)(S - 1) * v_row + 128);
     unsigned k_off[8 / NW], v_off[8 / NW];
 #pragma unroll
     for (int ps = 0; ps < 8 / NW; ++ps) {
         const int r = (ps * NW + wave) * 8 + (lane >> 3), ch = lane & 7;
-        k_off[ps] = r * k_row + ((ch ^ rb_swz(r)) << 4);
-        v_off[ps] = r * v_row + ((ch ^ rb_swz(r)) << 4);
+        k_off[ps] = r * k_row + ((ch ^ tt_swz(r)) << 4);
+        v_off[ps] = r * v_row + ((ch ^ tt_swz(r)) << 4);
     }
     auto stage_k = [&](int j, int buf) {
-        const unsigned dst = rb_lds(smem) + buf + wave_s * 1024;
+        const unsigned dst = tt_lds(smem) + buf + wave_s * 1024;
 #pragma unroll
-        for (int ps = 0; ps < 8 / NW; ++ps) rb_dma16(k_rsrc, k_off[ps], (unsigned)j * (RB_KV * k_row), dst + ps * (NW * 1024));
+        for (int ps = 0; ps < 8 / NW; ++ps) tt_dma16(k_rsrc, k_off[ps], (unsigned)j * (RB_KV * k_row), dst + ps * (NW * 1024));
     };
     auto stage_v = [&](int j, int buf) {
-        const unsigned dst = rb_lds(smem) + buf + RB_TILE + wave_s * 1024;
+        const unsigned dst = tt_lds(smem) + buf + RB_TILE + wave_s * 1024;
 #pragma unroll
-        for (int ps = 0; ps < 8 / NW; ++ps) rb_dma16(v_rsrc, v_off[ps], (unsigned)j * (RB_KV * v_row), dst + ps * (NW * 1024));
+        for (int ps = 0; ps < 8 / NW; ++ps) tt_dma16(v_rsrc, v_off[ps], (unsigned)j * (RB_KV * v_row), dst + ps * (NW * 1024));
     };
     auto stage = [&](int j, int buf) {
         stage_k(j, buf);
@@ -88,7 +88,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(PIPE ||
     if (p.mask) rb_fill_words(p.mask + (size_t)b * p.mask_sb, S, words8, NW * 64);
     int koff[4], voff[2][2];
     rb_row_offsets(lane, koff);
-    rb_tr_offsets(lane, voff);
+    tt_offsets(lane, voff);
 
     f32x16 o[2];
 #pragma unroll
@@ -233,7 +233,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(PIPE ||
             };
             half(std::integral_constant<int, 0>{});
             half(std::integral_constant<int, 1>{});
-            rb_tiles_landed();                                            // tile j1, issued one tile ago
+            tt_landed();                                            // tile j1, issued one tile ago
             if (j2 < nkv) stage(j2, rb_next(rb_next(buf)));               // its buffer was last read before the previous barrier
             rb_reads_done_barrier();
             j = j1; w = w1;
@@ -324,7 +324,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(PIPE ||
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                vc[i >> 1][i & 1] = rb_read_tr1(smem + kb + VO + 2048 * (i >> 1), voff[i & 1]);      // for the second half of the iteration
+                vc[i >> 1][i & 1] = tt_read(smem + kb + VO + 2048 * (i >> 1), voff[i & 1]);      // for the second half of the iteration
                 kc[i] = *(const bf16x8*)(smem + kb1 + KO + koff[i]);
                 scores(i, ka[i], x1);
                 soft(2 * i, x0, p0, l0, add, near_tag);
@@ -337,7 +337,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(PIPE ||
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                va[i >> 1][i & 1] = rb_read_tr1(smem + kb + VO + 4096 + 2048 * (i >> 1), voff[i & 1]);   // for the next iteration's first half
+                va[i >> 1][i & 1] = tt_read(smem + kb + VO + 4096 + 2048 * (i >> 1), voff[i & 1]);   // for the next iteration's first half
                 ka[i] = *(const bf16x8*)(smem + kb1 + KO + 4096 + koff[i]);
                 product(i, vc, p0, l0);
                 soft(2 * i, x1, p1, l1, add, near_tag);

@@ -2,6 +2,7 @@
 // of a tile.
 #pragma once
 #include "common.hpp"
+#include "turned_tile.hpp"
 
 namespace aether {
 
@@ -80,25 +81,6 @@ AE_DEV uint64_t rb_word(const RbArgs& p, const uint64_t* words, int j) {
     return left >= 64 ? ~0ull : (1ull << left) - 1;
 }
 
-// 16-byte LDS-DMA as in common.hpp (LDS destination: wave-uniform base + lane · 16; bytes beyond the descriptor are not fetched), in assembly: the compiler
-// waits for every LDS-DMA it knows of before a transposing LDS read, the next tile's included.  The loops wait for their tiles themselves.
-typedef int i32x4 __attribute__((ext_vector_type(4)));
-AE_DEV i32x4 rb_rsrc(const void* base, unsigned bytes) {
-    const uint64_t a = (uint64_t)base;
-    return i32x4{__builtin_amdgcn_readfirstlane((int)(unsigned)a), __builtin_amdgcn_readfirstlane((int)(unsigned)(a >> 32) & 0xffff), __builtin_amdgcn_readfirstlane((int)bytes), 0x00020000};
-}
-AE_DEV unsigned rb_lds(const void* p) { return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) char*)p; }
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"       // (that m0 is not preserved is what is meant)
-AE_DEV void rb_dma16(i32x4 rsrc, unsigned voff, unsigned soff, unsigned lds_wave_base) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds_wave_base), "v"(voff), "s"(rsrc), "s"(soff) : "memory", "m0");
-}
-#pragma clang diagnostic pop
-
-// A 64 x 64 tile in LDS: 128-byte rows, the 16-byte chunk c of row r stands at c ^ swz(r).  swz takes all eight values over r's bits 1 ... 3, so that 32 rows
-// read at one chunk spread over the banks; and rows r, r + 2 differ in its bit 1, so that the 4 x 32-byte pieces of a transposing read do too.
-AE_DEV int rb_swz(int r) { return (((r >> 1) & 3) << 1) | ((r >> 3) & 1); }
-
 // the row of a 32-row half that feeds MFMA row i: the 16 results of a lane are then rows 16(r >> 3) + 8hi + (r & 7), in register order the B operand
 // of a product over these rows
 AE_DEV int rb_pi(int i) { return 16 * (i >> 4) + 8 * ((i >> 2) & 1) + 4 * ((i >> 3) & 1) + (i & 3); }
@@ -107,18 +89,7 @@ AE_DEV int rb_pi(int i) { return 16 * (i >> 4) + 8 * ((i >> 2) & 1) + 4 * ((i >>
 AE_DEV void rb_row_offsets(int lane, int (&off)[4]) {
     const int r = rb_pi(lane & 31), hi = lane >> 5;
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) off[ks] = r * 128 + (((2 * ks + hi) ^ rb_swz(r)) << 4);
-}
-// offsets of a lane's transposed fragments: column 32 dt + (lane & 31), rows 8hi + 4f ... + 3 of 16; 16 rows further the swizzle is the same
-AE_DEV void rb_tr_offsets(int lane, int (&off)[2][2]) {
-    const int i = lane & 15, hi = lane >> 5;
-#pragma unroll
-    for (int dt = 0; dt < 2; ++dt)
-#pragma unroll
-        for (int f = 0; f < 2; ++f) {
-            const int r = 8 * hi + 4 * f + (i >> 2), chunk = dt * 4 + ((lane >> 4) & 1) * 2 + ((i & 3) >> 1);
-            off[dt][f] = r * 128 + ((chunk ^ rb_swz(r)) << 4) + (i & 1) * 8;
-        }
+    for (int ks = 0; ks < 4; ++ks) off[ks] = r * 128 + (((2 * ks + hi) ^ tt_swz(r)) << 4);
 }
 // Makes the wait for a fragment's loads happen here.  Left to its first use inside a loop, the compiler counts it together with the loop's own tile loads
 // and waits for those too.
@@ -156,27 +127,18 @@ AE_DEV void rb_store(const f32x16 (&o)[2], float f, bf16_t* row, int hi, bool ok
     }
 }
 
-// One transposed fragment: 16 rows from `at`, columns by off (rb_tr_offsets of a 32-column half)
-AE_DEV bf16x8 rb_read_tr1(const char* at, const int (&off)[2]) {
-    typedef short s16x4 __attribute__((ext_vector_type(4)));
-    typedef short s16x8 __attribute__((ext_vector_type(8)));
-    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + off[0]));
-    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + off[1]));
-    return __builtin_bit_cast(bf16x8, s16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]});
-}
 // The transposed fragments of 32 rows of a tile: f[s][dt] holds column 32 dt + (lane & 31), rows 16 s + 8hi ... + 7.  The transposing LDS read moves a 4 x 16 piece
 // per 16 lanes: lane 4r + c names row r, elements 4c ... 4c + 3, and lane i receives column i.
 AE_DEV void rb_read_tr(bf16x8 (&f)[2][2], const char* at, const int (&off)[2][2]) {
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
-        for (int dt = 0; dt < 2; ++dt) f[s][dt] = rb_read_tr1(at + 2048 * s, off[dt]);
+        for (int dt = 0; dt < 2; ++dt) f[s][dt] = tt_read(at + 2048 * s, off[dt]);
 }
 
 // Three buffers of two tiles: while one is worked on, the next one is complete or arriving, and the one after it is issued.
 constexpr int RB_RING = 3 * RB_BUF;
 AE_DEV int rb_next(int buf) { return buf == 2 * RB_BUF ? 0 : buf + RB_BUF; }   // buffers by their offsets
-AE_DEV void rb_tiles_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 AE_DEV void rb_reads_done_barrier() {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();

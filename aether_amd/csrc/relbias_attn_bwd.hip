@@ -87,21 +87,21 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     const float lse = qrow < S ? args.lse[(size_t)bh * S + qc] : INFINITY;   // rows behind the last one: P = 0, they add nothing to dT
 
     const unsigned k_row = (unsigned)p.k.ss * 2, v_row = (unsigned)p.v.ss * 2;
-    const i32x4 k_rsrc = rb_rsrc(p.k.p + (size_t)b * p.k.sb + (size_t)h * p.k.sh, (unsigned)(S - 1) * k_row + 128);
-    const i32x4 v_rsrc = rb_rsrc(p.v.p + (size_t)b * p.v.sb + (size_t)h * p.v.sh, (unsigned)(S - 1) * v_row + 128);
+    const i32x4 k_rsrc = tt_rsrc(p.k.p + (size_t)b * p.k.sb + (size_t)h * p.k.sh, (unsigned)(S - 1) * k_row + 128);
+    const i32x4 v_rsrc = tt_rsrc(p.v.p + (size_t)b * p.v.sb + (size_t)h * p.v.sh, (unsigned)(S - 1) * v_row + 128);
     unsigned k_off[8 / NW], v_off[8 / NW];
 #pragma unroll
     for (int ps = 0; ps < 8 / NW; ++ps) {
         const int r = (ps * NW + wave) * 8 + (lane >> 3), ch = lane & 7;
-        k_off[ps] = r * k_row + ((ch ^ rb_swz(r)) << 4);
-        v_off[ps] = r * v_row + ((ch ^ rb_swz(r)) << 4);
+        k_off[ps] = r * k_row + ((ch ^ tt_swz(r)) << 4);
+        v_off[ps] = r * v_row + ((ch ^ tt_swz(r)) << 4);
     }
     auto stage = [&](int j, int buf) __attribute__((always_inline)) {
-        const unsigned dst = rb_lds(smem) + buf + wave_s * 1024;
+        const unsigned dst = tt_lds(smem) + buf + wave_s * 1024;
 #pragma unroll
         for (int ps = 0; ps < 8 / NW; ++ps) {
-            rb_dma16(k_rsrc, k_off[ps], (unsigned)j * (RB_KV * k_row), dst + ps * (NW * 1024));
-            rb_dma16(v_rsrc, v_off[ps], (unsigned)j * (RB_KV * v_row), dst + RB_TILE + ps * (NW * 1024));
+            tt_dma16(k_rsrc, k_off[ps], (unsigned)j * (RB_KV * k_row), dst + ps * (NW * 1024));
+            tt_dma16(v_rsrc, v_off[ps], (unsigned)j * (RB_KV * v_row), dst + RB_TILE + ps * (NW * 1024));
         }
     };
     const int nkv = (S + RB_KV - 1) / RB_KV;
@@ -113,7 +113,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
         for (int i = tid; i < tab_bytes / 4 * 2 * NW; i += NW * 64) hist[i] = 0.f;
     int roff[4], toff[2][2];
     rb_row_offsets(lane, roff);
-    rb_tr_offsets(lane, toff);
+    tt_offsets(lane, toff);
 
     rb_arrived(qf);
     rb_arrived(gf);
@@ -178,8 +178,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
             constexpr int i = decltype(i_tag)::value;
             if constexpr (i < 16) return *(const bf16x8*)(base + (i & 1) * RB_TILE + (i >> 3) * 4096 + roff[(i >> 1) & 3]);
             else if constexpr (PART)
-                return rb_keep(rb_read_tr1(base + ((i >> 2) & 1) * 4096 + 2048 * ((i >> 1) & 1), toff[i & 1]), (unsigned)(w >> (32 * ((i >> 2) & 1) + 16 * ((i >> 1) & 1) + 8 * hi)) & 0xffu);
-            else return rb_read_tr1(base + ((i >> 2) & 1) * 4096 + 2048 * ((i >> 1) & 1), toff[i & 1]);
+                return rb_keep(tt_read(base + ((i >> 2) & 1) * 4096 + 2048 * ((i >> 1) & 1), toff[i & 1]), (unsigned)(w >> (32 * ((i >> 2) & 1) + 16 * ((i >> 1) & 1) + 8 * hi)) & 0xffu);
+            else return tt_read(base + ((i >> 2) & 1) * 4096 + 2048 * ((i >> 1) & 1), toff[i & 1]);
         };
         f32x16 x[2], dp[2];                                           // x[t][r], dp[t][r]: query l32, key 64j + 32t + 16(r >> 3) + 8hi + (r & 7)
         unsigned df[2][2][4];
@@ -238,7 +238,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     };
     auto advance = [&]() __attribute__((always_inline)) {
         const int j2 = next_tile(j1 + 1, w2);
-        rb_tiles_landed();                                            // tile j1, issued one tile ago
+        tt_landed();                                            // tile j1, issued one tile ago
         if (j2 < nkv) stage(j2, rb_next(rb_next(buf)));               // its buffer was last read before the previous barrier
         rb_reads_done_barrier();
         j = j1; w = w1;
@@ -364,18 +364,18 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     const bool lone = p.mask ? __syncthreads_count(mine != 0) == 1 && !__syncthreads_or(mine > 1) : S == 1;
     if (__syncthreads_or(some ? 1 : 0)) {
         const unsigned q_row = (unsigned)p.q.ss * 2, g_row = (unsigned)args.go.ss * 2;
-        const i32x4 q_rsrc = rb_rsrc(p.q.p + (size_t)b * p.q.sb + (size_t)h * p.q.sh, (unsigned)(S - 1) * q_row + 128);
-        const i32x4 g_rsrc = rb_rsrc(args.go.p + (size_t)b * args.go.sb + (size_t)h * args.go.sh, (unsigned)(S - 1) * g_row + 128);
+        const i32x4 q_rsrc = tt_rsrc(p.q.p + (size_t)b * p.q.sb + (size_t)h * p.q.sh, (unsigned)(S - 1) * q_row + 128);
+        const i32x4 g_rsrc = tt_rsrc(args.go.p + (size_t)b * args.go.sb + (size_t)h * args.go.sh, (unsigned)(S - 1) * g_row + 128);
         float next_l = 0.f, next_d = 0.f;
         // rows behind the last one repeat it: their P is 0 (L = +inf), and what they are multiplied with has to be a number
         auto stage = [&](int j, int buf) __attribute__((always_inline)) {
-            const unsigned dst = rb_lds(smem) + buf + wave_s * 1024;
+            const unsigned dst = tt_lds(smem) + buf + wave_s * 1024;
 #pragma unroll
             for (int ps = 0; ps < 8 / NW; ++ps) {
-                const int r = (ps * NW + wave) * 8 + (lane >> 3), sw = ((lane & 7) ^ rb_swz(r)) << 4;
+                const int r = (ps * NW + wave) * 8 + (lane >> 3), sw = ((lane & 7) ^ tt_swz(r)) << 4;
                 const unsigned row = min(j * RB_KV + r, S - 1);
-                rb_dma16(q_rsrc, row * q_row + sw, 0u, dst + ps * (NW * 1024));
-                rb_dma16(g_rsrc, row * g_row + sw, 0u, dst + RB_TILE + ps * (NW * 1024));
+                tt_dma16(q_rsrc, row * q_row + sw, 0u, dst + ps * (NW * 1024));
+                tt_dma16(g_rsrc, row * g_row + sw, 0u, dst + RB_TILE + ps * (NW * 1024));
             }
             if (tid < RB_KV) {
                 const int row = j * RB_KV + tid;
@@ -403,7 +403,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
         rb_arrived(vf);
         int roff[4], toff[2][2];
         rb_row_offsets(lane, roff);
-        rb_tr_offsets(lane, toff);
+        tt_offsets(lane, toff);
         drain_and_barrier();
         const float far_r = tab[2 * (p.reach + RB_PAD)], far_l = tab[0];
         // One tile of 64 queries.  The scores start from −L / c, so that one fma with the bias gives the exponent, and dP from −δ.  VALU issued between a wave's own matrix
@@ -428,7 +428,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
             // the A fragment of matrix instruction i of 32: scores and dP of the first half, of the second half, products of the first, of the second
             auto fragment = [&](int i) {
                 if (i < 16) return *(const bf16x8*)(base + (i & 1) * RB_TILE + (i >> 3) * 4096 + roff[(i >> 1) & 3]);
-                return rb_read_tr1(base + (i & 1 ? 0 : RB_TILE) + ((i >> 3) & 1) * 4096 + 2048 * ((i >> 2) & 1), toff[(i >> 1) & 1]);
+                return tt_read(base + (i & 1 ? 0 : RB_TILE) + ((i >> 3) & 1) * 4096 + 2048 * ((i >> 2) & 1), toff[(i >> 1) & 1]);
             };
             auto score = [&](int i, const bf16x8& a, f32x16& x, f32x16& dp) {
                 if (i & 1) dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, vf[(i >> 1) & 3], dp, 0, 0, 0);
@@ -475,7 +475,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
             });
         };
         auto advance = [&](int j) __attribute__((always_inline)) {
-            rb_tiles_landed();                                        // tile j + 1, issued one tile ago, and its rows' L and δ
+            tt_landed();                                        // tile j + 1, issued one tile ago, and its rows' L and δ
             put_rows(rb_next(buf));
             if (j + 2 < nq) stage(j + 2, rb_next(rb_next(buf)));      // its buffer was last read before the previous barrier
             rb_reads_done_barrier();

@@ -190,6 +190,25 @@ def test_backward_larger(cuda, hip_lib, M, K, F):
     _check_backward(x, wg, wu, dh, "gelu_tanh")
 
 
+@pytest.mark.parametrize("M,K,F", [(4200, 4096, 96), (4097, 2048, 64), (60, 2048, 4096), (250, 64, 4000), (128, 320, 8224)])
+def test_backward_paths_of_dx(cuda, hip_lib, M, K, F):
+    """Turned copies of the weights for many rows; the sum over F split for few ones, in many parts, with K not a multiple of the tile's columns."""
+    x, wg, wu, dh = _inputs(M, K, F, cuda, seed=7)
+    _check_backward(x, wg, wu, dh, "silu")
+
+
+def test_backward_keeps_a_nan_in_its_row(cuda, hip_lib):
+    from aether_amd import ops
+    for M in (40, 200):
+        x, wg, wu, dh = _inputs(M, 128, 96, cuda, seed=8)
+        _, gu = ops.gated_ff(x, wg, wu, need_gu=True)
+        want = ops.gated_ff_backward(dh, x, wg, wu, gu)[0]
+        dh[3, 7] = float("nan")
+        dx = ops.gated_ff_backward(dh, x, wg, wu, gu)[0]
+        keep = torch.arange(M, device=cuda) != 3
+        assert bool(torch.isnan(dx[3].float()).all()) and torch.equal(dx[keep], want[keep])
+
+
 @pytest.mark.parametrize("act", ["gelu_tanh", "silu"])
 def test_backward_against_differences(cuda, hip_lib, act):
     from aether_amd import ops
