@@ -175,6 +175,10 @@ def _like(t, dtype):
     return torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
 
 
+def _workspace(t, nbytes):
+    return t.new_empty((nbytes,), dtype=torch.uint8)
+
+
 _STREAMS = {torch.bfloat16: _lib.AETHER_STREAM_BF16, torch.float32: _lib.AETHER_STREAM_FP32}
 
 
@@ -235,13 +239,13 @@ def rms_norm_backward(dy, res, w, eps=1e-6, dres=None, need_ddelta=False):
     r2, g2, w = _rows(res, D), _rows(dy, D), _vector(w)
     s2 = None if dres is None else _rows(dres, D)
     rows = r2.shape[0]
-    dx = torch.empty(res.shape, dtype=res.dtype, device=dev)
+    dx = _like(res, res.dtype)
     # with a bf16 stream the rounded dx IS ddelta
-    ddelta = torch.empty(res.shape, dtype=torch.bfloat16, device=dev) if need_ddelta and res.dtype != torch.bfloat16 else None
-    dw = torch.empty(D, dtype=torch.float32, device=dev)
+    ddelta = _like(res, torch.bfloat16) if need_ddelta and res.dtype != torch.bfloat16 else None
+    dw = _like(w, torch.float32)
     lib = _lib.load()
     nbytes = lib.aether_rms_norm_bwd_workspace_bytes(rows, D)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    ws = _workspace(w, nbytes)
     _run("rms_norm_backward", dev, lib.aether_rms_norm_bwd, g2.data_ptr(), g2.stride(0), r2.data_ptr(), _STREAMS[res.dtype], r2.stride(0),
          _lib.ptr(s2), s2.stride(0) if s2 is not None else 0, w.data_ptr(), float(eps), dx.data_ptr(), D, _lib.ptr(ddelta), D, dw.data_ptr(), rows, D,
          ws.data_ptr(), nbytes)
@@ -336,7 +340,7 @@ def relbias_attn(q, k, v, table, max_distance=128, scale=1.0, key_mask=None, nee
     dev, d, keep = _relbias("relbias_attn", q, k, v, table, max_distance, scale, key_mask)
     o = _like(q, torch.bfloat16)
     n = o.numel() // 64
-    lse = torch.empty(_lse_pad(n) + 32 * n, dtype=torch.float32, device=dev) if need_lse else None
+    lse = q.new_empty((_lse_pad(n) + 32 * n,), dtype=torch.float32) if need_lse else None
     at = lse.data_ptr() if need_lse else None
     _run("relbias_attn", dev, _lib.load().aether_relbias_attn, d, o.data_ptr(), at + 4 * _lse_pad(n) if need_lse else None, at)
     return (o, lse) if need_lse else o
@@ -370,7 +374,7 @@ def relbias_attn_backward(do, q, k, v, o, lse, table, max_distance=128, scale=1.
     dtable = _like(table, torch.bfloat16) if need_dtable else None
     lib = _lib.load()
     nbytes = lib.aether_relbias_attn_bwd_workspace_bytes(d, need_dtable)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    ws = _workspace(q, nbytes)
     st = _strides(S * 3 * H * 64, 3 * H * 64, 64)
     _run(name, dev, lib.aether_relbias_attn_bwd, d, do.data_ptr(), _strides(*do.stride()[:3]), o.data_ptr(), _strides(*o.stride()[:3]), lse.data_ptr() + 4 * _lse_pad(n), lse.data_ptr(),
          dq.data_ptr(), st, dk.data_ptr(), st, dv.data_ptr(), st, _lib.ptr(dtable), ws.data_ptr(), nbytes)
@@ -451,7 +455,7 @@ def gated_ff_backward(dh, x, wg, wu, gu, act="gelu_tanh", need_dx=True, need_dw=
         gu = gu.contiguous()
     lib = _lib.load()
     nbytes = lib.aether_gated_ff_bwd_workspace_bytes(M, F, K)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    ws = _workspace(x, nbytes)
     _run(name, dev, lib.aether_gated_ff_bwd, d2.data_ptr(), d2.stride(0), x2.data_ptr(), x2.stride(0), wg.data_ptr(), wu.data_ptr(), wg.stride(0), gu.data_ptr(),
          _lib.ptr(dx), K, _lib.ptr(dw), M, F, K, _ACTS[act], ws.data_ptr(), nbytes)
     return out
