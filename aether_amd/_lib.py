@@ -71,7 +71,7 @@ SIGNATURES = {
     "aether_flash_attn_fwd": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
     "aether_rms_norm": (_i, [_vp, _i, _l, _vp, _l, _vp, _l, _fp, _f, _vp, _l, _fp, _i, _i, _vp]),
     "aether_rms_norm_bwd_workspace_bytes": (_sz, [_i, _i]),
-    "aether_rms_norm_bwd": (_i, [_vp, _l, _vp, _i, _l, _vp, _l, _fp, _f, _vp, _l, _vp, _l, _fp, _i, _i, _vp, _sz, _vp]),
+    "aether_rms_norm_bwd": (_i, [_vp, _l, _vp, _i, _l, _vp, _l, _vp, _l, _fp, _f, _vp, _l, _vp, _l, _fp, _i, _i, _vp, _sz, _vp]),
     "aether_quantize_rows_e4m3": (_i, [_vp, _l, _vp, _l, _fp, _i, _i, _vp]),
     # descriptors and strides are passed as packed bytes
     "aether_relbias_attn": (_i, [_vp, _vp, _vp, _fp, _vp]),

@@ -120,7 +120,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     f32x16 dq[2], minus_delta;                                        // dP starts from −δ
 #pragma unroll
     for (int i = 0; i < 16; ++i) { dq[0][i] = 0.f; dq[1][i] = 0.f; minus_delta[i] = -delta; }
-    float sum_r = 0.f, sum_l = 0.f, far_sum = 0.f;                    // dS beyond the reach, on either side
+    float sum_r = 0.f, sum_l = 0.f, far_sum[2] = {0.f, 0.f};                    // dS beyond the reach, on either side
     float carry = 0.f;                                                // diagonals that go on into the keys from carry_at on (wave-uniform; < 0: none)
     int carry_at = -1;
     auto put = [&](int at, float v) {
@@ -197,10 +197,9 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
             x[t][2 * e + 1] = d1;
             const unsigned pk = pack_bf16x2(d0, d1);
             df[t][e >> 2][e & 3] = pk;
-            if constexpr (!NEAR) {                                    // a far bucket's share, from the rounded values: one instruction a pair
-                bf16x2 ones;
-                ones[0] = (__bf16)1.0f; ones[1] = (__bf16)1.0f;
-                far_sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pk), ones, far_sum, false);
+            if constexpr (!NEAR) {                                    // a far bucket's share.  (A row's dS add up to 0: summed after their rounding, the far ones of a long row
+                far_sum[0] += d0;                                     // lose what they differ by from the near ones.)
+                far_sum[1] += d1;
             }
         };
         constexpr int AHEAD = 3;                                      // fragments are read this many instructions before they are used
@@ -255,15 +254,15 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
         advance();
     };
     while (j < min(near_from, nkv)) far(far_l - lse);
-    sum_l = far_sum;
-    far_sum = 0.f;
+    sum_l = far_sum[0] + far_sum[1];
+    far_sum[0] = far_sum[1] = 0.f;
     while (j < min(near_to, nkv)) {
         if (__builtin_expect(w != ~0ull, 0)) tile(-lse, std::true_type{}, std::true_type{});
         else tile(-lse, std::true_type{}, std::false_type{});
         advance();
     }
     while (j < nkv) far(far_r - lse);
-    sum_r = far_sum;
+    sum_r = far_sum[0] + far_sum[1];
     if (lone) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) { dq[0][i] = 0.f; dq[1][i] = 0.f; }

@@ -35,7 +35,8 @@ struct RmsArgs {
 
 struct RmsBwdArgs {
     const bf16_t* dy; long lddy;
-    const void* res; long ldr;         // h as the forward pass stored it
+    const void* res; long ldr;         // h as the forward pass stored it; with delta the stream before the addition
+    const bf16_t* delta; long ldd;     // or null
     const void* dres; long lddr;       // the gradient that reaches h from elsewhere, stream type, or null
     const float* w;
     void* dx; long lddx;               // stream type
@@ -210,7 +211,7 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(RmsArgs p) {
     }
 }
 
-template <class XT, int WPR, int NCH>
+template <class XT, int WPR, int NCH, bool SUM>      // SUM: h is taken from the stream and delta
 __global__ __launch_bounds__(256) void rms_norm_bwd_kernel(RmsBwdArgs p) {
     __shared__ float red[2][8];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -233,7 +234,7 @@ __global__ __launch_bounds__(256) void rms_norm_bwd_kernel(RmsBwdArgs p) {
         }
     }
     Raw8<XT> x[NCH], dr[NCH];
-    u16x8 g[NCH];
+    u16x8 g[NCH], dl[NCH];
     auto fetch = [&](int row) {
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
@@ -242,6 +243,7 @@ __global__ __launch_bounds__(256) void rms_norm_bwd_kernel(RmsBwdArgs p) {
                 load8(x[c], (const XT*)p.res + (size_t)row * p.ldr + d);
                 g[c] = *(const u16x8*)((const unsigned short*)p.dy + (size_t)row * p.lddy + d);
                 if (p.dres) load8(dr[c], (const XT*)p.dres + (size_t)row * p.lddr + d);
+                if constexpr (SUM) dl[c] = *(const u16x8*)((const unsigned short*)p.delta + (size_t)row * p.ldd + d);
             }
         }
     };
@@ -255,6 +257,7 @@ __global__ __launch_bounds__(256) void rms_norm_bwd_kernel(RmsBwdArgs p) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 h[c][e] = in ? get8(x[c], e) : 0.f;
+                if constexpr (SUM) h[c][e] += in ? bf16_bits_to_f32(dl[c][e]) : 0.f;
                 n[c][e] = in ? bf16_bits_to_f32(g[c][e]) : 0.f;
                 o[c][e] = in && p.dres ? get8(dr[c], e) : 0.f;
                 sq += h[c][e] * h[c][e];
@@ -393,27 +396,32 @@ extern "C" size_t aether_rms_norm_bwd_workspace_bytes(int rows, int D) {
     return (size_t)rms_grid(rows, rpb, RMS_BWD_WG) * rpb * D * sizeof(float);
 }
 
-extern "C" int aether_rms_norm_bwd(const void* dy, long lddy, const void* res, int x_dtype, long ldr, const void* dres, long lddr, const float* w, float eps,
-                                   void* dx, long lddx, void* ddelta, long ldds, float* dw, int rows, int D, void* workspace, size_t workspace_bytes, void* stream) {
+extern "C" int aether_rms_norm_bwd(const void* dy, long lddy, const void* res, int x_dtype, long ldr, const void* delta, long ldd, const void* dres, long lddr,
+                                   const float* w, float eps, void* dx, long lddx, void* ddelta, long ldds, float* dw, int rows, int D, void* workspace, size_t workspace_bytes, void* stream) {
     int rc = rms_check(res, x_dtype, rows, D, "rms_norm_bwd: null stream");
     if (rc) return rc;
     if (!w || !dw) return aether_set_error(AETHER_ERR_ARG, "rms_norm_bwd: null weight or weight gradient");
     if (rows > 0 && (!dy || !dx)) return aether_set_error(AETHER_ERR_ARG, "rms_norm_bwd: null gradient");
-    if (lddy % 8 || ldr % 8 || (dres && lddr % 8) || lddx % 8 || (ddelta && ldds % 8)) return aether_set_error(AETHER_ERR_ALIGN, "rms_norm_bwd: leading dimensions must be multiples of 8");
-    if (((uintptr_t)dy | (uintptr_t)res | (uintptr_t)dres | (uintptr_t)w | (uintptr_t)dx | (uintptr_t)ddelta | (uintptr_t)workspace) & 15)
+    if (lddy % 8 || ldr % 8 || (delta && ldd % 8) || (dres && lddr % 8) || lddx % 8 || (ddelta && ldds % 8)) return aether_set_error(AETHER_ERR_ALIGN, "rms_norm_bwd: leading dimensions must be multiples of 8");
+    if (((uintptr_t)dy | (uintptr_t)res | (uintptr_t)delta | (uintptr_t)dres | (uintptr_t)w | (uintptr_t)dx | (uintptr_t)ddelta | (uintptr_t)workspace) & 15)
         return aether_set_error(AETHER_ERR_ALIGN, "rms_norm_bwd: pointers must be 16-byte aligned");
     if (rows > 0 && (!workspace || workspace_bytes < aether_rms_norm_bwd_workspace_bytes(rows, D)))
         return aether_set_error(AETHER_ERR_ARG, "rms_norm_bwd: workspace too small (aether_rms_norm_bwd_workspace_bytes)");
     hipStream_t s = (hipStream_t)stream;
     int slots = 0;
     if (rows > 0) {
-        RmsBwdArgs p = {(const bf16_t*)dy, lddy, res, ldr, dres, lddr, w, dx, lddx, (bf16_t*)ddelta, ldds, (float*)workspace, rows, D, eps, 1.0f / (float)D};
+        RmsBwdArgs p = {(const bf16_t*)dy, lddy, res, ldr, (const bf16_t*)delta, ldd, dres, lddr, w, dx, lddx, (bf16_t*)ddelta, ldds, (float*)workspace, rows, D, eps, 1.0f / (float)D};
 #define RMS_BWD(WPR, NCH)                                                                                                       \
     do {                                                                                                                        \
         dim3 grid(rms_grid(rows, 4 / WPR, RMS_BWD_WG));                                                                         \
         slots = grid.x * (4 / WPR);                                                                                             \
-        if (x_dtype == AETHER_STREAM_FP32) hipLaunchKernelGGL((rms_norm_bwd_kernel<float, WPR, NCH>), grid, dim3(256), 0, s, p); \
-        else hipLaunchKernelGGL((rms_norm_bwd_kernel<bf16_t, WPR, NCH>), grid, dim3(256), 0, s, p);                             \
+        if (x_dtype == AETHER_STREAM_FP32) {                                                                                    \
+            if (delta) hipLaunchKernelGGL((rms_norm_bwd_kernel<float, WPR, NCH, true>), grid, dim3(256), 0, s, p);              \
+            else hipLaunchKernelGGL((rms_norm_bwd_kernel<float, WPR, NCH, false>), grid, dim3(256), 0, s, p);                   \
+        } else {                                                                                                                \
+            if (delta) hipLaunchKernelGGL((rms_norm_bwd_kernel<bf16_t, WPR, NCH, true>), grid, dim3(256), 0, s, p);             \
+            else hipLaunchKernelGGL((rms_norm_bwd_kernel<bf16_t, WPR, NCH, false>), grid, dim3(256), 0, s, p);                  \
+        }                                                                                                                       \
     } while (0)
         RMS_PICK(D, RMS_BWD);
 #undef RMS_BWD

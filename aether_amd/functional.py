@@ -1,6 +1,6 @@
 """The text encoder's operators with autograd: the forward and backward entry points of `aether_amd.ops` as differentiable functions.
 
-Each call outside of `torch.no_grad()` keeps what its backward pass needs (rms_norm: the sum; relbias_attn: its output in two bf16 parts and the rows'
+Each call outside of `torch.no_grad()` keeps what its backward pass needs (rms_norm: the sum, or with a bfloat16 stream both of its terms; relbias_attn: its output in two bf16 parts and the rows'
 log-sums; gated_ff: both projections in fp32).  Gradients are first order, and the same bits every time.
 
 Into a captured graph, record the backward pass with `torch.autograd.grad` on leaves that no eager graph holds at that time: `Tensor.backward` accumulates
@@ -18,7 +18,8 @@ class _RmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, delta, w, eps):
         y, res = ops.rms_norm(x, w, eps, delta=delta)
-        ctx.save_for_backward(res, w)
+        again = delta is not None and x.dtype == torch.bfloat16          # the stored sum is rounded, the norm's was not
+        ctx.save_for_backward(x if again else res, w, delta if again else None)
         ctx.eps, ctx.summed = eps, delta is not None
         ctx.set_materialize_grads(False)
         return (y, res) if ctx.summed else y
@@ -26,13 +27,13 @@ class _RmsNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dres=None):
-        res, w = ctx.saved_tensors
+        res, w, delta = ctx.saved_tensors
         need_x, need_delta, need_w = ctx.needs_input_grad[:3]
         if dy is None and dres is None:
             return None, None, None, None
         if dy is None:                      # only the sum was used
             return dres if need_x else None, dres.to(torch.bfloat16) if need_delta else None, torch.zeros_like(w) if need_w else None, None
-        dx, ddelta, dw = ops.rms_norm_backward(dy, res, w, ctx.eps, dres=dres, need_ddelta=need_delta)
+        dx, ddelta, dw = ops.rms_norm_backward(dy, res, w, ctx.eps, dres=dres, need_ddelta=need_delta, delta=delta)
         return dx if need_x else None, ddelta, dw if need_w else None, None
 
 

@@ -228,16 +228,20 @@ def rms_norm_e4m3(x, w, eps=1e-6, delta=None):
     return _rms_norm(x, w, eps, delta, True)
 
 
-def rms_norm_backward(dy, res, w, eps=1e-6, dres=None, need_ddelta=False):
-    """Gradients of `rms_norm` from its stored h (`res`): dy bfloat16 [..., D] for y, dres (the stream's type) for h or None.
+def rms_norm_backward(dy, res, w, eps=1e-6, dres=None, need_ddelta=False, delta=None):
+    """Gradients of `rms_norm` from its stored h (`res`): dy bfloat16 [..., D] for y, dres (the stream's type) for h or None.  With delta, `res` is the stream before
+    the addition and the sum is taken again: a bfloat16 stream's h is rounded, the norm was of the unrounded sum.
     -> (dx in the stream's type, ddelta bfloat16 or None, dw float32 [D]).  Summed in an order that depends on the sizes alone."""
-    dev = _same_device(res, dy, w, dres)
+    dev = _same_device(res, dy, w, dres, delta)
     D = _norm_operands(res, w, dy, "rms_norm_backward")
+    if delta is not None:
+        _norm_operands(res, w, delta, "rms_norm_backward")
     if dres is not None:
         if not (dres.dtype == res.dtype and dres.shape == res.shape):
             raise ValueError(f"rms_norm_backward: dres is {res.dtype} {list(res.shape)}, got {dres.dtype} {list(dres.shape)}")
     r2, g2, w = _rows(res, D), _rows(dy, D), _vector(w)
     s2 = None if dres is None else _rows(dres, D)
+    d2 = None if delta is None else _rows(delta, D)
     rows = r2.shape[0]
     dx = _like(res, res.dtype)
     # with a bf16 stream the rounded dx IS ddelta
@@ -247,7 +251,7 @@ def rms_norm_backward(dy, res, w, eps=1e-6, dres=None, need_ddelta=False):
     nbytes = lib.aether_rms_norm_bwd_workspace_bytes(rows, D)
     ws = _workspace(w, nbytes)
     _run("rms_norm_backward", dev, lib.aether_rms_norm_bwd, g2.data_ptr(), g2.stride(0), r2.data_ptr(), _STREAMS[res.dtype], r2.stride(0),
-         _lib.ptr(s2), s2.stride(0) if s2 is not None else 0, w.data_ptr(), float(eps), dx.data_ptr(), D, _lib.ptr(ddelta), D, dw.data_ptr(), rows, D,
+         _lib.ptr(d2), d2.stride(0) if d2 is not None else 0, _lib.ptr(s2), s2.stride(0) if s2 is not None else 0, w.data_ptr(), float(eps), dx.data_ptr(), D, _lib.ptr(ddelta), D, dw.data_ptr(), rows, D,
          ws.data_ptr(), nbytes)
     return dx, (dx if res.dtype == torch.bfloat16 else ddelta) if need_ddelta else None, dw
 

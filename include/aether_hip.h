@@ -136,11 +136,12 @@ int aether_flash_attn_fwd(const void* Qh, const void* Kh, const void* Vt, void* 
  * D % 8 == 0, D <= 16384; leading dimensions in elements, multiples of 8.  Σ h² must stay in fp32's range. */
 int aether_rms_norm(const void* x, int x_dtype, long ldx, const void* delta, long ldd, void* res, long ldr, const float* w, float eps,
                     void* y, long ldy, float* scale, int rows, int D, void* stream);
-/* Backward pass from the stored h (res): n = dy·w, ĥ = h·r:  dx = r·(n − ĥ·mean(n·ĥ)) + dres (the stream's type; dres may be NULL; may alias dres),
+/* Backward pass from the stored h (res), or, with delta (else NULL), from the stream before the addition and delta: the sum is taken again, unrounded, where a
+ * stored bf16 h would cost dw its rounding.  n = dy·w, ĥ = h·r:  dx = r·(n − ĥ·mean(n·ĥ)) + dres (the stream's type; dres may be NULL; may alias dres),
  * ddelta = dx rounded to bf16 (may be NULL), dw = Σ_rows dy·ĥ (fp32 [D], summed in an order that depends on the sizes alone). */
 size_t aether_rms_norm_bwd_workspace_bytes(int rows, int D);
-int aether_rms_norm_bwd(const void* dy, long lddy, const void* res, int x_dtype, long ldr, const void* dres, long lddr, const float* w, float eps,
-                        void* dx, long lddx, void* ddelta, long ldds, float* dw, int rows, int D, void* workspace, size_t workspace_bytes, void* stream);
+int aether_rms_norm_bwd(const void* dy, long lddy, const void* res, int x_dtype, long ldr, const void* delta, long ldd, const void* dres, long lddr,
+                        const float* w, float eps, void* dx, long lddx, void* ddelta, long ldds, float* dw, int rows, int D, void* workspace, size_t workspace_bytes, void* stream);
 /* q = e4m3(x / scale) with one power of two per row, chosen as above.  x bf16 [rows, K], K % 8 == 0. */
 int aether_quantize_rows_e4m3(const void* x, long ldx, void* q, long ldq, float* scale, int rows, int K, void* stream);
 

@@ -186,6 +186,18 @@ def test_one_side_switched_off(cuda, hip_lib, low, S, scale):
             assert bool(((x[1, 25:].double() - y[0].double()).norm() <= 4 * BF16 * y.double().norm()))
 
 
+def test_far_buckets_of_long_rows(cuda, hip_lib):
+    """A row's dS add up to 0, so the far buckets' sums are what the near ones are, over ten times as many terms: their relative error (in the norm) is that of
+    sums in fp32 and one rounding to bf16 (2^-8 / sqrt(12) · 1.2 in the mean), not of terms rounded before they are summed."""
+    qkv, table = inputs(1, 2039, 4, device=cuda, seed=38, qk=0.3)
+    q, k, v = qkv.unbind(2)
+    do = _do(q)
+    got = _run(q, k, v, table, do)[3].double()
+    leaf = [t.double().requires_grad_(True) for t in (q, k, v, table)]
+    want, = torch.autograd.grad((attention(*leaf)[0] * do.double()).sum(), leaf[3:])
+    assert (got - want).norm() <= 2.0 ** -9 * want.norm()
+
+
 def test_empty_row_with_non_finite_gradient(cuda, hip_lib):
     """A NaN in the gradient of one row reaches that row and the keys it attends to, not the keys that do not count."""
     qkv, table = inputs(2, 100, 2, device=cuda, seed=25)

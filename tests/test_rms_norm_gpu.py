@@ -129,6 +129,35 @@ def test_backward(cuda, hip_lib, rows, D, stream, with_dres):
     assert torch.equal(again[0], gx) and torch.equal(again[2], gw), "the same order of sums every time"
 
 
+@pytest.mark.parametrize("stream", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,D", [(1, 8), (11, 2224), (300, 520), (700, 4096), (5, 8200), (3, 16384)])
+def test_backward_from_both_terms(cuda, hip_lib, rows, D, stream):
+    """With delta the sum is taken again: the gradients of the norm of the unrounded sum, dw to fp32's accuracy with a bfloat16 stream too."""
+    from aether_amd import functional, ops
+    x, delta, w, dy, dres = _inputs(rows, D, stream, seed=5, cuda=cuda)
+    h, wd = (x.double() + delta.double()).requires_grad_(True), w.double().requires_grad_(True)
+    y = h / torch.sqrt(h.square().mean(-1, keepdim=True) + 1e-6) * wd
+    dx, dw = torch.autograd.grad((y * dy.double()).sum() + (h * dres.double()).sum(), (h, wd))
+    gx, gd, gw = ops.rms_norm_backward(dy, x, w, dres=dres, need_ddelta=True, delta=delta)
+    with torch.no_grad():
+        r = 1 / torch.sqrt(h.square().mean(-1, keepdim=True) + 1e-6)
+        n = (dy.double() * wd).abs()
+        hm = (x.double().abs() + delta.double().abs()) * 2.0 ** -24 * r              # the sum's own rounding in fp32
+        terms = r * (n + (h * r).abs() * (n * (h * r).abs()).mean(-1, keepdim=True)) + dres.double().abs()
+        moved = r * (hm * (n * (h * r).abs()).mean(-1, keepdim=True) + (h * r).abs() * (n * hm).mean(-1, keepdim=True))
+        wterms = (dy.double() * h * r).abs().sum(0)
+        wmoved = (dy.double().abs() * hm).sum(0)
+    assert bool(((gx.double() - dx).abs() <= F32 * terms + 2 * moved + (BF16 if stream == torch.bfloat16 else 0.0) * dx.abs()).all())
+    assert torch.equal(gd, gx.to(torch.bfloat16))
+    assert bool(((gw.double() - dw).abs() <= (F32 + (rows / 512 + 64) * 2.0 ** -24) * wterms + 2 * wmoved).all())
+    leaves = [t.clone().requires_grad_(True) for t in (x, delta, w)]
+    got = torch.autograd.grad(functional.rms_norm(leaves[0], leaves[2], delta=leaves[1]), leaves, [dy, dres])
+    if stream == torch.bfloat16:
+        assert all(torch.equal(a, b) for a, b in zip(got, (gx, gd, gw)))
+    with pytest.raises(ValueError):
+        ops.rms_norm_backward(dy, x, w, delta=delta[:, :-1])
+
+
 def test_backward_against_differences(cuda, hip_lib):
     """(f(h + e d) − f(h − e d)) / 2e of the float64 formula along random directions equals the kernel's gradient · d."""
     from aether_amd import ops

@@ -34,8 +34,8 @@ def test_rms_norm_entry_without_rows(hip_lib):
     assert _norm(hip_lib, rows=0, x=None, y=None) == 0
 
 
-def _norm_bwd(lib, dy=4096, ldy=64, res=4096, xt=1, ldr=64, dres=None, lds=64, w=4096, dx=4096, ldx=64, dd=None, ldd=64, dw=4096, rows=4, D=64, ws=4096, n=1 << 20):
-    return lib.aether_rms_norm_bwd(dy, ldy, res, xt, ldr, dres, lds, w, 1e-6, dx, ldx, dd, ldd, dw, rows, D, ws, n, None)
+def _norm_bwd(lib, dy=4096, ldy=64, res=4096, xt=1, ldr=64, delta=None, ldl=64, dres=None, lds=64, w=4096, dx=4096, ldx=64, dd=None, ldd=64, dw=4096, rows=4, D=64, ws=4096, n=1 << 20):
+    return lib.aether_rms_norm_bwd(dy, ldy, res, xt, ldr, delta, ldl, dres, lds, w, 1e-6, dx, ldx, dd, ldd, dw, rows, D, ws, n, None)
 
 
 @pytest.mark.parametrize("kw,code,text", [
@@ -46,6 +46,8 @@ def _norm_bwd(lib, dy=4096, ldy=64, res=4096, xt=1, ldr=64, dres=None, lds=64, w
     (dict(res=None), -1, b"null"),
     (dict(ldy=4), -3, b"leading"),
     (dict(dres=4096, lds=4), -3, b"leading"),
+    (dict(delta=4096, ldl=4), -3, b"leading"),
+    (dict(delta=4104), -3, b"aligned"),
     (dict(dx=4104), -3, b"aligned"),
     (dict(ws=None), -1, b"workspace"),
     (dict(n=4 * 64 * 4 - 1), -1, b"workspace"),
