@@ -212,7 +212,9 @@ def _own_norm(s):
     y, res = ops.rms_norm(s["x"], s["w"], s["eps"], delta=s["delta"])
     if s["mode"] == "infer":
         return {"y": y, "res": res}
-    dx, ddelta, dw = ops.rms_norm_backward(s["dy"], res, s["w"], s["eps"], dres=s["dres"], need_ddelta=True)
+    # a bf16 stream's stored sum is rounded, the norm's was not: both terms again
+    h, delta = (s["x"], s["delta"]) if res.dtype == torch.bfloat16 else (res, None)
+    dx, ddelta, dw = ops.rms_norm_backward(s["dy"], h, s["w"], s["eps"], dres=s["dres"], need_ddelta=True, delta=delta)
     return {"y": y, "res": res, "dx": dx, "ddelta": ddelta, "dw": dw}
 
 
