@@ -136,17 +136,19 @@ def flash_attn_fwd(Qh, Kh, Vt, flags=0):
 
 def _same_device(first, *others):
     """The device of the call.  Every operand lives there."""
-    _need_cuda(first, *others)
     dev = first.device
     for t in others:
         if t is not None and t.device != dev:
+            _need_cuda(first, *others)
             raise ValueError(f"operands are on different devices: {dev} and {t.device}")
+    if not first.is_cuda:
+        _need_cuda(first)
     return dev
 
 
 def _run(what, dev, fn, *args):
     """fn(*args, stream) on `dev` and its current stream."""
-    if dev.index == torch.cuda.current_device():
+    if dev.index == torch._C._cuda_getDevice():
         rc = fn(*args, _lib.stream_of(dev.index))
     else:
         with torch.cuda.device(dev):
@@ -188,7 +190,7 @@ def _norm_operands(x, w, delta, name):
     if not (x.dim() >= 1 and x.shape[-1] > 0):
         raise ValueError(f"{name}: the stream has no last dimension")
     D = x.shape[-1]
-    if not (w.dtype == torch.float32 and tuple(w.shape) == (D,)):
+    if w.dtype != torch.float32 or w.shape != (D,):
         raise ValueError(f"{name}: the weight is float32 [{D}], got {w.dtype} {list(w.shape)}")
     if delta is not None:
         if not (delta.dtype == torch.bfloat16 and delta.shape == x.shape):
