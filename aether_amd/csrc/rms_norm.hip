@@ -351,7 +351,8 @@ static int rms_check(const void* x, int x_dtype, long rows, int D, const char* w
 
 using namespace aether;
 
-// D -> waves per row and chunks per lane: one wave up to 1024 elements (no barrier), four above
+// D -> waves per row and chunks per lane: one wave up to 1024 elements (no barrier), four above.  3616 rows, fp32: forward 5.1 ... 6.5 TB/s at 4096 ... 16384
+// elements; backward 5.0 at 4096, 4.7 at 8192, 3.3 above, where a lane's 64 elements of six vectors no longer fit its registers.
 #define RMS_PICK(D, CALL)                     \
     do {                                      \
         if ((D) <= 512) { CALL(1, 1); }       \
