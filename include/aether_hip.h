@@ -151,7 +151,8 @@ int aether_quantize_rows_e4m3(const void* x, long ldx, void* q, long ldq, float*
  * array of half − near − 1 distances, not falling) is where each bucket behind the first logarithmic one begins, at 1024 or before.
  * q, k, v bf16 [B, S, H, 64] with strides (batch, position, head) in elements, multiples of 8, last dimension dense; S <= 65536.
  * table bf16 [num_buckets, H]; mask: bytes [B, S] with batch stride mask_sb, 0 = the key does not count, or NULL.  What stands at a key that does not
- * count (NaN, infinities) reaches no output. */
+ * count (NaN, infinities) reaches no output.  scale is 0 or of a magnitude in [1e-20, 1e20]; |v| up to 1e22 (weighted sums are held in fp32 before they are
+ * normalized); table entries of -inf or the lowest value switch a bucket off. */
 typedef struct AetherRelbias {
     const void* q; const void* k; const void* v;
     long q_strides[3], k_strides[3], v_strides[3];
@@ -165,7 +166,7 @@ typedef struct AetherRelbias {
     int n_borders;
 } AetherRelbias;
 /* o bf16 [B, S, H, 64] dense.  For a backward pass also o_low bf16 [B, S, H, 64] (what the rounding of o left: o + o_low is good to 2^-16) and
- * lse fp32 [B, H, S] (base-2 log of the row sums, +inf for a row without keys); both or neither. */
+ * lse fp32 [B, H, S] (base-2 log of the row sums; +inf, which means no gradient, for a row without keys and where the log lies beyond 2^20); both or neither. */
 int aether_relbias_attn(const AetherRelbias* d, void* o, void* o_low, float* lse, void* stream);
 /* Backward pass: go = dO and o as above with strides of their own (batch, position, head); dq, dk, dv bf16 [B, S, H, 64] with strides of their own (they
  * may be thirds of one packed buffer); dtable bf16 [num_buckets, H] or NULL.  dk and dv are 0 at keys that do not count.  Sums in an order that depends on
