@@ -298,7 +298,14 @@ __global__ __launch_bounds__(1024) void rms_norm_dw_kernel(const float* __restri
     const int d = blockIdx.x * 32 + c;
     float s = 0.f;
     if (d < D)
-        for (int i = g; i < slots; i += 32) s += part[(size_t)i * D + d];
+        for (int i0 = g; i0 < slots; i0 += 8 * 32) {           // eight loads on their way together
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = part[(size_t)min(i0 + 32 * k, slots - 1) * D + d];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (i0 + 32 * k < slots) s += v[k];
+        }
     red[g][c] = s;
     __syncthreads();
     if (g == 0 && d < D) {
