@@ -14,7 +14,7 @@
 // WPR waves share a row (1 up to 1024 elements, 4 above), NCH chunks of 8 elements a lane: D <= WPR·64·8·NCH.
 //
 // Measured (a large copy on this card moves 4.9 TB/s): 14464 x 4096, fp32 stream with delta, e4m3 out: 652 MB in 124 µs, 5.3 TB/s; 3616 x 4096 forward and backward:
-// 415 MB in 82 µs, 5.1 TB/s; 226 x 4096: 11 µs, what a call costs on the host (the kernel itself 3).
+// 415 MB in 79 µs, 5.3 TB/s; 226 x 4096: 11 µs, what a call costs on the host (the kernel itself 4).
 #include "common.hpp"
 #include "../../include/aether_hip.h"
 
