@@ -381,14 +381,15 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(PIPE ||
     if (PIPE && whole >= RB_PIPE_TILES) {
         pipeline(whole);
         if (whole < nkv) sweep(whole, false);
-        float worst = fabsf(l_run);
+        const float l_row = l_run + __shfl_xor(l_run, 32, 64);        // the row's sum: two finite halves may add up to more than fp32 holds
+        float worst = fabsf(l_row);
         if (fabsf(m_run) > RB_FAR_SHIFT) worst = INFINITY;
 #pragma unroll
         for (int i = 0; i < 16; ++i) worst = fmaxf(worst, fmaxf(fabsf(o[0][i]), fabsf(o[1][i])));
         bool bad = !(worst <= 3.4e38f);
 #pragma unroll
         for (int i = 0; i < 16; ++i) bad |= o[0][i] != o[0][i] || o[1][i] != o[1][i];   // (fmaxf passes over a NaN)
-        bad |= l_run != l_run;
+        bad |= l_row != l_row;
         if (__syncthreads_or(bad ? 1 : 0)) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) { o[0][i] = 0.f; o[1][i] = 0.f; }

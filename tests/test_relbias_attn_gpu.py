@@ -341,3 +341,34 @@ def test_graph(cuda, hip_lib):
         want = ops.relbias_attn(q, k, v, table, key_mask=mask)
         torch.cuda.synchronize()
         assert torch.equal(o, want)
+
+
+@pytest.mark.parametrize("S", [600, 1030])
+@pytest.mark.parametrize("apart", [8, 16, 64])
+def test_row_sums_next_to_the_largest_float(cuda, hip_lib, S, apart):
+    """Two keys far above all others, 2^126 ... 2^129 times the row's first scores each: a row's sum lies next to fp32's largest number on either side, with the two keys'
+    shares in one lane or in two (8 keys apart).  Scores are sums of two exact products: 66 · 2^-24 · 90, numerator and denominator each, is below 2^-10."""
+    from aether_amd import ops
+    levels = torch.arange(126.0, 129.01, 0.125, dtype=torch.float64) * math.log(2)
+    B, H, at = len(levels), 1, 200
+    g = torch.Generator().manual_seed(S + apart)
+    q, k = torch.zeros(B, S, H, 64), torch.zeros(B, S, H, 64)
+    q[..., 0], q[..., 1] = 4.0, 1.0
+    coarse = (levels / 4).float().bfloat16()
+    rest = (levels - 4 * coarse.double()).float().bfloat16()
+    for j in (at, at + apart):
+        k[:, j, 0, 0], k[:, j, 0, 1] = coarse.float(), rest.float()
+    v = (torch.rand(B, S, H, 64, generator=g) - 0.5) / 2
+    q, k, v = (t.to(torch.bfloat16).to(cuda) for t in (q, k, v))
+    table = torch.zeros(32, H, dtype=torch.bfloat16, device=cuda)
+    _check_o(ops.relbias_attn(q, k, v, table), q, k, v, table)
+    o, lse = ops.relbias_attn(q, k, v, table, need_lse=True)
+    _, p = _check_o(o, q, k, v, table)
+    level = 4 * coarse.double() + rest.double()
+    want = level / math.log(2) + 1
+    assert bool(((lse[:B * S].view(B, S).double().cpu() - want[:, None]).abs() <= 66 * 2.0 ** -24 * 130).all())
+    do = torch.randn(B, S, H, 64, generator=g).to(torch.bfloat16).to(cuda)
+    dv = ops.relbias_attn_backward(do, q, k, v, o, lse, table)[2]
+    pt, gd = p.transpose(2, 3).contiguous(), do.double().permute(0, 2, 1, 3).contiguous()
+    want, lim = torch.matmul(pt, gd).permute(0, 2, 1, 3), (BF16 + 2.0 ** -10) * torch.matmul(pt, gd.abs()).permute(0, 2, 1, 3)
+    assert bool(((dv.double() - want).abs() <= lim + BF16 * want.abs() + 1e-30).all())
