@@ -317,26 +317,30 @@ __global__ __launch_bounds__(1024) void rms_norm_dw_kernel(const float* __restri
 }
 
 // q = e4m3(x / s), s per row as in the norm above: the form in which gated_ff takes a weight matrix in 8 bits.  One workgroup per row, two passes
-// over it (the second hits the caches); run once when weights are laid out.
-__global__ __launch_bounds__(256) void quantize_rows_kernel(const bf16_t* __restrict__ x, long ldx, u8_t* __restrict__ q, long ldq, float* __restrict__ scale, int K) {
+// over it (the second hits the caches); run once when weights are laid out.  A grid of 2^32 threads or more
+// is cut short without an error, so a workgroup of a large matrix takes several rows.
+constexpr int QUANT_WG = 1 << 20;
+__global__ __launch_bounds__(256) void quantize_rows_kernel(const bf16_t* __restrict__ x, long ldx, u8_t* __restrict__ q, long ldq, float* __restrict__ scale, int rows, int K) {
     __shared__ float red[2][8];
-    const unsigned short* xr = (const unsigned short*)x + (size_t)blockIdx.x * ldx;
     int slot = 0;
-    unsigned top = 0;
-    for (int k = threadIdx.x * 8; k < K; k += 2048) {
-        const u16x8 v = *(const u16x8*)(xr + k);
+    for (int row = blockIdx.x; row < rows; row += gridDim.x) {
+        const unsigned short* xr = (const unsigned short*)x + (size_t)row * ldx;
+        unsigned top = 0;
+        for (int k = threadIdx.x * 8; k < K; k += 2048) {
+            const u16x8 v = *(const u16x8*)(xr + k);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) top = max(top, ((unsigned)v[e] & 0x7fffu) << 16);
-    }
-    top = row_max_u32<4>(top, red, slot, threadIdx.x >> 6);
-    const RowScale s(top);
-    if (threadIdx.x == 0) scale[blockIdx.x] = s.value();
-    for (int k = threadIdx.x * 8; k < K; k += 2048) {
-        const u16x8 v = *(const u16x8*)(xr + k);
-        float f[8];
+            for (int e = 0; e < 8; ++e) top = max(top, ((unsigned)v[e] & 0x7fffu) << 16);
+        }
+        top = row_max_u32<4>(top, red, slot, threadIdx.x >> 6);
+        const RowScale s(top);
+        if (threadIdx.x == 0) scale[row] = s.value();
+        for (int k = threadIdx.x * 8; k < K; k += 2048) {
+            const u16x8 v = *(const u16x8*)(xr + k);
+            float f[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = bf16_bits_to_f32(v[e]);
-        *(uint2*)(q + (size_t)blockIdx.x * ldq + k) = s.pack(f);
+            for (int e = 0; e < 8; ++e) f[e] = bf16_bits_to_f32(v[e]);
+            *(uint2*)(q + (size_t)row * ldq + k) = s.pack(f);
+        }
     }
 }
 
@@ -445,6 +449,6 @@ extern "C" int aether_quantize_rows_e4m3(const void* x, long ldx, void* q, long 
     if (rows == 0) return AETHER_OK;
     if (!x || !q || !scale) return aether_set_error(AETHER_ERR_ARG, "quantize_rows: null operand");
     if (ldx % 8 || ldq % 8 || ((uintptr_t)x & 15) || ((uintptr_t)q & 7)) return aether_set_error(AETHER_ERR_ALIGN, "quantize_rows: rows must be 16-byte (x) and 8-byte (q) aligned");
-    hipLaunchKernelGGL(quantize_rows_kernel, dim3(rows), dim3(256), 0, (hipStream_t)stream, (const bf16_t*)x, ldx, (u8_t*)q, ldq, scale, K);
+    hipLaunchKernelGGL(quantize_rows_kernel, dim3(min(rows, QUANT_WG)), dim3(256), 0, (hipStream_t)stream, (const bf16_t*)x, ldx, (u8_t*)q, ldq, scale, rows, K);
     return aether_check_launch("quantize_rows");
 }

@@ -255,3 +255,14 @@ def test_stream_and_graph(cuda, hip_lib):
         want = (y1, r1, *ops.rms_norm_backward(dy, r1, w, dres=dres, need_ddelta=True))
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip((y, r, *b), want))
+
+
+@pytest.mark.parametrize("rows", [2 ** 24 - 1, 2 ** 24 + 3])
+def test_quantize_many_rows(cuda, hip_lib, rows):
+    """More rows than a launch of one workgroup each can hold."""
+    from aether_amd import ops
+    g = torch.Generator(device=cuda).manual_seed(9)
+    x = torch.randn(rows, 8, generator=g, device=cuda, dtype=torch.bfloat16)
+    q, s = ops.quantize_rows_e4m3(x)
+    assert torch.equal(s, torch.exp2(torch.ceil(torch.log2(x.float().abs().amax(-1).double() / 448))).float())
+    assert torch.equal(q.float(), (x.float() / s[:, None]).to(torch.float8_e4m3fn).float())
