@@ -451,7 +451,9 @@ int rb_setup(RbArgs& p, const AetherRelbias* d) {
     p.c = d->scale * RB_LOG2E;
     p.table = (const bf16_t*)d->table;
     p.mask = (const unsigned char*)d->mask; p.mask_sb = d->mask_sb;
-    if ((long)d->B * d->H * ((d->S + 31) / 32) > 0x7fffffffl) return fail(AETHER_ERR_SHAPE, "relbias_attn: too many query blocks");
+    // a grid of 2^32 threads or more is cut short without an error  (the backward pass takes as many waves or fewer)
+    const int nw = rb_waves(p);
+    if ((size_t)d->B * d->H * ((d->S + nw * 32 - 1) / (nw * 32)) >= (1ull << 32) / (nw * 64)) return fail(AETHER_ERR_SHAPE, "relbias_attn: too many query blocks for one launch");
     if (d->B == 0 || d->S == 0) return AETHER_OK;
     if (!d->table) return fail(AETHER_ERR_ARG, "relbias_attn: null table");
     int rc = rb_tensor(p.q, d->q, d->q_strides, d->S);

@@ -149,7 +149,8 @@ int aether_quantize_rows_e4m3(const void* x, long ldx, void* q, long ldq, float*
  *   S_ij = scale · q_i·k_j + table[bucket(j − i)][h] where key j counts;  O = softmax_j(S) V;  a row without keys gives 0.
  * bucket(d), n = |d|, half = num_buckets / 2, near = half / 2:  (d > 0 ? half : 0) + (n < near ? n : near + #{i : borders[i] <= n}); borders (HOST
  * array of half − near − 1 distances, not falling) is where each bucket behind the first logarithmic one begins, at 1024 or before.
- * q, k, v bf16 [B, S, H, 64] with strides (batch, position, head) in elements, multiples of 8, last dimension dense; S <= 65536.
+ * q, k, v bf16 [B, S, H, 64] with strides (batch, position, head) in elements, multiples of 8, last dimension dense; S <= 65536; B·H below 2^26 for
+ * S <= 32, 2^25 for S <= 64, B·H·⌈S / 128⌉ below 2^24 above (one launch).
  * table bf16 [num_buckets, H]; mask: bytes [B, S] with batch stride mask_sb, 0 = the key does not count, or NULL.  What stands at a key that does not
  * count (NaN, infinities) reaches no output.  scale is 0 or of a magnitude in [1e-20, 1e20]; |v| up to 1e22 (weighted sums are held in fp32 before they are
  * normalized); table entries of -inf or the lowest value switch a bucket off. */

@@ -195,3 +195,18 @@ def test_gated_ff_backward_entry_refuses(hip_lib, kw, code, text):
 def test_gated_ff_entries_without_rows(hip_lib):
     assert hip_lib.aether_gated_ff(None, 128, None, None, 128, None, 64, None, 0, 64, 128, 0, None) == 0
     assert hip_lib.aether_gated_ff_e4m3(None, 128, None, None, None, None, None, 128, None, 64, 0, 64, 128, 0, None) == 0
+
+
+@pytest.mark.parametrize("kw,refused", [(dict(B=1 << 20, H=64, S=1), True), (dict(B=(1 << 20) - 1, H=64, S=1), False), (dict(B=1 << 18, H=128, S=40), True),
+                                        (dict(B=1 << 14, H=64, S=2000), True), (dict(B=1 << 26, H=1, S=32), True), (dict(B=(1 << 25), H=1, S=64), True),
+                                        (dict(B=(1 << 25) - 1, H=1, S=64), False)])
+def test_relbias_grids_beyond_a_launch(hip_lib, kw, refused):
+    """A grid of 2^32 threads or more would be cut short: such calls are refused, forward and backward.  (The others come as far as the missing output.)"""
+    import ctypes as C
+    from aether_amd import _lib
+    text = b"blocks" if refused else b"output"
+    assert _relbias(hip_lib, o=None, st=(0, 64, 0), **kw) == (-2 if refused else -1) and text in hip_lib.aether_last_error()
+    st = (0, 64, 0)
+    b = (C.c_int * 7)(12, 16, 23, 32, 46, 64, 91)
+    d = _lib.AetherRelbias(4096, 4096, 4096, st, st, st, 4096, None, 0, kw["B"], kw["S"], kw["H"], 1.0, 32, b, 7)
+    assert (hip_lib.aether_relbias_attn_bwd_workspace_bytes(C.byref(d), 1) == 0) == refused

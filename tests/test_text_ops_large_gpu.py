@@ -109,3 +109,16 @@ def test_rows_far_apart(cuda, hip_lib):
     lim = 2 * BF16 * want.float().abs() + 2 * 128 * 2.0 ** -24 * (1.2 * A[0] * gu[:, F:].abs() + A[1] * gu[:, :F].abs())
     assert bool(((h.float() - want.float()).abs() <= lim).all())
     assert all(torch.equal(a, b) for a, b in zip(ops.gated_ff_backward(h, wide, wg, wu, gu), ops.gated_ff_backward(h, x, wg, wu, gu)))
+
+
+def test_the_most_batch_items_of_a_launch(cuda, hip_lib):
+    """2^26 - 64 heads of one token each: every one gets its only value.  One batch item more is refused."""
+    from aether_amd import ops
+    B, H = 2 ** 20 - 1, 64
+    g = torch.Generator(device=cuda).manual_seed(5)
+    v = torch.randn(B + 1, 1, H, 64, generator=g, device=cuda, dtype=torch.bfloat16)
+    one = torch.ones(1, 1, 1, 64, dtype=torch.bfloat16, device=cuda).expand(B + 1, 1, H, 64)
+    table = torch.zeros(32, H, dtype=torch.bfloat16, device=cuda)
+    assert torch.equal(ops.relbias_attn(one[:B], one[:B], v[:B], table), v[:B])
+    with pytest.raises(ValueError, match="blocks"):
+        ops.relbias_attn(one, one, v, table)
