@@ -32,7 +32,7 @@ class _RmsNorm(torch.autograd.Function):
         if dy is None and dres is None:
             return None, None, None, None
         if dy is None:                      # only the sum was used
-            return dres if need_x else None, dres.to(torch.bfloat16) if need_delta else None, torch.zeros_like(w) if need_w else None, None
+            return dres if need_x else None, dres.to(torch.bfloat16, copy=True) if need_delta else None, torch.zeros_like(w) if need_w else None, None
         dx, ddelta, dw = ops.rms_norm_backward(dy, res, w, ctx.eps, dres=dres, need_ddelta=need_delta, delta=delta)
         return dx if need_x else None, ddelta, dw if need_w else None, None
 

@@ -246,8 +246,7 @@ def rms_norm_backward(dy, res, w, eps=1e-6, dres=None, need_ddelta=False, delta=
     d2 = None if delta is None else _rows(delta, D)
     rows = r2.shape[0]
     dx = _like(res, res.dtype)
-    # with a bf16 stream the rounded dx IS ddelta
-    ddelta = _like(res, torch.bfloat16) if need_ddelta and res.dtype != torch.bfloat16 else None
+    ddelta = _like(res, torch.bfloat16) if need_ddelta else None      # (a bf16 stream's dx again, in memory of its own: either may be changed in place)
     dw = _like(w, torch.float32)
     lib = _lib.load()
     nbytes = lib.aether_rms_norm_bwd_workspace_bytes(rows, D)
@@ -255,7 +254,7 @@ def rms_norm_backward(dy, res, w, eps=1e-6, dres=None, need_ddelta=False, delta=
     _run("rms_norm_backward", dev, lib.aether_rms_norm_bwd, g2.data_ptr(), g2.stride(0), r2.data_ptr(), _STREAMS[res.dtype], r2.stride(0),
          _lib.ptr(d2), d2.stride(0) if d2 is not None else 0, _lib.ptr(s2), s2.stride(0) if s2 is not None else 0, w.data_ptr(), float(eps), dx.data_ptr(), D, _lib.ptr(ddelta), D, dw.data_ptr(), rows, D,
          ws.data_ptr(), nbytes)
-    return dx, (dx if res.dtype == torch.bfloat16 else ddelta) if need_ddelta else None, dw
+    return dx, ddelta, dw
 
 
 def quantize_rows_e4m3(x):

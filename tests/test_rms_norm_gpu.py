@@ -266,3 +266,26 @@ def test_quantize_many_rows(cuda, hip_lib, rows):
     q, s = ops.quantize_rows_e4m3(x)
     assert torch.equal(s, torch.exp2(torch.ceil(torch.log2(x.float().abs().amax(-1).double() / 448))).float())
     assert torch.equal(q.float(), (x.float() / s[:, None]).to(torch.float8_e4m3fn).float())
+
+
+@pytest.mark.parametrize("stream", [torch.float32, torch.bfloat16])
+def test_gradients_do_not_share_memory(cuda, hip_lib, stream):
+    """dx and ddelta are tensors of their own: scaling one in place leaves the other as it was."""
+    from aether_amd import functional, ops
+    x, delta, w, dy, dres = _inputs(19, 520, stream, seed=8, cuda=cuda)
+    dx, ddelta, _ = ops.rms_norm_backward(dy, x, w, dres=dres, need_ddelta=True, delta=delta)
+    keep = ddelta.clone()
+    dx.mul_(0.5)
+    assert torch.equal(ddelta, keep)
+    leaves = [t.clone().requires_grad_(True) for t in (x, delta)]
+    y, h = functional.rms_norm(leaves[0], w, delta=leaves[1])
+    a, b = torch.autograd.grad([y, h], leaves, [dy, dres])
+    a.mul_(0.5)
+    assert torch.equal(b, keep)
+    # only the sum is used
+    y, h = functional.rms_norm(leaves[0], w, delta=leaves[1])
+    keep = dres.bfloat16().clone()
+    a, b = torch.autograd.grad(h, leaves, dres)
+    assert torch.equal(a, dres) and torch.equal(b, keep)
+    a.mul_(0.5)
+    assert torch.equal(b, keep)
