@@ -739,6 +739,7 @@ extern "C" int aether_gated_ff_bwd(const void* dh, long lddh, const void* x, lon
     if (M == 0) return aether_set_error(AETHER_ERR_SHAPE, "gated_ff_bwd: no rows");
     if (lddh < F || lddh % 8 || (dx && (lddx < K || lddx % 8)) || (((uintptr_t)dh | (uintptr_t)gu | (uintptr_t)dx | (uintptr_t)dw | (uintptr_t)workspace) & 15))
         return aether_set_error(AETHER_ERR_ALIGN, "gated_ff_bwd: rows must be 16-byte aligned");
+    if (dx && lddx > 0x7fffffffl) return aether_set_error(AETHER_ERR_SHAPE, "gated_ff_bwd: a row of dx is too far from the next (aether_gemm_bf16 takes 32 bits)");
     const size_t Mp = ((size_t)M + 63) / 64 * 64;
     if (Mp * 2 * F * 2 >= (1ull << 32) || (size_t)2 * F * K * 2 >= (1ull << 32)) return aether_set_error(AETHER_ERR_SHAPE, "gated_ff_bwd: M·2F and 2F·K elements must stay below 4 GiB");
     if (!workspace || workspace_bytes < aether_gated_ff_bwd_workspace_bytes(M, F, K)) return aether_set_error(AETHER_ERR_ARG, "gated_ff_bwd: workspace too small (aether_gated_ff_bwd_workspace_bytes)");

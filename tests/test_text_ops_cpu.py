@@ -210,3 +210,11 @@ def test_relbias_grids_beyond_a_launch(hip_lib, kw, refused):
     b = (C.c_int * 7)(12, 16, 23, 32, 46, 64, 91)
     d = _lib.AetherRelbias(4096, 4096, 4096, st, st, st, 4096, None, 0, kw["B"], kw["S"], kw["H"], 1.0, 32, b, 7)
     assert (hip_lib.aether_relbias_attn_bwd_workspace_bytes(C.byref(d), 1) == 0) == refused
+
+
+def test_gated_ff_backward_refuses_a_row_stride_beyond_32_bits(hip_lib):
+    """The product behind dx takes its row stride as 32 bits: one that would be cut is refused before anything is enqueued."""
+    a = {**_FF, **dict(M=70000, F=64)}
+    lddx = (1 << 32) + 128
+    rc = hip_lib.aether_gated_ff_bwd(4096, 64, a["x"], a["ldx"], a["wg"], a["wu"], a["ldw"], 4096, 4096, lddx, None, a["M"], a["F"], a["K"], 0, 4096, 1 << 40, None)
+    assert rc == -2 and b"too far" in hip_lib.aether_last_error()
