@@ -406,7 +406,7 @@ template <int ACT>
 __global__ __launch_bounds__(256) void gated_ff_dgu_kernel(const float* __restrict__ gu, const bf16_t* __restrict__ dh, long lddh, int M, int F, int Mp,
                                                            bf16_t* __restrict__ dgu, bf16_t* __restrict__ dgut) {
     __shared__ unsigned short t[2][64][66];
-    const int m0 = blockIdx.y * 64, f0 = blockIdx.x * 64;
+    const int nf = (F + 63) / 64, m0 = blockIdx.x / nf * 64, f0 = blockIdx.x % nf * 64;   // (one axis: the others hold 65535 pieces)
     for (int i = threadIdx.x; i < 64 * 16; i += 256) {                // four columns at a time
         const int r = i >> 4, c = (i & 15) * 4, m = m0 + r, f = f0 + c;
         unsigned short g4[4] = {0, 0, 0, 0}, u4[4] = {0, 0, 0, 0};
@@ -441,7 +441,7 @@ __global__ __launch_bounds__(256) void gated_ff_dgu_kernel(const float* __restri
 // out[c][r] = in[r][c] for r < rows, 0 for rows <= r < fill
 __global__ __launch_bounds__(256) void transpose_bf16_kernel(const bf16_t* __restrict__ in, long ldi, int rows, int cols, bf16_t* __restrict__ out, long ldo, int fill) {
     __shared__ unsigned short t[64][66];
-    const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
+    const int nc = (cols + 63) / 64, r0 = blockIdx.x / nc * 64, c0 = blockIdx.x % nc * 64;
     for (int i = threadIdx.x; i < 64 * 16; i += 256) {
         const int r = i >> 4, c = (i & 15) * 4;
         u16x4 v = {0, 0, 0, 0};
@@ -741,7 +741,7 @@ extern "C" int aether_gated_ff_bwd(const void* dh, long lddh, const void* x, lon
         return aether_set_error(AETHER_ERR_ALIGN, "gated_ff_bwd: rows must be 16-byte aligned");
     if (dx && lddx > 0x7fffffffl) return aether_set_error(AETHER_ERR_SHAPE, "gated_ff_bwd: a row of dx is too far from the next (aether_gemm_bf16 takes 32 bits)");
     const size_t Mp = ((size_t)M + 63) / 64 * 64;
-    if (Mp * 2 * F * 2 >= (1ull << 32) || (size_t)2 * F * K * 2 >= (1ull << 32)) return aether_set_error(AETHER_ERR_SHAPE, "gated_ff_bwd: M·2F and 2F·K elements must stay below 4 GiB");
+    if (Mp * 2 * F * 2 >= (1ull << 32) || (size_t)2 * F * K * 2 >= (1ull << 32)) return aether_set_error(AETHER_ERR_SHAPE, "gated_ff_bwd: M·2F and 2F·K elements of 16 bits must stay below 4 GiB each");
     if (!workspace || workspace_bytes < aether_gated_ff_bwd_workspace_bytes(M, F, K)) return aether_set_error(AETHER_ERR_ARG, "gated_ff_bwd: workspace too small (aether_gated_ff_bwd_workspace_bytes)");
     hipStream_t s = (hipStream_t)stream;
     auto up = [](char* p) { return (char*)(((uintptr_t)p + 255) & ~(uintptr_t)255); };
@@ -750,7 +750,8 @@ extern "C" int aether_gated_ff_bwd(const void* dh, long lddh, const void* x, lon
     bf16_t* dgut = (bf16_t*)w; w = up(w + 2 * (size_t)F * Mp * 2);
     bf16_t* xt = (bf16_t*)w; w = up(w + (size_t)K * Mp * 2);
     bf16_t* wt = (bf16_t*)w;
-    const dim3 eg((F + 63) / 64, (unsigned)(Mp / 64));
+    auto pieces = [](size_t rows, size_t cols) { return dim3((unsigned)((rows + 63) / 64 * ((cols + 63) / 64))); };   // of 64 x 64
+    const dim3 eg = pieces(M, F);
     if (act == ACT_SILU) hipLaunchKernelGGL((gated_ff_dgu_kernel<ACT_SILU>), eg, dim3(256), 0, s, gu, (const bf16_t*)dh, lddh, M, F, (int)Mp, dgu, dgut);
     else hipLaunchKernelGGL((gated_ff_dgu_kernel<ACT_GELU_TANH>), eg, dim3(256), 0, s, gu, (const bf16_t*)dh, lddh, M, F, (int)Mp, dgu, dgut);
     rc = aether_check_launch("gated_ff_bwd");
@@ -778,15 +779,19 @@ extern "C" int aether_gated_ff_bwd(const void* dh, long lddh, const void* x, lon
             rc = aether_check_launch("ff_dx_join");
         }
     } else if (!rc && dx) {
-        hipLaunchKernelGGL(transpose_bf16_kernel, dim3((K + 63) / 64, (F + 63) / 64), dim3(256), 0, s, (const bf16_t*)wg, ldw, F, K, wt, 2 * (long)F, F);
-        hipLaunchKernelGGL(transpose_bf16_kernel, dim3((K + 63) / 64, (F + 63) / 64), dim3(256), 0, s, (const bf16_t*)wu, ldw, F, K, wt + F, 2 * (long)F, F);
+        hipLaunchKernelGGL(transpose_bf16_kernel, pieces(F, K), dim3(256), 0, s, (const bf16_t*)wg, ldw, F, K, wt, 2 * (long)F, F);
+        hipLaunchKernelGGL(transpose_bf16_kernel, pieces(F, K), dim3(256), 0, s, (const bf16_t*)wu, ldw, F, K, wt + F, 2 * (long)F, F);
         rc = aether_check_launch("gated_ff_bwd (weights turned)");
         if (!rc) rc = aether_gemm_bf16(dgu, 2 * F, wt, 2 * F, dx, (int)lddx, M, K, 2 * F, nullptr, AETHER_EPI_BIAS, nullptr, 0, nullptr, nullptr, 0, 0, 0, nullptr, 0, 0, stream);
     }
     if (!rc && dw) {
-        hipLaunchKernelGGL(transpose_bf16_kernel, dim3((K + 63) / 64, (unsigned)(Mp / 64)), dim3(256), 0, s, (const bf16_t*)x, ldx, M, K, xt, (long)Mp, (int)Mp);
+        hipLaunchKernelGGL(transpose_bf16_kernel, pieces(M, K), dim3(256), 0, s, (const bf16_t*)x, ldx, M, K, xt, (long)Mp, (int)Mp);
         rc = aether_check_launch("gated_ff_bwd (input turned)");
-        if (!rc) rc = aether_gemm_bf16(dgut, (int)Mp, xt, (int)Mp, dw, K, 2 * F, K, (int)Mp, nullptr, AETHER_EPI_BIAS, nullptr, 0, nullptr, nullptr, 0, 0, 0, nullptr, 0, 0, stream);
+        // columns in launches whose part of the turned x a buffer descriptor reaches: whole tiles of them, and 64 at least (Mp is below 2^25)
+        const size_t reach = ((1ull << 32) - 1) / (2 * Mp), most = std::min((size_t)K, reach >= 256 ? reach / 256 * 256 : reach / 64 * 64);
+        for (size_t c = 0; !rc && c < (size_t)K; c += most)
+            rc = aether_gemm_bf16(dgut, (int)Mp, xt + c * Mp, (int)Mp, (bf16_t*)dw + c, K, 2 * F, (int)std::min(most, (size_t)K - c), (int)Mp, nullptr, AETHER_EPI_BIAS, nullptr, 0, nullptr, nullptr, 0, 0, 0,
+                                  nullptr, 0, 0, stream);
     }
     return rc;
 }

@@ -186,7 +186,8 @@ int aether_gated_ff(const void* x, long ldx, const void* wg, const void* wu, lon
 /* Operands in e4m3 with one fp32 scale per row of x [M], wg [F], wu [F] (aether_rms_norm, aether_quantize_rows_e4m3). */
 int aether_gated_ff_e4m3(const void* x, long ldx, const float* x_scale, const void* wg, const float* wg_scale, const void* wu, const float* wu_scale, long ldw,
                          void* h, long ldh, int M, int F, int K, int act, void* stream);
-/* Backward pass, M > 0: dx bf16 [M, K]; dw bf16 [2F, K] dense, the gradient of wg and then that of wu; either may be NULL.  dh bf16 [M, F]; gu as the forward pass wrote it. */
+/* Backward pass, M > 0: dx bf16 [M, K]; dw bf16 [2F, K] dense, the gradient of wg and then that of wu; either may be NULL.  dh bf16 [M, F]; gu as the forward pass wrote it.
+ * ⌈M / 64⌉·64·2F and 2F·K stay below 2^31. */
 size_t aether_gated_ff_bwd_workspace_bytes(int M, int F, int K);
 int aether_gated_ff_bwd(const void* dh, long lddh, const void* x, long ldx, const void* wg, const void* wu, long ldw, const float* gu, void* dx, long lddx,
                         void* dw, int M, int F, int K, int act, void* workspace, size_t workspace_bytes, void* stream);

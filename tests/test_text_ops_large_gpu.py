@@ -122,3 +122,48 @@ def test_the_most_batch_items_of_a_launch(cuda, hip_lib):
     assert torch.equal(ops.relbias_attn(one[:B], one[:B], v[:B], table), v[:B])
     with pytest.raises(ValueError, match="blocks"):
         ops.relbias_attn(one, one, v, table)
+
+
+def _check_ff_gradients(dh, x, wg, wu, gu, got, rows, cols):
+    """dx of some rows and the weights' gradients of some columns, bounds as in test_gated_ff_gpu.py; g and u are the stored projections."""
+    M, F = dh.shape
+    dx, dwg, dwu = got
+    cat = torch.cat([wg, wu]).double()
+    F64 = torch.float64
+    sum_g, sum_u, lim_g, lim_u = (torch.zeros(F, len(cols), dtype=F64, device=x.device) for _ in range(4))
+    for m in range(0, M, 1 << 18):
+        g = gu[m:m + (1 << 18), :F].double().requires_grad_(True)
+        u, d = gu[m:m + (1 << 18), F:].double(), dh[m:m + (1 << 18)].double()
+        a = torch.nn.functional.gelu(g, approximate="tanh")
+        dg = torch.autograd.grad((a * u * d).sum(), g)[0]
+        du, xc = (d * a).detach(), x[m:m + (1 << 18)][:, cols].double()
+        eg, eu = (2.0 ** -14 * (d * u).abs() + BF16 * dg.abs()), 2.0 ** -14 * (d * g.detach()).abs() + BF16 * du.abs()
+        t = lambda z: z.t().contiguous()  # noqa: E731
+        sum_g += t(dg) @ xc
+        sum_u += t(du) @ xc
+        lim_g += t(eg + M * 2.0 ** -24 * dg.abs()) @ xc.abs()
+        lim_u += t(eu + M * 2.0 ** -24 * du.abs()) @ xc.abs()
+        here = [r for r in rows if m <= r < m + (1 << 18)]
+        if here and dx is not None:
+            i = torch.tensor(here, device=x.device) - m
+            both, e = torch.cat([dg[i], du[i]], 1), torch.cat([eg[i], eu[i]], 1)
+            want = both @ cat
+            assert bool(((dx[i + m].double() - want).abs() <= (e + 2 * F * 2.0 ** -24 * both.abs()) @ cat.abs() + BF16 * want.abs()).all())
+    for grad, want, lim in ((dwg, sum_g, lim_g), (dwu, sum_u, lim_u)):
+        assert bool(((grad[:, cols].double() - want).abs() <= lim + BF16 * want.abs()).all())
+
+
+@pytest.mark.parametrize("M,K,F", [(131072 + 40, 16384, 256), (4200001, 64, 32)])
+def test_feed_forward_gradients_of_many_rows(cuda, hip_lib, M, K, F):
+    """x of more than 4 GiB, whose turned copy is an operand of the weights' gradients; and more than 65535 blocks of 64 rows."""
+    from aether_amd import ops
+    g = torch.Generator(device=cuda).manual_seed(6)
+    r = lambda *s: torch.randn(*s, generator=g, device=cuda, dtype=torch.bfloat16)  # noqa: E731
+    x, wg, wu, dh = r(M, K), r(F, K) * K ** -0.5, r(F, K) * K ** -0.5, r(M, F)
+    _, gu = ops.gated_ff(x, wg, wu, need_gu=True)
+    got = ops.gated_ff_backward(dh, x, wg, wu, gu)
+    assert all(bool(torch.isfinite(t).all()) for t in got)
+    cols = torch.tensor([0, 1, 31, K // 2, K - 65 if K > 64 else 40, K - 64, K - 1], device=cuda)
+    _check_ff_gradients(dh, x, wg, wu, gu, got, [0, 63, 64, 65536, 131071, M - 65, M - 64, M - 1], cols)
+    frozen = ops.gated_ff_backward(dh, x, wg, wu, gu, need_dw=False)
+    assert torch.equal(frozen[0], got[0]) and frozen[1] is None
