@@ -618,6 +618,14 @@ static int ff_check(const void* x, long ldx, const void* wg, const void* wu, lon
     return AETHER_OK;
 }
 
+// what the products of the backward pass reach; asked for where the projections are written, too
+static int ff_bwd_check(int M, int F, int K) {
+    const size_t Mp = ((size_t)M + 63) / 64 * 64;
+    if (Mp * 2 * F * 2 >= (1ull << 32) || (size_t)2 * F * K * 2 >= (1ull << 32))
+        return aether_set_error(AETHER_ERR_SHAPE, "gated_ff: the backward pass takes M·2F and 2F·K elements of 16 bits below 4 GiB each");
+    return AETHER_OK;
+}
+
 // Which kernel, from the sizes alone.  A tile kernel runs its workgroups in rounds of one a CU; a round's time is that of one workgroup's K loop, measured per
 // K tile of 128 bytes (K = 4096, F = 1024 ... 10240, µs): 64 x 64 (rows x pairs of columns) 0.42, 128 x 64 0.6, 128 x 128 and 256 x 64 0.9, the 256 x 128
 // kernel with alternating waves 1.45.  The least rounds x time wins; for instance, bf16, F = 10240: 64 rows 36 µs (256 x 128: 91), 128 rows 44 (91), 226 rows
@@ -710,6 +718,7 @@ extern "C" int aether_gated_ff(const void* x, long ldx, const void* wg, const vo
     if (rc || M == 0) return rc;
     if (!h) return aether_set_error(AETHER_ERR_ARG, "gated_ff: null output");
     if (ldh < F || ldh % 8 || (((uintptr_t)h | (uintptr_t)gu) & 15)) return aether_set_error(AETHER_ERR_ALIGN, "gated_ff: rows of the output must be 16-byte aligned");
+    if (gu && (rc = ff_bwd_check(M, F, K)) != AETHER_OK) return rc;
     FfArgs p = {x, ldx, wg, wu, ldw, nullptr, nullptr, nullptr, (bf16_t*)h, ldh, gu, M, F, K};
     return ff_forward<bf16_t>(p, act, (hipStream_t)stream);
 }
@@ -740,8 +749,9 @@ extern "C" int aether_gated_ff_bwd(const void* dh, long lddh, const void* x, lon
     if (lddh < F || lddh % 8 || (dx && (lddx < K || lddx % 8)) || (((uintptr_t)dh | (uintptr_t)gu | (uintptr_t)dx | (uintptr_t)dw | (uintptr_t)workspace) & 15))
         return aether_set_error(AETHER_ERR_ALIGN, "gated_ff_bwd: rows must be 16-byte aligned");
     if (dx && lddx > 0x7fffffffl) return aether_set_error(AETHER_ERR_SHAPE, "gated_ff_bwd: a row of dx is too far from the next (aether_gemm_bf16 takes 32 bits)");
+    rc = ff_bwd_check(M, F, K);
+    if (rc) return rc;
     const size_t Mp = ((size_t)M + 63) / 64 * 64;
-    if (Mp * 2 * F * 2 >= (1ull << 32) || (size_t)2 * F * K * 2 >= (1ull << 32)) return aether_set_error(AETHER_ERR_SHAPE, "gated_ff_bwd: M·2F and 2F·K elements of 16 bits must stay below 4 GiB each");
     if (!workspace || workspace_bytes < aether_gated_ff_bwd_workspace_bytes(M, F, K)) return aether_set_error(AETHER_ERR_ARG, "gated_ff_bwd: workspace too small (aether_gated_ff_bwd_workspace_bytes)");
     hipStream_t s = (hipStream_t)stream;
     auto up = [](char* p) { return (char*)(((uintptr_t)p + 255) & ~(uintptr_t)255); };

@@ -84,7 +84,8 @@ class _GatedFf(torch.autograd.Function):
 
 
 def gated_ff(x, wg, wu, act="gelu_tanh"):
-    """`ops.gated_ff` with gradients for x, wg and wu."""
+    """`ops.gated_ff` with gradients for x, wg and wu.  More rows than the backward pass takes (rows · 2F of 2^31) are refused here; without gradients
+    `ops.gated_ff` has no such limit."""
     return _GatedFf.apply(x, wg, wu, act)
 
 

@@ -408,7 +408,7 @@ def _ff_operands(name, x, wg, wu, act, dtype):
 def gated_ff(x, wg, wu, act="gelu_tanh", need_gu=False):
     """h = act(x wgᵀ) ⊙ (x wuᵀ): both projections, the activation and the product in one kernel.  x bfloat16 [..., K], wg and wu bfloat16 [F, K], K a multiple
     of 64, F of 32; act "gelu_tanh" or "silu".  -> h bfloat16 [..., F]; with need_gu (h, gu), where gu float32 [rows, 2F] holds both projections for
-    `gated_ff_backward`."""
+    `gated_ff_backward`; that takes rows · 2F (rows rounded up to 64) and 2F · K below 2^31, and need_gu is refused beyond."""
     dev = _same_device(x, wg, wu)
     x2, wg, wu, F, K = _ff_operands("gated_ff", x, wg, wu, act, torch.bfloat16)
     M = x2.shape[0]

@@ -179,7 +179,7 @@ int aether_relbias_attn_bwd(const AetherRelbias* d, const void* go, const long* 
 
 /* Gated feed-forward product: h = act(x·Wgᵀ) ⊙ (x·Wuᵀ).  x [M, K], wg and wu [F, K] (one leading dimension, elements), h bf16 [M, F] (ldh % 8 == 0).
  * F % 32 == 0; K % 64 == 0 (bf16) or K % 128 == 0 (e4m3); rows 16-byte aligned; a weight below 4 GiB.  gu: fp32 [M][2F], x·Wgᵀ then x·Wuᵀ, for the backward
- * pass, or NULL. */
+ * pass, or NULL; given only for sizes that the backward pass takes. */
 #define AETHER_ACT_GELU_TANH 0
 #define AETHER_ACT_SILU 1
 int aether_gated_ff(const void* x, long ldx, const void* wg, const void* wu, long ldw, void* h, long ldh, float* gu, int M, int F, int K, int act, void* stream);

@@ -218,3 +218,14 @@ def test_gated_ff_backward_refuses_a_row_stride_beyond_32_bits(hip_lib):
     lddx = (1 << 32) + 128
     rc = hip_lib.aether_gated_ff_bwd(4096, 64, a["x"], a["ldx"], a["wg"], a["wu"], a["ldw"], 4096, 4096, lddx, None, a["M"], a["F"], a["K"], 0, 4096, 1 << 40, None)
     assert rc == -2 and b"too far" in hip_lib.aether_last_error()
+
+
+@pytest.mark.parametrize("kw", [dict(M=1 << 25, F=32, K=64), dict(M=104896, F=10240, K=4096, ldx=4096, ldw=4096, ldh=10240), dict(F=8192, K=131072, ldx=131072, ldw=131072, ldh=8192)])
+def test_gated_ff_refuses_projections_that_have_no_backward_pass(hip_lib, kw):
+    """What the backward pass does not take is refused where its projections are asked for, not after the forward pass has run."""
+    a = {**_FF, **kw}
+    text = b"4 GiB"
+    rc = hip_lib.aether_gated_ff_bwd(4096, a["F"], a["x"], a["ldx"], a["wg"], a["wu"], a["ldw"], 4096, 4096, a["ldx"], 4096, a["M"], a["F"], a["K"], 0, 4096, 1 << 60, None)
+    assert rc == -2 and text in hip_lib.aether_last_error()
+    rc = hip_lib.aether_gated_ff(a["x"], a["ldx"], a["wg"], a["wu"], a["ldw"], a["h"], a["ldh"], 4096, a["M"], a["F"], a["K"], 0, None)
+    assert rc == -2 and text in hip_lib.aether_last_error()
