@@ -7,7 +7,8 @@ The reference fills the slot with transformers' `T5EncoderModel` (/root/referenc
     h, y = rms_norm(h + delta);  delta = gated_ff(y; Wg, Wu) Wdᵀ
 
 on the HIP kernels of libaether_hip.so: the residual stream h stays in fp32, everything between is bf16, one bias table serves all blocks.  Gradients
-(prompt tuning through `inputs_embeds`, fine-tuning of any parameter) go through `aether_amd.functional`.  There is no PyTorch fallback.
+(prompt tuning through `inputs_embeds`, fine-tuning of any parameter) go through `aether_amd.functional`; forward-mode derivatives are refused.  There is no
+PyTorch fallback.
 """
 from __future__ import annotations
 
@@ -18,6 +19,7 @@ from typing import Dict, Optional
 
 import torch
 from torch import nn
+from torch.autograd import forward_ad
 
 from . import _lib, functional, ops
 
@@ -197,6 +199,8 @@ class AetherTextEncoder(nn.Module):
             attention_mask = attention_mask.to(h.device) != 0
         if h.numel() == 0:
             return (h.to(torch.bfloat16),)
+        if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in (h, *self.parameters())):
+            raise ValueError("the text encoder has no forward-mode derivatives (the kernels would drop the tangent)")
         grad = torch.is_grad_enabled() and (h.requires_grad or any(p.requires_grad for p in self.parameters()))
         if grad and self._e4m3 is not None:
             raise ValueError("the 8-bit feed-forward has no gradients: run under torch.no_grad(), or without quantize_feed_forward()")

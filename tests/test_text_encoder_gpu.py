@@ -272,3 +272,23 @@ def test_pipeline_slot(cuda, hip_lib, world):
     with torch.no_grad():
         want, eager = world.t64(ids)[0], world.t16(ids)[0]
     assert _rel(emb[:1], want) <= 1.5 * _rel(eager, want) + 5e-3
+
+
+def test_forward_mode_derivatives_are_refused(cuda, world):
+    """A tangent has nowhere to go in the kernels: refused for frozen weights too, where nothing else asks for derivatives."""
+    import torch.autograd.forward_ad as fwd
+    m = world.native_frozen
+    e = torch.randn(1, 9, KW["d_model"], generator=torch.Generator().manual_seed(10)).to(cuda)
+    want = m(inputs_embeds=e)[0]
+    with fwd.dual_level():
+        with pytest.raises((ValueError, RuntimeError), match="forward-mode"):
+            m(inputs_embeds=fwd.make_dual(e, torch.ones_like(e)))
+        assert torch.equal(m(inputs_embeds=e)[0], want)
+        ids = _ids(1, 9, 11).to(cuda)
+        for name in ("final_norm", "bias_table", "embedding"):
+            p = getattr(m, name).detach()
+            with pytest.raises((ValueError, RuntimeError), match="forward-mode"):
+                torch.func.functional_call(m, {name: fwd.make_dual(p, torch.ones_like(p))}, (ids,))
+    with pytest.raises((ValueError, RuntimeError)):
+        torch.func.jvp(lambda t: m(inputs_embeds=t)[0], (e,), (torch.ones_like(e),))
+    assert torch.equal(m(inputs_embeds=e)[0], want)
