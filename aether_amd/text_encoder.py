@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import json
 import os
+import warnings
 from types import SimpleNamespace
 from typing import Dict, Optional
 
@@ -93,6 +94,8 @@ class AetherTextEncoder(nn.Module):
     @torch.no_grad()
     def load_t5_state_dict(self, sd: Dict[str, torch.Tensor]):
         """Packs a state dict with T5EncoderModel's keys into this module's parameters."""
+        self._drop_e4m3()                                       # (first: a dict that is refused halfway has changed some weights)
+
         def put(param, *keys):
             rows = 0
             for key in keys:
@@ -114,12 +117,12 @@ class AetherTextEncoder(nn.Module):
             put(b.up, ff + "DenseReluDense.wi_1.weight")
             put(b.down, ff + "DenseReluDense.wo.weight")
         put(self.final_norm, "encoder.final_layer_norm.weight")
-        self._e4m3 = None
         return self
 
     @torch.no_grad()
     def init_random_weights(self, seed: int = 0):
         """Seeded random weights of the trained model's scales (no checkpoint: smoke runs, benchmarks, tests)."""
+        self._drop_e4m3()
         g = torch.Generator(device=self.embedding.device).manual_seed(seed)
         c = self.config
         inner = c.num_heads * c.d_kv
@@ -139,14 +142,14 @@ class AetherTextEncoder(nn.Module):
             normal(b.up, c.d_model ** -0.5)
             normal(b.down, c.d_ff ** -0.5)
         self.final_norm.fill_(1.0)
-        self._e4m3 = None
         return self
 
     # ------------------------------------------------------------------------------------------
     @torch.no_grad()
     def quantize_feed_forward(self):
         """Serve the feed-forward's two input projections (half of a block's weights) in e4m3: half their bytes, twice the matrix rate, for an error of
-        e4m3's rounding (2^-4) on each factor.  The 16-bit weights stay as they are; call it again after changing them.  No gradients in this form."""
+        e4m3's rounding (2^-4) on each factor.  The 16-bit weights stay as they are; call it again after changing them.  Moving the module
+        (`to`, also to where it is) or loading weights ends this form, with a warning.  No gradients in it."""
         if self.config.d_model % 128:
             raise ValueError("aether_amd: d_model must be a multiple of 128 for 8-bit operands")
         self._e4m3 = [(*ops.quantize_rows_e4m3(b.gate.detach()), *ops.quantize_rows_e4m3(b.up.detach())) for b in self.blocks]
@@ -154,8 +157,13 @@ class AetherTextEncoder(nn.Module):
 
     # the 8-bit weights are laid out for where and what the weights were
 
-    def _apply(self, fn, *args, **kwargs):
+    def _drop_e4m3(self):
+        if self._e4m3 is not None:
+            warnings.warn("the text encoder's weights were moved or loaded: its 8-bit feed-forward is gone, the 16-bit one serves; call quantize_feed_forward() again", stacklevel=3)
         self._e4m3 = None
+
+    def _apply(self, fn, *args, **kwargs):
+        self._drop_e4m3()
         return super()._apply(fn, *args, **kwargs)
 
     def load_state_dict(self, *args, **kwargs):
@@ -163,7 +171,7 @@ class AetherTextEncoder(nn.Module):
         return super().load_state_dict(*args, **kwargs)
 
     def _load_from_state_dict(self, *args, **kwargs):        # (a module around this one comes in here)
-        self._e4m3 = None
+        self._drop_e4m3()
         return super()._load_from_state_dict(*args, **kwargs)
 
     # ------------------------------------------------------------------------------------------

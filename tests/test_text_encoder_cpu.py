@@ -76,3 +76,29 @@ def test_loading_drops_the_eight_bit_copies(hip_lib):
         m._e4m3 = [()]
         load()
         assert m._e4m3 is None
+
+
+def test_dropped_eight_bit_copies_are_named(hip_lib):
+    """Where 8-bit weights go, a warning says that the 16-bit ones serve from there; nothing is said where there were none."""
+    import warnings
+    from aether_amd.text_encoder import AetherTextEncoder
+    m = AetherTextEncoder(dict(vocab_size=32, d_model=128, num_heads=2, d_ff=128, num_layers=1), device="cpu")
+    sd = {"shared.weight": m.embedding, "encoder.block.0.layer.0.SelfAttention.relative_attention_bias.weight": m.bias_table, "encoder.final_layer_norm.weight": m.final_norm}
+    b, inner = m.blocks[0], 128
+    sd.update({f"encoder.block.0.layer.0.SelfAttention.{n}.weight": b.qkv[i * inner:(i + 1) * inner] for i, n in enumerate("qkv")})
+    sd.update({"encoder.block.0.layer.0.SelfAttention.o.weight": b.out, "encoder.block.0.layer.0.layer_norm.weight": b.norm1, "encoder.block.0.layer.1.layer_norm.weight": b.norm2,
+               "encoder.block.0.layer.1.DenseReluDense.wi_0.weight": b.gate, "encoder.block.0.layer.1.DenseReluDense.wi_1.weight": b.up,
+               "encoder.block.0.layer.1.DenseReluDense.wo.weight": b.down})
+    sd = {k: v.detach().clone() for k, v in sd.items()}
+    for drop in (lambda: m.to("cpu"), lambda: m.load_state_dict(m.state_dict()), lambda: m.load_t5_state_dict(sd), lambda: m.init_random_weights()):
+        m._e4m3 = [()]
+        with pytest.warns(UserWarning, match="quantize_feed_forward"):
+            drop()
+        assert m._e4m3 is None
+        with warnings.catch_warnings():
+            warnings.simplefilter("error")
+            drop()
+    m._e4m3 = [()]
+    with pytest.warns(UserWarning), pytest.raises(KeyError):
+        m.load_t5_state_dict({k: v for k, v in sd.items() if "final" not in k})
+    assert m._e4m3 is None
