@@ -484,8 +484,14 @@ extern "C" int aether_relbias_attn(const AetherRelbias* d, void* o, void* o_low,
     p.nqb = (p.S + nw * 32 - 1) / (nw * 32);
     const dim3 grid((unsigned)((long)p.B * p.H * p.nqb));
     hipStream_t s = (hipStream_t)stream;
+    // ring, table and mask words pass 64 KiB where S, the mask and the reach are all near their limits
 #define RB_LAUNCH(NW, PIPE)                                                                                          \
     do {                                                                                                             \
+        const void* f = lse ? (const void*)relbias_attn_fwd_kernel<NW, true, PIPE> : (const void*)relbias_attn_fwd_kernel<NW, false, PIPE>; \
+        if (lds > 64 * 1024 && hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) { \
+            (void)hipGetLastError();                                                                                 \
+            return aether_set_error(AETHER_ERR_LAUNCH, "relbias_attn: the workgroup's LDS could not be set");        \
+        }                                                                                                            \
         if (lse) hipLaunchKernelGGL((relbias_attn_fwd_kernel<NW, true, PIPE>), grid, dim3(NW * 64), lds, s, args);   \
         else hipLaunchKernelGGL((relbias_attn_fwd_kernel<NW, false, PIPE>), grid, dim3(NW * 64), lds, s, args);      \
     } while (0)

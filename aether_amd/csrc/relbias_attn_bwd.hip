@@ -561,8 +561,10 @@ extern "C" int aether_relbias_attn_bwd(const AetherRelbias* d, const void* go, c
         const size_t lds_k = RB_RING + 1536 + rb_table_bytes(p.reach);
 #define RB_LAUNCH(NW)                                                                                       \
     do {                                                                                                    \
-        if (lds_q > 64 * 1024 && hipFuncSetAttribute((const void*)relbias_attn_dq_kernel<NW>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_q) != hipSuccess) \
+        if (lds_q > 64 * 1024 && hipFuncSetAttribute((const void*)relbias_attn_dq_kernel<NW>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_q) != hipSuccess) { \
+            (void)hipGetLastError();                                                                        \
             return aether_set_error(AETHER_ERR_LAUNCH, "relbias_attn_bwd: the workgroup's LDS could not be set"); \
+        }                                                                                                   \
         hipLaunchKernelGGL((relbias_attn_dq_kernel<NW>), grid, dim3(NW * 64), lds_q, s, args);              \
         rc = aether_check_launch("relbias_attn_dq");                                                        \
         if (rc) return rc;                                                                                  \

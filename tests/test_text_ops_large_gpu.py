@@ -167,3 +167,30 @@ def test_feed_forward_gradients_of_many_rows(cuda, hip_lib, M, K, F):
     _check_ff_gradients(dh, x, wg, wu, gu, got, [0, 63, 64, 65536, 131071, M - 65, M - 64, M - 1], cols)
     frozen = ops.gated_ff_backward(dh, x, wg, wu, gu, need_dw=False)
     assert torch.equal(frozen[0], got[0]) and frozen[1] is None
+
+
+def test_largest_tables_at_the_longest(cuda, hip_lib):
+    """S = 65536 with a mask and a bias that reaches 1020 positions: ring, table and mask words together are more than 64 KiB of LDS.  Rows that are picked out,
+    bound as in test_relbias_attn_gpu.py."""
+    from aether_amd import ops
+    S, nb, far = 65536, 128, 1140
+    assert ops.relbias_borders(nb, far)[-1] == 1020
+    g = torch.Generator().manual_seed(4)
+    qkv = torch.randn(1, S, 3, 1, 64, generator=g)
+    qkv[:, :, :2] *= math.sqrt(0.5)
+    q, k, v = qkv.to(torch.bfloat16).to(cuda).unbind(2)
+    table = (torch.randn(nb, 1, generator=g) * 2).to(torch.bfloat16).to(cuda)
+    mask = torch.ones(1, S, dtype=torch.bool, device=cuda)
+    mask[0, 20000:50000], mask[0, -70:] = False, False
+    of = torch.tensor([bucket(d, nb, far) for d in range(-1100, 1101)], device=cuda)
+    at = torch.arange(S, device=cuda)
+    i = torch.tensor([0, 1, 1000, 19990, 20000, 35000, 49999, 51000, 65400, S - 1], device=cuda)
+    s = q[0, i, 0].double() @ k[0, :, 0].double().t().contiguous() + table[:, 0].double()[of[(at[None, :] - i[:, None]).clamp(-1100, 1100) + 1100]]
+    p = torch.softmax(s.masked_fill(~mask, -math.inf), -1)
+    want, T = p @ v[0, :, 0].double(), p @ v[0, :, 0].double().abs()
+    plain = ops.relbias_attn(q, k, v, table, far, key_mask=mask)
+    train, lse = ops.relbias_attn(q, k, v, table, far, key_mask=mask, need_lse=True)
+    for o in (plain, train):
+        assert bool(((o[0, i, 0].double() - want).abs() <= (BF16 + S32) * T + BF16 * want.abs()).all())
+    got = ops.relbias_attn_backward(o, q, k, v, train, lse, table, far, key_mask=mask)
+    assert all(bool(torch.isfinite(t.float()).all()) for t in got) and not got[1][0, 20000:50000].any()
