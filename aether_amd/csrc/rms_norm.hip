@@ -445,7 +445,7 @@ extern "C" int aether_rms_norm_bwd(const void* dy, long lddy, const void* res, i
 }
 
 extern "C" int aether_quantize_rows_e4m3(const void* x, long ldx, void* q, long ldq, float* scale, int rows, int K, void* stream) {
-    if (rows < 0 || rows > (1 << 30) || K <= 0 || K % 8 != 0) return aether_set_error(AETHER_ERR_SHAPE, "quantize_rows: K must be a positive multiple of 8, rows in [0, 2^30]");
+    if (rows < 0 || rows > (1 << 30) || K <= 0 || K % 8 != 0 || K > (1 << 30)) return aether_set_error(AETHER_ERR_SHAPE, "quantize_rows: K must be a positive multiple of 8 up to 2^30, rows in [0, 2^30]");
     if (rows == 0) return AETHER_OK;
     if (!x || !q || !scale) return aether_set_error(AETHER_ERR_ARG, "quantize_rows: null operand");
     if (ldx % 8 || ldq % 8 || ((uintptr_t)x & 15) || ((uintptr_t)q & 7)) return aether_set_error(AETHER_ERR_ALIGN, "quantize_rows: rows must be 16-byte (x) and 8-byte (q) aligned");

@@ -142,7 +142,7 @@ int aether_rms_norm(const void* x, int x_dtype, long ldx, const void* delta, lon
 size_t aether_rms_norm_bwd_workspace_bytes(int rows, int D);
 int aether_rms_norm_bwd(const void* dy, long lddy, const void* res, int x_dtype, long ldr, const void* delta, long ldd, const void* dres, long lddr,
                         const float* w, float eps, void* dx, long lddx, void* ddelta, long ldds, float* dw, int rows, int D, void* workspace, size_t workspace_bytes, void* stream);
-/* q = e4m3(x / scale) with one power of two per row, chosen as above.  x bf16 [rows, K], K % 8 == 0. */
+/* q = e4m3(x / scale) with one power of two per row, chosen as above.  x bf16 [rows, K], K % 8 == 0, rows and K up to 2^30. */
 int aether_quantize_rows_e4m3(const void* x, long ldx, void* q, long ldq, float* scale, int rows, int K, void* stream);
 
 /* Self-attention with a learned bias by bucket of the relative position, head_dim 64:

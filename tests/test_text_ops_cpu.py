@@ -229,3 +229,9 @@ def test_gated_ff_refuses_projections_that_have_no_backward_pass(hip_lib, kw):
     assert rc == -2 and text in hip_lib.aether_last_error()
     rc = hip_lib.aether_gated_ff(a["x"], a["ldx"], a["wg"], a["wu"], a["ldw"], a["h"], a["ldh"], 4096, a["M"], a["F"], a["K"], 0, None)
     assert rc == -2 and text in hip_lib.aether_last_error()
+
+
+@pytest.mark.parametrize("K,code", [(0x7ffffff8, -2), ((1 << 30) + 8, -2), (1 << 30, -1)])
+def test_quantize_rows_refuses_what_its_counter_does_not_hold(hip_lib, K, code):
+    """The kernel counts a row's elements in 32 bits, 2048 at a time: K ends at 2^30.  (-1: as far as the missing operand.)"""
+    assert hip_lib.aether_quantize_rows_e4m3(None, K, 4096, K, 4096, 4, K, None) == code
