@@ -46,8 +46,17 @@ def source_digest() -> str:
     return h.hexdigest()[:16]
 
 
+def _recipe() -> str:
+    """What a library was built with besides its sources' text: compiler, flags, which sources there were."""
+    return "\n".join([HIPCC, *FLAGS, *(s.name for s in _sources())])
+
+
+def _recipe_file() -> Path:
+    return CSRC / "build" / "recipe.txt"
+
+
 def _stale() -> bool:
-    if not LIB.exists():
+    if not LIB.exists() or not _recipe_file().exists() or _recipe_file().read_text() != _recipe():
         return True
     t = LIB.stat().st_mtime
     deps = list(_sources()) + list(CSRC.glob("*.hpp")) + [CSRC.parent.parent / "include" / "aether_hip.h"]
@@ -75,6 +84,7 @@ def build_native(force: bool = False, verbose: bool = False) -> Path:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    _recipe_file().write_text(_recipe())
     if verbose:
         print(f"built {LIB} from {len(srcs)} sources", file=sys.stderr)
     return LIB
