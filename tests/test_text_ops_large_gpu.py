@@ -194,3 +194,57 @@ def test_largest_tables_at_the_longest(cuda, hip_lib):
         assert bool(((o[0, i, 0].double() - want).abs() <= (BF16 + S32) * T + BF16 * want.abs()).all())
     got = ops.relbias_attn_backward(o, q, k, v, train, lse, table, far, key_mask=mask)
     assert all(bool(torch.isfinite(t.float()).all()) for t in got) and not got[1][0, 20000:50000].any()
+
+
+def test_table_gradient_at_the_longest(cuda, hip_lib):
+    """S = 65536, masked tiles in between: the table's gradient.  Near buckets, entry by entry: dS is off by E of test_relbias_attn_backward_gpu.py without its rounding
+    (near dS are summed in fp32), the entry by 2^-8.  Of the far ones, two sums over half a million keys each whose terms nearly cancel, the sum of all E says nothing:
+    their errors are independent from row to row, and what remains is the rounding of the result, 2^-9 in the norm as in test_far_buckets_of_long_rows."""
+    from aether_amd import ops
+    S, near = 65536, 91
+    g = torch.Generator().manual_seed(12)
+    qkv = torch.randn(1, S, 3, 1, 64, generator=g)
+    qkv[:, :, :2] *= math.sqrt(0.5)
+    q, k, v = qkv.to(torch.bfloat16).to(cuda).unbind(2)
+    table = (torch.randn(32, 1, generator=g) * 2).to(torch.bfloat16).to(cuda)
+    do = torch.randn(1, S, 1, 64, generator=g).to(torch.bfloat16).to(cuda)
+    mask = torch.ones(1, S, dtype=torch.bool, device=cuda)
+    mask[0, 30000:41000], mask[0, 50010:50100], mask[0, -3:] = False, False, False
+    o, lse = ops.relbias_attn(q, k, v, table, key_mask=mask, need_lse=True)
+    got = ops.relbias_attn_backward(do, q, k, v, o, lse, table, key_mask=mask)[3][:, 0].double()
+
+    qd, kd, vd, gd = (t[0, :, 0].double() for t in (q, k, v, do))
+    kt, vt, va = kd.t().contiguous(), vd.t().contiguous(), vd.abs()
+    of = torch.tensor([bucket(d, 32, 128) for d in range(-200, 201)], device=cuda)
+    td, at = table[:, 0].double(), torch.arange(S, device=cuda)
+    assert int(of[200 - near]) == 15 and int(of[200 + near]) == 31 and int(of[200 - near + 1]) == 14 and int(of[200 + near - 1]) == 30
+    want, lim = torch.zeros(32, dtype=torch.float64, device=cuda), torch.zeros(32, dtype=torch.float64, device=cuda)
+    band = torch.arange(1 - near, near, device=cuda)
+    for at0 in range(0, S, 1024):
+        i = at[at0:at0 + 1024]
+        d = at[None, :] - i[:, None]
+        s = (qd[i] @ kt) + td[of[d.clamp(-200, 200) + 200]]
+        p = torch.softmax(s.masked_fill_(~mask, -math.inf), -1)
+        dP = gd[i] @ vt
+        delta = (p * dP).sum(-1, keepdim=True)
+        ds = p * (dP - delta)
+        want[15] += (ds * (d <= -near)).sum()
+        want[31] += (ds * (d >= near)).sum()
+        j = i[:, None] + band[None, :]
+        ok, jc = (j >= 0) & (j < S), j.clamp(0, S - 1)
+        D = (gd[i].abs() * (2.0 ** -16 + S32) * (p @ va)).sum(-1, keepdim=True)
+        pick = lambda t: torch.gather(t, 1, jc) * ok  # noqa: E731
+        pj, dj = pick(p), pick(dP)
+        dPa = (gd[i].abs()[:, None, :] * va[jc]).sum(-1)
+        E = pj * (S32 * (dj.abs() + delta.abs()) + D + 66 * 2.0 ** -24 * dPa)
+        b = of[band + 200].expand(len(i), -1).reshape(-1)
+        want.index_add_(0, b, pick(ds).reshape(-1))
+        lim.index_add_(0, b, E.reshape(-1))
+    few = torch.ones(32, dtype=torch.bool, device=cuda)
+    few[15] = few[31] = False
+    few[16] = False                                           # no pair has it: distance 0 is of the other side
+    err = (got - want).abs()
+    print("near", err[few].max().item(), lim[few].min().item(), want[few].abs().median().item(), "far", err[~few].tolist(), want[~few].tolist())
+    assert bool((err[few] <= lim[few] + BF16 * want[few].abs()).all()) and got[16] == 0
+    assert bool((lim[few] < 0.5 * want[few].abs().max()).all()), "a gradient of zeros does not pass"
+    assert (got - want).norm() <= 2.0 ** -9 * want.norm()
