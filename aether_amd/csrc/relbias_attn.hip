@@ -1,6 +1,6 @@
 // Self-attention with a learned bias by bucket of the relative position, forward pass, head dimension 64:
 //
-//   S_ij = scale · q_i·k_j + T[bucket(j − i), h]  where key j counts,   P = softmax_j(S),   O = P V;   a row without keys gives 0.
+//   S_ij = scale · q_i·k_j + T[bucket(j − i), h]  where key j counts,   P = softmax_j(S),   O = P V;   a row without keys gives 0, and one whose keys all score −inf.
 //
 // gfx950 design
 //   * A wave owns 32 queries, a workgroup NW waves of one (batch, head); tiles of 64 keys, K and V by 16-byte LDS-DMA into a ring of three, one barrier a tile.
@@ -402,7 +402,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(PIPE ||
     } else sweep(0, true);
     // ---- epilogue: O[b][q][h][d], d = 32dt + 8(r >> 2) + 4hi + (r & 3) ----
     const float l_tot = l_run + __shfl_xor(l_run, 32, 64);
-    const float inv = started ? 1.0f / l_tot : 0.f;
+    const float inv = started && l_tot != 0.f ? 1.0f / l_tot : 0.f;   // (a sum of 0: the keys that count all score -inf)
     const size_t at = (((size_t)b * S + min(qrow, S - 1)) * p.H + h) * RB_D;
     if constexpr (TRAIN) {
         if (hi == 0 && qrow < S) {            // +inf: the backward pass gets P = 0 everywhere in such a row; beyond 2^20 a log-sum's digits do not tell P any more

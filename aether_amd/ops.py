@@ -337,8 +337,8 @@ def _relbias(name, q, k, v, table, max_distance, scale, key_mask):
 def relbias_attn(q, k, v, table, max_distance=128, scale=1.0, key_mask=None, need_lse=False):
     """Self-attention with a learned bias by relative position: S_ij = scale q_i·k_j + table[bucket(j − i), h], O = softmax(S) V over the keys that count.
     q, k, v bfloat16 [B, S, H, 64] (views of a packed projection included), table bfloat16 [num_buckets, H] (buckets of both directions, exact up to
-    num_buckets / 4, logarithmic up to max_distance), key_mask bool [B, S], True where a key counts.  A row without keys gives 0; what stands at
-    keys that do not count reaches nothing.  |v| up to 1e22: weighted sums are held in float32 before they are normalized.
+    num_buckets / 4, logarithmic up to max_distance), key_mask bool [B, S], True where a key counts.  A row without keys gives 0, also where buckets
+    at -inf leave none; what stands at keys that do not count reaches nothing.  |v| up to 1e22: weighted sums are held in float32 before they are normalized.
     -> o bfloat16 [B, S, H, 64]; with need_lse (o, lse), where lse (float32, flat) is what
     `relbias_attn_backward` needs besides o: the rows' log-sums to base 2 [B, H, S], then, from the next 16 bytes on, o's rounding remainders
     (bfloat16 [B, S, H, 64]).  P then multiplies v in two parts, and o is a little more exact than without."""

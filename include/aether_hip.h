@@ -153,7 +153,8 @@ int aether_quantize_rows_e4m3(const void* x, long ldx, void* q, long ldq, float*
  * S <= 32, 2^25 for S <= 64, B·H·⌈S / 128⌉ below 2^24 above (one launch).
  * table bf16 [num_buckets, H]; mask: bytes [B, S] with batch stride mask_sb, 0 = the key does not count, or NULL.  What stands at a key that does not
  * count (NaN, infinities) reaches no output.  scale is 0 or of a magnitude in [1e-20, 1e20]; |v| up to 1e22 (weighted sums are held in fp32 before they are
- * normalized); table entries of -inf or the lowest value switch a bucket off. */
+ * normalized); table entries of -inf or the lowest value switch a bucket off; a row whose counted keys all score -inf gives 0, as one without keys.
+ * (Where all are at the lowest value they are equal, and the row is their mean.) */
 typedef struct AetherRelbias {
     const void* q; const void* k; const void* v;
     long q_strides[3], k_strides[3], v_strides[3];

@@ -372,3 +372,33 @@ def test_row_sums_next_to_the_largest_float(cuda, hip_lib, S, apart):
     pt, gd = p.transpose(2, 3).contiguous(), do.double().permute(0, 2, 1, 3).contiguous()
     want, lim = torch.matmul(pt, gd).permute(0, 2, 1, 3), (BF16 + 2.0 ** -10) * torch.matmul(pt, gd.abs()).permute(0, 2, 1, 3)
     assert bool(((dv.double() - want).abs() <= lim + BF16 * want.abs() + 1e-30).all())
+
+
+@pytest.mark.parametrize("S", [1, 40, 70, 500, 1030])
+def test_rows_whose_buckets_are_all_switched_off(cuda, hip_lib, S):
+    """A row is without keys too where the mask and buckets at −inf leave none together: 0, and no gradient through it.  Here rows see no key to their right, and the
+    second item is padded in front."""
+    from aether_amd import ops
+    n = min(25, S - 1)
+    qkv, table = inputs(2, S, 2, device=cuda, seed=23)
+    table[table.shape[0] // 2:] = -math.inf
+    q, k, v = qkv.unbind(2)
+    do = torch.randn(q.shape, generator=torch.Generator().manual_seed(S)).to(torch.bfloat16).to(cuda)
+    mask = torch.ones(2, S, dtype=torch.bool, device=cuda)
+    mask[1, :n] = False
+    o = ops.relbias_attn(q, k, v, table, key_mask=mask)
+    o2, lse = ops.relbias_attn(q, k, v, table, key_mask=mask, need_lse=True)
+    assert not o[1, :n].any() and not o2[1, :n].any() and bool(torch.isposinf(lse[:2 * S * 2].view(2, 2, S)[1, :, :n]).all())
+    for got in (o, o2):
+        assert bool(torch.isfinite(got.float()).all())
+        alone = ops.relbias_attn(q[1:, n:], k[1:, n:], v[1:, n:], table)
+        assert bool(((got[1, n:].double() - alone[0].double()).norm() <= 2 * BF16 * alone.double().norm()))
+    grads = ops.relbias_attn_backward(do, q, k, v, o2, lse, table, key_mask=mask)
+    assert all(bool(torch.isfinite(t.float()).all()) for t in grads) and not any(t[1, :n].any() for t in grads[:3])
+    a, l = ops.relbias_attn(q[1:, n:], k[1:, n:], v[1:, n:], table, need_lse=True)
+    for x, y in zip(grads[:3], ops.relbias_attn_backward(do[1:, n:], q[1:, n:], k[1:, n:], v[1:, n:], a, l, table)):
+        assert bool((x[1, n:].double() - y[0].double()).norm() <= 4 * BF16 * y.double().norm())
+    # every bucket off: nothing anywhere
+    off = torch.full_like(table, -math.inf)
+    o, lse = ops.relbias_attn(q, k, v, off, need_lse=True)
+    assert not o.any() and not any(t.any() for t in ops.relbias_attn_backward(do, q, k, v, o, lse, off))
