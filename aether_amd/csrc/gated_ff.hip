@@ -9,8 +9,8 @@
 // Main loop: 8 waves as WM x WN; a wave owns MT·32 rows and 32 pairs of columns on v_mfma_f32_32x32x16_bf16, or v_mfma_..._32x32x64_f8f6f4 for e4m3.  A K tile is
 // 128 bytes of every row either way.  Tiles come by 16-byte LDS-DMA into two buffers; 128-byte LDS rows are XOR-swizzled in 16-byte chunks.  The two
 // waves that share a SIMD alternate: one reads its next fragments and issues the next tile's DMA while the other feeds the matrix pipe.
-// Measured, F = 10240, K = 4096: 14464 rows in e4m3 940 µs, 2580 TFLOP/s (a large library product in 8 bits: 2440); 3616 rows in bf16, writing both projections,
-// 620 ... 660 µs, 940 TFLOP/s (library 1390; of these, 75 µs are the projections' 296 MB).
+// Measured, F = 10240, K = 4096: 14464 rows in e4m3 930 ... 963 µs, 2520 ... 2610 TFLOP/s (a large library product in 8 bits: 2440); 3616 rows in bf16 500 µs, 1210 TFLOP/s
+// (library 1390), and 610 µs writing both projections, 296 MB.
 #include <algorithm>
 #include <type_traits>
 #include "common.hpp"
@@ -310,9 +310,9 @@ __global__ __launch_bounds__(256) void gated_ff_rows_kernel(FfArgs p) {
 
 // ---- some rows: small tiles ------------------------------------------------------------------------------------------------------------------------
 // 4 or 8 waves as WM x WN over (WM MT 32) rows x (WN 32) pairs of columns; a ring of NS tiles, one barrier a tile.
-// Measured, F = 10240, K = 4096 (168 MB of weights): one row 33 µs, 5.1 TB/s, bound by reading them; 226 rows 58 µs, 2.9 TB/s: there every workgroup reads x too, and
-// what all of them take out of the L2s, 8 TB/s of tiles, is the bound (80 workgroups of this size go through a K tile in 0.5 µs, 160 in 0.9).  Tried at 226 rows without
-// gain: rings of 2 ... 6 tiles for the weights with loading waves of their own, and 256 x 48 tiles, so that 214 CUs share the work (57 µs).
+// Measured, F = 10240, K = 4096 (168 MB of weights): one row 33 µs, 5.1 TB/s, bound by reading them; 226 rows 59 µs, 2.8 TB/s: one round of 160
+// workgroups, which leaves 96 CUs idle and reads x in every one (80 workgroups of this size go through a K tile in 0.5 µs, 160 in 0.9: 8 TB/s of tiles out of the L2s, where the kernel above takes 10 with
+// larger tiles).  K split over the idle CUs is not built.  Tried at 226 rows without gain: rings of 2 ... 6 tiles for the weights with loading waves of their own, and 256 x 48 tiles, so that 214 CUs share the work (57 µs).
 template <class ET, int WM, int WN, int MT, int NS, int ACT>
 __global__ __launch_bounds__(WM * WN * 64) void gated_ff_small_kernel(FfArgs p) {
     constexpr int NW = WM * WN;
@@ -400,7 +400,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gated_ff_small_kernel(FfArgs p) 
 }
 
 // ---- backward ------------------------------------------------------------------------------------------------------------------------------
-// dg = dh u act'(g), du = dh act(g), as [M][2F] for the product with the weights and transposed, [2F][Mp], for the one with x.  A workgroup turns a
+// dg = dh u act'(g), du = dh act(g), each rounded to bf16 once, as the products' operands (error of the gradients against 64 bits 0.0023, the outputs' own rounding 0.0017), as [M][2F] for the product with the weights and transposed, [2F][Mp], for the one with x.  A workgroup turns a
 // 64 x 64 piece through LDS.  Columns M ... Mp − 1 of the transposed form are zeros.
 template <int ACT>
 __global__ __launch_bounds__(256) void gated_ff_dgu_kernel(const float* __restrict__ gu, const bf16_t* __restrict__ dh, long lddh, int M, int F, int Mp,
@@ -630,6 +630,7 @@ static int ff_bwd_check(int M, int F, int K) {
 // K tile of 128 bytes (K = 4096, F = 1024 ... 10240, µs): 64 x 64 (rows x pairs of columns) 0.42, 128 x 64 0.6, 128 x 128 and 256 x 64 0.9, the 256 x 128
 // kernel with alternating waves 1.45.  The least rounds x time wins; for instance, bf16, F = 10240: 64 rows 36 µs (256 x 128: 91), 128 rows 44 (91), 226 rows
 // 58 (92), 300 rows 64 (96), 400 rows 95 with 256 x 128 (the others 110 and more), 1024 rows 184 (199), 2048 rows 300.
+// The same times choose for e4m3, whose K tile holds twice the depth: only their ratios count there, and they were not measured for it (F = 10240, K = 4096, µs: 1 row 15, 226 rows 31, 400 rows 41).
 // The kernel without tiles splits K over its waves and needs no round: up to 32 rows it is ahead where F / 64 workgroups of the smallest tile leave most CUs
 // idle (F = 2048, K = 4096: 1 row 12 µs against 23, 32 rows 18.5 against 23.5; F = 8192, K = 2048: 16 rows 14.5 against 15.3, 32 rows 18.6 against 15.6).
 enum FfVariant { FF_ROWS_16, FF_ROWS_32, FF_64X64, FF_128X64, FF_128X128, FF_256X64, FF_256X128 };

@@ -14,7 +14,7 @@
 // WPR waves share a row (1 up to 1024 elements, 4 above), NCH chunks of 8 elements a lane: D <= WPR·64·8·NCH.
 //
 // Measured (a large copy on this card moves 4.9 TB/s): 14464 x 4096, fp32 stream with delta, e4m3 out: 652 MB in 124 µs, 5.3 TB/s; 3616 x 4096 forward and backward:
-// 415 MB in 79 µs, 5.3 TB/s; 226 x 4096: 11 µs, what a call costs on the host (the kernel itself 4).
+// 415 MB in 79 µs, 5.3 TB/s; 226 x 4096: 10.6 µs, what a call costs on the host (the kernel itself 4.4).
 #include "common.hpp"
 #include "../../include/aether_hip.h"
 
@@ -317,7 +317,7 @@ __global__ __launch_bounds__(1024) void rms_norm_dw_kernel(const float* __restri
 }
 
 // q = e4m3(x / s), s per row as in the norm above: the form in which gated_ff takes a weight matrix in 8 bits.  One workgroup per row, two passes
-// over it (the second hits the caches); run once when weights are laid out.  A grid of 2^32 threads or more
+// over it (the second hits the caches); run once when weights are laid out: 10240 x 4096 in 25 µs, 126 MB at 5.0 TB/s.  A grid of 2^32 threads or more
 // is cut short without an error, so a workgroup of a large matrix takes several rows.
 constexpr int QUANT_WG = 1 << 20;
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const bf16_t* __restrict__ x, long ldx, u8_t* __restrict__ q, long ldq, float* __restrict__ scale, int rows, int K) {
@@ -363,7 +363,8 @@ static int rms_check(const void* x, int x_dtype, long rows, int D, const char* w
 using namespace aether;
 
 // D -> waves per row and chunks per lane: one wave up to 1024 elements (no barrier), four above.  3616 rows, fp32: forward 5.1 ... 6.5 TB/s at 4096 ... 16384
-// elements; backward 5.0 at 4096, 4.7 at 8192, 3.3 above, where a lane's 64 elements of six vectors no longer fit its registers.
+// elements; backward 5.0 at 4096, 4.7 at 8192, 3.3 above, where a lane of four waves a row holds 64 elements of six vectors, more than its registers
+// (eight waves a row are not built).
 #define RMS_PICK(D, CALL)                     \
     do {                                      \
         if ((D) <= 512) { CALL(1, 1); }       \
