@@ -310,9 +310,10 @@ __global__ __launch_bounds__(256) void gated_ff_rows_kernel(FfArgs p) {
 
 // ---- some rows: small tiles ------------------------------------------------------------------------------------------------------------------------
 // 4 or 8 waves as WM x WN over (WM MT 32) rows x (WN 32) pairs of columns; a ring of NS tiles, one barrier a tile.
-// Measured, F = 10240, K = 4096 (168 MB of weights): one row 33 µs, 5.1 TB/s, bound by reading them; 226 rows 59 µs, 2.8 TB/s: one round of 160
-// workgroups, which leaves 96 CUs idle and reads x in every one (80 workgroups of this size go through a K tile in 0.5 µs, 160 in 0.9: 8 TB/s of tiles out of the L2s, where the kernel above takes 10 with
-// larger tiles).  K split over the idle CUs is not built.  Tried at 226 rows without gain: rings of 2 ... 6 tiles for the weights with loading waves of their own, and 256 x 48 tiles, so that 214 CUs share the work (57 µs).
+// Measured, F = 10240, K = 4096 (168 MB of weights): one row 33 µs, 5.1 TB/s, bound by reading them; 226 rows 59 µs, 2.8 TB/s: one round of 160 workgroups, which
+// leaves 96 CUs idle and reads x in every one (80 workgroups of this size go through a K tile in 0.5 µs, 160 in 0.9: 8 TB/s of tiles out of the L2s, where the
+// kernel above takes 10 with larger tiles).  K split over the idle CUs is not built.  Tried at 226 rows without gain: rings of 2 ... 6 tiles for the weights with
+// loading waves of their own, and 256 x 48 tiles, so that 214 CUs share the work (57 µs).
 template <class ET, int WM, int WN, int MT, int NS, int ACT>
 __global__ __launch_bounds__(WM * WN * 64) void gated_ff_small_kernel(FfArgs p) {
     constexpr int NW = WM * WN;
@@ -400,8 +401,9 @@ __global__ __launch_bounds__(WM * WN * 64) void gated_ff_small_kernel(FfArgs p) 
 }
 
 // ---- backward ------------------------------------------------------------------------------------------------------------------------------
-// dg = dh u act'(g), du = dh act(g), each rounded to bf16 once, as the products' operands (error of the gradients against 64 bits 0.0023, the outputs' own rounding 0.0017), as [M][2F] for the product with the weights and transposed, [2F][Mp], for the one with x.  A workgroup turns a
-// 64 x 64 piece through LDS.  Columns M ... Mp − 1 of the transposed form are zeros.
+// dg = dh u act'(g), du = dh act(g), each rounded to bf16 once, as the products' operands (error of the gradients against 64 bits 0.0023, the outputs' own rounding
+// 0.0017), as [M][2F] for the product with the weights and transposed, [2F][Mp], for the one with x.  A workgroup turns a 64 x 64 piece through LDS.  Columns
+// M ... Mp − 1 of the transposed form are zeros.
 template <int ACT>
 __global__ __launch_bounds__(256) void gated_ff_dgu_kernel(const float* __restrict__ gu, const bf16_t* __restrict__ dh, long lddh, int M, int F, int Mp,
                                                            bf16_t* __restrict__ dgu, bf16_t* __restrict__ dgut) {
